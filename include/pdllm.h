@@ -419,6 +419,77 @@ int pdllm_denoise_unmask_static(const void* logits, int64_t logits_stride, const
                                 int32_t* n_masked_left, pdllm_stream_t stream);
 
 /* ------------------------------------------------------------------------- *
+ * The vocabulary head: from hidden states, without logits in memory          *
+ * ------------------------------------------------------------------------- */
+
+/* The head's logits z = hidden weight^T are formed tile by tile on the matrix cores (bf16 products, fp32 sums) and
+ * reduced where they are made; they are not rounded to bf16.  hidden [n_rows, dim], weight [vocab, dim] bf16, row strides in
+ * elements and multiples of 8, bases 16-byte aligned, dim a multiple of 8 (at most 2^20), weight_stride below 2^22,
+ * n_rows <= 2^24, vocab <= 2^30.  workspace: 16-byte aligned. */
+int64_t pdllm_head_workspace_bytes(int64_t n_rows, int64_t vocab);
+
+/* pdllm_selfinfo_logprob (ENG:1148-1152) from the states: logp[r] = log softmax(z[r])[label[r]], computed as
+ * -log(1 + exp(L - z[r, label])) with L the log-sum of the other entries, so that a label that is all but certain keeps
+ * the digits of 1 - p.  lse_out (may be NULL): log sum exp of the row.  A label outside [0, vocab) yields -inf. */
+int pdllm_head_selfinfo_logprob(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
+                                const int64_t* labels, int64_t n_rows, int64_t vocab, int32_t dim, void* workspace,
+                                int64_t workspace_bytes, float* logp_out, float* lse_out, pdllm_stream_t stream);
+
+/* Gradients of sum_r grad_logp[r] * logp[r] with respect to hidden and weight, from logp and lse as
+ * pdllm_head_selfinfo_logprob gave them for the same inputs: with d[r, v] = grad_logp[r] * ([v == label[r]] - p[r, v]),
+ * grad_hidden = d weight and grad_weight = d^T hidden (bf16, every element written).  Rows whose label lies outside
+ * [0, vocab) have no gradient and add nothing to grad_weight, whatever their states hold.  The vocabulary is taken in
+ * pieces: the piece of d (bf16) lies in the workspace.  With the bytes the query returns a piece is up to 256 MB; a smaller
+ * workspace makes the pieces shorter (PDLLM_ERR_WORKSPACE where not even 256 entries fit).  d is rounded to bf16; up to 64
+ * rows a second bf16 plane carries the remainder.  workspace: 256-byte aligned; gradient strides multiples of 4, their
+ * bases 8-byte aligned.  n_rows == 0 clears grad_weight.  Same bits on every call. */
+int64_t pdllm_head_selfinfo_grad_workspace_bytes(int64_t n_rows, int64_t vocab, int32_t dim);
+int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
+                             const int64_t* labels, const float* logp, const float* lse, const float* grad_logp,
+                             int64_t n_rows, int64_t vocab, int32_t dim, void* workspace, int64_t workspace_bytes,
+                             void* grad_hidden, int64_t grad_hidden_stride, void* grad_weight, int64_t grad_weight_stride,
+                             pdllm_stream_t stream);
+
+/* pdllm_conf_argmax (ENG:1647-1681) from the states: row i of block b uses state row b*block_len + i, or with shift the
+ * row before it: for i = 0 last_hidden[b] (the state in front of the block; the block's own row 0 when NULL).
+ * Confidence = max softmax probability, token = first index of the largest logit (of the fp32 logits: where two round
+ * to the same bf16 value, pdllm_conf_argmax sees a tie and this call does not).  A row whose logits are all NaN: token 0. */
+int pdllm_head_conf_argmax(const void* hidden, int64_t hidden_stride, const void* last_hidden, int64_t last_hidden_stride,
+                           const void* weight, int64_t weight_stride, int64_t n_seqs, int64_t block_len, int64_t vocab,
+                           int32_t dim, int32_t shift, void* workspace, int64_t workspace_bytes, float* conf_out,
+                           int64_t* token_out, pdllm_stream_t stream);
+
+/* pdllm_denoise_unmask from the states: pdllm_head_conf_argmax, then the transfer rule of pdllm_threshold_unmask. */
+int pdllm_head_denoise_unmask(const void* hidden, int64_t hidden_stride, const void* last_hidden, int64_t last_hidden_stride,
+                              const void* weight, int64_t weight_stride, int64_t n_seqs, int64_t block_len, int64_t vocab,
+                              int32_t dim, int32_t shift, int64_t* block_ids, int64_t mask_token_id, float threshold,
+                              void* workspace, int64_t workspace_bytes, float* conf_out, int64_t* token_out,
+                              uint8_t* transfer_out, int32_t* n_masked_left, pdllm_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * Products with 8-bit operands and a scale for each block of 128              *
+ * ------------------------------------------------------------------------- */
+
+/* Quantisation of bf16 [n_rows, k] to e4m3 (OCP) with one scale for each row and 128 columns (rows) or for each block of
+ * 128 x 128 (blocks): s = the smallest power of two with amax / s <= 448 (1 for a block of zeros; not below 2^-126), q = x / s
+ * rounded to nearest even.  A block that holds an infinity or a NaN gets the scale NaN.  scale[r * row_stride +
+ * b * block_stride], r = row (rows) or row / 128 (blocks), b = column / 128.  k a multiple of 16 (at most 2^20), strides in
+ * elements: x_stride a multiple of 8, q_stride of 16; x and q 16-byte aligned. */
+int pdllm_fp8_quantize_rows(const void* x, int64_t x_stride, int64_t n_rows, int32_t k, void* q, int64_t q_stride,
+                            float* scale, int64_t scale_row_stride, int64_t scale_block_stride, pdllm_stream_t stream);
+int pdllm_fp8_quantize_blocks(const void* w, int64_t w_stride, int64_t n_rows, int32_t k, void* q, int64_t q_stride,
+                              float* scale, int64_t scale_row_stride, int64_t scale_block_stride, pdllm_stream_t stream);
+
+/* out[i, j] = sum_b x_scale[i, b] * weight_scale[j / 128, b] * sum_{c in block b} x[i, c] * weight[j, c] for e4m3 x [m, k]
+ * and weight [n, k] (rows contiguous, strides in elements, multiples of 16, below 2^23; bases 16-byte aligned), blocks of 128
+ * columns, any fp32 scales; out bf16.  Sums in fp32, apart from those of eight neighbouring products, which the matrix
+ * instruction adds on a grid of 2^-13 of the largest of them.  k a multiple of 16 (at most 2^20), m <= 2^24, n <= 2^30.  Same bits on every call. */
+int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_scale, int64_t x_scale_row_stride,
+                     int64_t x_scale_block_stride, const void* weight, int64_t weight_stride, const float* weight_scale,
+                     int64_t weight_scale_row_stride, int64_t weight_scale_block_stride, int64_t m, int64_t n, int32_t k,
+                     void* out, int64_t out_stride, pdllm_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
  * Rotary embedding (the step in front of the path)                           *
  * ------------------------------------------------------------------------- */
 

@@ -91,6 +91,16 @@ SIGNATURES = {
     "pdllm_denoise_unmask_static": (C.c_int, [vp, i64, vp, i64, i64, i64, i64, i32, vp, i64, f32, vp, vp, vp, vp, vp]),
     "pdllm_chunk_select": (C.c_int, [vp, i64, vp, i64, i64, i64, i32, i64, i32, vp, i64, vp, vp, vp, vp]),
     "pdllm_rope_inplace": (C.c_int, [vp, i64, vp, vp, i64, i64, i32, i32, vp]),
+    "pdllm_head_workspace_bytes": (i64, [i64, i64]),
+    "pdllm_head_selfinfo_logprob": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, i32, vp, i64, vp, vp, vp]),
+    "pdllm_head_selfinfo_grad_workspace_bytes": (i64, [i64, i64, i32]),
+    "pdllm_head_selfinfo_grad": (C.c_int, [vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, i32, vp, i64, vp, i64, vp, i64, vp]),
+    "pdllm_head_conf_argmax": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, i64, i64, i32, i32, vp, i64, vp, vp, vp]),
+    "pdllm_head_denoise_unmask": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, i64, i64, i32, i32, vp, i64, f32, vp, i64, vp, vp,
+                                            vp, vp, vp]),
+    "pdllm_fp8_quantize_rows": (C.c_int, [vp, i64, i64, i32, vp, i64, vp, i64, i64, vp]),
+    "pdllm_fp8_quantize_blocks": (C.c_int, [vp, i64, i64, i32, vp, i64, vp, i64, i64, vp]),
+    "pdllm_fp8_linear": (C.c_int, [vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, i64, i64, i32, vp, i64, vp]),
     "pdllm_anchor_delta_add": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, vp, vp, i64, vp, i64, i64, i64, i64, i32, i32,
                                          i32, i32, i32, f32, f32, i32, vp]),
 }

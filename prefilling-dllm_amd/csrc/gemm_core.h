@@ -1,0 +1,266 @@
+// The matrix-product loop shared by the vocabulary-head and fp8 kernels for gfx950: one workgroup forms a tile
+// C[m][n] = sum_k A[m][k] B[n][k] on the matrix cores, fp32 accumulation.
+//
+// Orientation.  A is the operand whose index is contiguous in the output (vocabulary entries, output features, state
+// columns), B the one over rows (tokens): in the 32x32 result layout a lane then owns ONE row of the output (lane & 31)
+// and 16 of its columns in registers, so softmax statistics of a row are sums over a lane's own registers and
+// stores are groups of four neighbouring columns.
+//
+// LDS.  A stage holds 128 bytes of k per row of A and of B (64 bf16 or 128 fp8 values).  Operands that lie with k
+// contiguous ("KC") are kept as rows of 128 bytes, 16-byte chunk c of row r at position c ^ ((r >> 1) & 7): 16
+// consecutive rows of one chunk cover all 64 banks.  Operands that lie with k as their row index ("KS", bf16 only)
+// are kept as 64 rows of TM * 2 bytes, chunk c of row r at c ^ ((r & 3) << 2), and read through the transposing
+// 64-bit reads (four rows of four neighbouring chunks per half wave, again all banks).  Copies go straight from memory to
+// LDS, ST - 1 stages ahead; operand reads are hand-issued with counted waits so that they do not wait for the copies.
+#pragma once
+
+#include <type_traits>
+
+#include "attn_common.h"
+
+namespace pdllm {
+
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void lgkm_wait() {
+  asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wg_barrier() {
+  asm volatile("s_barrier" ::: "memory");
+}
+
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ lds_void* lds_at(unsigned a) { return (lds_void*)(size_t)a; }
+
+constexpr unsigned kOutOfRange = 0x80000000u;  // an offset behind every buffer (their sizes stay below 2 GiB)
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, unsigned bytes) {
+  // the same in every lane; said explicitly, since 64-bit comparisons on the way leave the scalar registers
+  const uint64_t a = (uint64_t)base;
+  const uint64_t lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a);
+  const uint64_t hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+
+// Rows of k-contiguous data, through a buffer whose size ends with the last valid row: rows and k behind the end read
+// as zero.  L 1-KB copies per wave and stage.
+template <int L>
+struct LoadKC {
+  __amdgpu_buffer_rsrc_t rs;
+  unsigned off[L], kc[L], kbytes, bytes;
+  __device__ __forceinline__ void init(const void* base, long rows_left, unsigned stride, unsigned kb, int wave, int lane) {
+    const unsigned rows = rows_left <= 0 ? 0u : (rows_left < 4096 ? (unsigned)rows_left : 4096u);
+    bytes = rows ? (rows - 1) * stride + kb : 0u;
+    rs = make_rsrc(base, bytes);
+    kbytes = kb;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const unsigned row = 8 * (wave * L + i) + (lane >> 3);
+      const unsigned c = (lane & 7) ^ ((row >> 1) & 7);
+      kc[i] = 16 * c;
+      off[i] = row < rows ? row * stride + 16 * c : kOutOfRange;
+    }
+  }
+  __device__ __forceinline__ void rebase(const void* base) { rs = make_rsrc(base, bytes); }
+  __device__ __forceinline__ void issue(int t, unsigned dst) const {
+    const unsigned k = 128u * t;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const unsigned o = k + kc[i] < kbytes ? off[i] + k : kOutOfRange;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, o, 0, 0, 0);
+    }
+  }
+};
+
+// Rows of k-contiguous data at a 64-bit address per row (rows gathered from two tensors).  Rows past the end repeat a
+// valid row (their results are dropped); k behind the end repeats the row's first bytes (the other operand is zero
+// there).
+template <int L>
+struct LoadRows {
+  const char* p[L];
+  unsigned kc[L], kbytes;
+  template <typename F>
+  __device__ __forceinline__ void init(F&& row_ptr, unsigned kb, int wave, int lane) {
+    kbytes = kb;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const unsigned row = 8 * (wave * L + i) + (lane >> 3);
+      kc[i] = 16 * ((lane & 7) ^ ((row >> 1) & 7));
+      p[i] = row_ptr(row);
+    }
+  }
+  __device__ __forceinline__ void issue(int t, unsigned dst) const {
+    const unsigned k = 128u * t;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const unsigned o = k + kc[i] < kbytes ? k + kc[i] : 0u;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[i] + o), lds_at(dst + 1024 * i),
+                                       16, 0, 0);
+    }
+  }
+};
+
+// 64 rows of k per stage, W columns (bf16) of each: base = first row, first column.  Rows from k_rows on read as zero;
+// so do columns from col_bytes on.
+template <int L, int W>
+struct LoadKS {
+  const char* base;
+  long stride;   // bytes
+  long k_rows;
+  unsigned off[L], colb;
+  __device__ __forceinline__ void init(const void* b, long stride_bytes, long rows, unsigned col_bytes, int wave, int lane) {
+    constexpr int CH = W / 8;  // chunks per row
+    base = static_cast<const char*>(b);
+    stride = stride_bytes;
+    k_rows = rows;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const unsigned q = 64 * (wave * L + i) + lane;
+      const unsigned row = q / CH, c = (q % CH) ^ ((row & 3) << 2);
+      off[i] = 16 * c < col_bytes ? row * (unsigned)stride_bytes + 16 * c : kOutOfRange;
+    }
+    colb = col_bytes;
+  }
+  __device__ __forceinline__ void issue(int t, unsigned dst) const {
+    const long r0 = 64L * t;
+    const long left = k_rows - r0;
+    const unsigned rows = left <= 0 ? 0u : (left < 64 ? (unsigned)left : 64u);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + r0 * stride, rows ? (rows - 1) * (unsigned)stride + colb : 0u);
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, off[i], 0, 0, 0);
+  }
+};
+
+template <int MT_, int NT_, int WM_, int WN_, int ST_>
+struct Tile {
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, ST = ST_;
+  static constexpr int NW = WM * WN, THREADS = 64 * NW;
+  static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN;
+  static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int LA = A_BYTES / 1024 / NW, LB = B_BYTES / 1024 / NW;
+  static_assert(LA * NW * 1024 == A_BYTES && LB * NW * 1024 == B_BYTES, "every wave copies the same number of pieces");
+  static constexpr int LDS = ST * STAGE;
+  static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
+};
+
+// A wave's operand fragments: N_ blocks of 32 rows (KC) or columns (KS), the first one at `first` of the tile.  A fragment of
+// step ks holds, in lane half h, the k values 16 ks + 8 h .. + 7 (bf16) of its row; for fp8 two fragments make one operand
+// (the k values of both operands are permuted alike, which a sum over k does not see).
+template <int N_, bool KS, int W>
+struct Frag;
+template <int N_, int W>
+struct Frag<N_, false, W> {
+  unsigned a[4];
+  typedef bf16x8 raw;
+  static constexpr int READS = 1;  // LDS operations per fragment
+  __device__ __forceinline__ void init(unsigned lds_base, int first, int lane) {
+    const int l32 = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) a[ks] = lds_base + (first + l32) * 128 + (((2 * ks + h) ^ ((l32 >> 1) & 7)) << 4);
+  }
+  template <int KS_, int J>
+  __device__ __forceinline__ void read(raw& d, unsigned stage) const {
+    lds_read_b128<J * 4096>(d, a[KS_] + stage);
+  }
+  static __device__ __forceinline__ bf16x8 value(const raw& r) { return r; }
+};
+struct TrPair {
+  s16x4 lo, hi;
+};
+template <int N_, int W>
+struct Frag<N_, true, W> {
+  unsigned a[N_];
+  typedef TrPair raw;
+  static constexpr int READS = 2;
+  __device__ __forceinline__ void init(unsigned lds_base, int first, int lane) {
+    const int l32 = lane & 31, h = lane >> 5, i16 = lane & 15, g = l32 >> 4;
+    const int row = 8 * h + (i16 >> 2);
+#pragma unroll
+    for (int j = 0; j < N_; ++j) {
+      const int c = (first + 32 * j) / 8 + 2 * g + ((i16 & 3) >> 1);
+      a[j] = lds_base + row * (W * 2) + ((c ^ ((row & 3) << 2)) << 4) + ((i16 & 1) << 3);
+    }
+  }
+  template <int KS_, int J>
+  __device__ __forceinline__ void read(raw& d, unsigned stage) const {
+    lds_read_tr16_b64<(16 * KS_) * W * 2>(d.lo, a[J] + stage);
+    lds_read_tr16_b64<(16 * KS_ + 4) * W * 2>(d.hi, a[J] + stage);
+  }
+  static __device__ __forceinline__ bf16x8 value(const raw& r) {
+    typedef __attribute__((ext_vector_type(8))) short s16x8;
+    const s16x8 v = __builtin_shufflevector(r.lo, r.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(bf16x8, v);
+  }
+};
+// Ties a wait that has been issued to the registers the reads before it filled: nothing that uses them moves above it.
+__device__ __forceinline__ void tie(bf16x8& r) { asm volatile("" : "+v"(r)::"memory"); }
+__device__ __forceinline__ void tie(TrPair& r) { asm volatile("" : "+v"(r.lo), "+v"(r.hi)::"memory"); }
+
+// The bf16 loop over T stages.  issue(t, lds address of the stage) starts the copies of stage t (T::LA + T::LB per wave);
+// every wave passes one barrier per stage: behind it stage t has landed for all waves and stage t - 1 has been read by all
+// of them, so its buffer takes the copies of stage t + ST - 1.
+template <class T, bool AKS, bool BKS, class Issue>
+__device__ __forceinline__ void mainloop_bf16(f32x16 (&acc)[T::MT][T::NT], int steps, unsigned lds_base, Issue&& issue) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  Frag<T::MT, AKS, T::TM> fa;
+  Frag<T::NT, BKS, T::TN> fb;
+  fa.init(lds_base, wm * T::MT * 32, lane);
+  fb.init(lds_base + T::A_BYTES, wn * T::NT * 32, lane);
+  typename Frag<T::MT, AKS, T::TM>::raw A[2][T::MT];
+  typename Frag<T::NT, BKS, T::TN>::raw B[2][T::NT];
+  constexpr int READS = T::MT * Frag<T::MT, AKS, T::TM>::READS + T::NT * Frag<T::NT, BKS, T::TN>::READS;
+  static_assert(READS <= 15, "the wait counts 15 LDS operations at most");
+#pragma unroll
+  for (int s = 0; s < T::ST - 1; ++s)
+    if (s < steps) issue(s, lds_base + s * T::STAGE);
+  unsigned cur = 0, nxt = (T::ST - 1) * T::STAGE;
+  for (int t = 0; t < steps; ++t) {
+    if (T::ST > 2 && t + T::ST - 2 < steps) vm_wait<(T::ST - 2) * (T::LA + T::LB)>();
+    else vm_wait<0>();
+    wg_barrier();
+    auto read = [&](auto ks_tag, int set) __attribute__((always_inline)) {
+      constexpr int KS = decltype(ks_tag)::value;
+      fb.template read<KS, 0>(B[set][0], cur);
+      if constexpr (T::NT > 1) fb.template read<KS, 1>(B[set][1], cur);
+      fa.template read<KS, 0>(A[set][0], cur);
+      if constexpr (T::MT > 1) fa.template read<KS, 1>(A[set][1], cur);
+      if constexpr (T::MT > 2) fa.template read<KS, 2>(A[set][2], cur);
+      if constexpr (T::MT > 3) fa.template read<KS, 3>(A[set][3], cur);
+    };
+    auto mul = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < T::MT; ++i) tie(A[set][i]);
+#pragma unroll
+      for (int j = 0; j < T::NT; ++j) tie(B[set][j]);
+#pragma unroll
+      for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < T::NT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Frag<T::MT, AKS, T::TM>::value(A[set][i]),
+                                                              Frag<T::NT, BKS, T::TN>::value(B[set][j]), acc[i][j], 0, 0, 0);
+    };
+    read(std::integral_constant<int, 0>{}, 0);
+    if (t + T::ST - 1 < steps) issue(t + T::ST - 1, lds_base + nxt);
+    read(std::integral_constant<int, 1>{}, 1);
+    lgkm_wait<READS>();
+    mul(0);
+    read(std::integral_constant<int, 2>{}, 0);
+    lgkm_wait<READS>();
+    mul(1);
+    read(std::integral_constant<int, 3>{}, 1);
+    lgkm_wait<READS>();
+    mul(0);
+    lgkm_wait<0>();
+    mul(1);
+    cur = cur == (T::ST - 1) * T::STAGE ? 0u : cur + T::STAGE;
+    nxt = nxt == (T::ST - 1) * T::STAGE ? 0u : nxt + T::STAGE;
+  }
+}
+
+}  // namespace pdllm

@@ -1,0 +1,725 @@
+// The vocabulary head for gfx950: z = h w^T from hidden states h [rows, D] and the head's weight w [V, D] (bf16), never
+// written to memory.  Each workgroup forms a tile of logits on the matrix cores (gemm_core.h) and keeps of it what the
+// call needs: the softmax statistics of its rows (maximum, sum, position of the maximum, logit of the label), which a
+// small second kernel joins, or, for the gradient, the tile of softmax gradients that the two products behind it read.
+//
+//   logp[r] = -log(1 + exp(L - z[r, l])),  L = log sum over v != l of exp z[r, v]
+//
+// (the label's own term stays out of the sum: where the model is all but certain, 1 - p keeps its digits).
+//   d[r, v] = -g[r] exp(z[r, v] - lse[r]) (v != l),  d[r, l] = -g[r] expm1(logp[r]);  grad_h = d w,  grad_w = d^T h.
+
+#include "gemm_core.h"
+
+namespace pdllm {
+
+constexpr float kLog2eH = 1.4426950408889634f;
+
+struct HeadParams {
+  const char* w;        // [V, D] bf16, row stride in bytes
+  const char* h;        // [N, D]
+  const char* last;     // [n_seqs, D] or NULL: the row in front of each block when the rows are read shifted by one
+  long w_stride, h_stride, last_stride;  // bytes
+  long V, N;
+  int D;
+  int block_len, shift;
+  const long* labels;
+  int n_tok_tiles, n_voc_tiles;
+  // statistics
+  float2* part;   // [parts][N]: maximum and sum over the part's entries (the label's excluded when labels are given)
+  int* part_idx;  // [parts][N]: position of the maximum
+  float* xlab;    // [N]: logit of the label
+  // gradient
+  const float* lse;
+  const float* logp;
+  const float* g;
+  __bf16* d;      // [N, ldd]: a piece of the softmax gradient, entries from v0 on
+  __bf16* dlo;    // second plane: what the rounding of the first left (or NULL)
+  long ldd;
+  long v0;        // first entry of the piece; n_voc_tiles covers it
+  char* hz;       // [N, D]: h with the rows of labels outside the vocabulary cleared
+};
+
+// workgroup -> tile: four neighbouring token tiles share a strip of the weight in the L2 of one XCD
+__device__ __forceinline__ void head_tile(const HeadParams& p, int& vt, int& nt) {
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int per = 4 * p.n_voc_tiles;
+  const int g = id / per;
+  const int left = p.n_tok_tiles - 4 * g;
+  const int width = left < 4 ? left : 4;
+  const int r = id - g * per;
+  vt = __builtin_amdgcn_readfirstlane(r / width);  // (a division leaves scalar registers)
+  nt = __builtin_amdgcn_readfirstlane(4 * g + r - r / width * width);
+}
+
+template <class T>
+__device__ __forceinline__ void head_logits(const HeadParams& p, int vt, int nt, f32x16 (&acc)[T::MT][T::NT], char* lds) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned lds_base = (unsigned)(size_t)lds;
+  const long v0 = p.v0 + (long)vt * T::TM;
+  const unsigned kbytes = 2u * p.D;
+  LoadKC<T::LA> la;
+  la.init(p.w + v0 * p.w_stride, p.V - v0, (unsigned)p.w_stride, kbytes, wave, lane);
+  LoadRows<T::LB> lb;
+  lb.init(
+      [&](unsigned row) __attribute__((always_inline)) {
+        long t = (long)nt * T::TN + row;
+        t = t < p.N ? t : p.N - 1;
+        if (p.shift) {
+          const long b = t / p.block_len;
+          if (t - b * p.block_len != 0) --t;
+          else if (p.last) return p.last + b * p.last_stride;
+        }
+        return p.h + t * p.h_stride;
+      },
+      kbytes, wave, lane);
+#pragma unroll
+  for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  mainloop_bf16<T, false, false>(acc, (p.D + 63) / 64, lds_base, [&](int t, unsigned dst) __attribute__((always_inline)) {
+    la.issue(t, dst + wave * (T::LA * 1024));
+    lb.issue(t, dst + T::A_BYTES + wave * (T::LB * 1024));
+  });
+}
+
+// register e of a 32x32 result of lane half h holds row 8 (e / 4) + 4 h + e % 4
+__device__ __forceinline__ constexpr int row_of(int e, int h) { return 8 * (e >> 2) + 4 * h + (e & 3); }
+
+// exp(x - m) sums of a lane's 16 MT values; m = the maximum over them
+template <class T, bool CONF>
+__global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
+  int vt, nt;
+  head_tile(p, vt, nt);
+  f32x16 acc[T::MT][T::NT];
+  head_logits<T>(p, vt, nt, acc, lds);
+
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const long vw = (long)vt * T::TM + wm * (32 * T::MT);  // first entry of the wave
+  if (vw + 32 * T::MT > p.V) {                           // entries behind the vocabulary do not exist
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (vw + 32 * i + row_of(e, h) >= p.V)
+#pragma unroll
+          for (int j = 0; j < T::NT; ++j) acc[i][j][e] = -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < T::NT; ++j) {
+    const long row = (long)nt * T::TN + (wn * T::NT + j) * 32 + l32;
+    if constexpr (!CONF) {
+      const long lab = row < p.N ? p.labels[row] : -1;
+      const long rel = lab - vw;
+      const bool mine = rel >= 0 && rel < 32 * T::MT && lab < p.V;
+      if (__builtin_amdgcn_ballot_w64(mine) != 0) {
+        const int at = mine ? (int)rel : -1;
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (at == 32 * i + row_of(e, h)) {
+              x = acc[i][j][e];
+              acc[i][j][e] = -INFINITY;
+            }
+        if (mine && ((at >> 2) & 1) == h) p.xlab[row] = x;
+      }
+    }
+    float m = -INFINITY;
+    int idx = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = acc[i][j][e];
+        if constexpr (CONF) {
+          if (x > m) idx = 32 * i + row_of(e, 0);
+        }
+        m = fmaxf(m, x);
+      }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - ref) * kLog2eH);
+    // the other lane half holds the other rows of the same token
+    const float m2 = half_swap_max(m);
+    const float ref2 = m2 == -INFINITY ? 0.f : m2;
+    if (m != -INFINITY) s *= __builtin_amdgcn_exp2f((m - ref2) * kLog2eH);  // (else s is 0, or NaN from NaN alone)
+    s = half_swap_sum(s);
+    if constexpr (CONF) {
+      // the lowest position among the halves that hold the maximum
+      if (idx != 0x7fffffff) idx += 4 * h;
+      int cand = m == m2 ? idx : 0x7fffffff;
+      const int other = __shfl_xor(cand, 32, 64);
+      cand = other < cand ? other : cand;
+      idx = cand == 0x7fffffff ? cand : cand + (int)vw;
+    }
+    if (h == 0 && row < p.N) {
+      const long o = ((long)vt * T::WM + wm) * p.N + row;
+      p.part[o] = make_float2(m2, s);
+      if constexpr (CONF) p.part_idx[o] = idx;
+    }
+  }
+}
+
+struct Stat {
+  float m, s;
+  int idx;
+};
+__device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
+  Stat r;
+  r.m = fmaxf(a.m, b.m);
+  const float ref = r.m == -INFINITY ? 0.f : r.m;
+  r.s = a.s * __builtin_amdgcn_exp2f((a.m - ref) * kLog2eH) + b.s * __builtin_amdgcn_exp2f((b.m - ref) * kLog2eH);
+  const int ia = a.m == r.m ? a.idx : 0x7fffffff, ib = b.m == r.m ? b.idx : 0x7fffffff;
+  r.idx = ia < ib ? ia : ib;
+  return r;
+}
+
+// Joins the parts of 16 rows per workgroup, 64 threads to a row, in a fixed order.
+template <bool CONF>
+__global__ __launch_bounds__(1024) void head_join_kernel(const float2* __restrict__ part, const int* __restrict__ part_idx,
+                                                         const float* __restrict__ xlab, const long* __restrict__ labels,
+                                                         int parts, long N, long V, float* __restrict__ out,
+                                                         float* __restrict__ lse_out, long* __restrict__ token_out) {
+  __shared__ Stat sh[16][16];
+  const int r = threadIdx.x & 15;
+  const long row = (long)blockIdx.x * 16 + r;
+  Stat a = {-INFINITY, 0.f, 0x7fffffff};
+  if (row < N) {
+    for (int q = threadIdx.x >> 4; q < parts; q += 64) {
+      const float2 v = part[(long)q * N + row];
+      a = stat_join(a, {v.x, v.y, CONF ? part_idx[(long)q * N + row] : 0});
+    }
+  }
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    const Stat b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.idx, o, 64)};
+    a = stat_join(a, b);
+  }
+  if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][r] = a;
+  __syncthreads();
+  if (threadIdx.x >= 16 || row >= N) return;
+  a = sh[0][r];
+  for (int q = 1; q < 16; ++q) a = stat_join(a, sh[q][r]);
+  if constexpr (CONF) {
+    out[row] = 1.f / a.s;
+    token_out[row] = a.idx == 0x7fffffff ? 0 : a.idx;  // a row of NaN alone has no maximum
+  } else {
+    const float L = a.m + logf(a.s);
+    const long lab = labels[row];
+    if (lab < 0 || lab >= V) {
+      out[row] = -INFINITY;
+      if (lse_out) lse_out[row] = L;
+    } else {
+      const float x = xlab[row];
+      const float d = L - x;
+      float lp = -(fmaxf(d, 0.f) + log1pf(expf(-fabsf(d))));
+      if (x == INFINITY || (x == -INFINITY && L == -INFINITY)) lp = NAN;
+      out[row] = lp;
+      if (lse_out) lse_out[row] = x - lp;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// gradient
+// ------------------------------------------------------------------------------------------------------------------
+
+// One piece of the softmax gradient, rounded to bf16 as the operand of the two products behind it (each entry off by at
+// most 2^-8 of itself).  For few rows, where few entries make up a result and the products wait for memory anyway, the
+// second plane carries the remainder of the rounding.
+template <class T>
+__global__ __launch_bounds__(T::THREADS, 2) void head_dlogits_kernel(const HeadParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
+  int vt, nt;
+  head_tile(p, vt, nt);
+  if (p.hz) {
+    // grad_w must not see the rows without a label (their states may hold anything): a copy with those rows cleared
+    const int chunks = p.D / 8;
+    for (long i = (long)blockIdx.x * T::THREADS + threadIdx.x; i < p.N * chunks; i += (long)gridDim.x * T::THREADS) {
+      const long r = i / chunks;
+      const int c = (int)(i - r * chunks);
+      const long lab = p.labels[r];
+      uint4 v = {0, 0, 0, 0};
+      if (lab >= 0 && lab < p.V) v = *reinterpret_cast<const uint4*>(p.h + r * p.h_stride + 16 * c);
+      *reinterpret_cast<uint4*>(p.hz + i * 16) = v;
+    }
+  }
+  f32x16 acc[T::MT][T::NT];
+  head_logits<T>(p, vt, nt, acc, lds);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const long vl = (long)vt * T::TM + wm * (32 * T::MT);  // first entry of the wave, in the piece
+#pragma unroll
+  for (int j = 0; j < T::NT; ++j) {
+    const long row = (long)nt * T::TN + (wn * T::NT + j) * 32 + l32;
+    if (row >= p.N) continue;
+    const long lab = p.labels[row];
+    const bool in = lab >= 0 && lab < p.V;
+    const float lse = p.lse[row], g = p.g[row];
+    const float at_label = -g * expm1f(p.logp[row]);
+    const long rel = in ? lab - p.v0 - vl : -1;
+    const long left = p.V - p.v0 - vl;  // entries of the vocabulary from the wave's first on
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = 32 * i + row_of(4 * q + e, h);
+          float v = -g * __builtin_amdgcn_exp2f((acc[i][j][4 * q + e] - lse) * kLog2eH);
+          v = at == rel ? at_label : v;
+          y[e] = in && at < left ? v : 0.f;
+        }
+        const long o = row * p.ldd + vl + 32 * i + row_of(4 * q, h);
+        uint2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        *reinterpret_cast<uint2*>(p.d + o) = w;
+        if (p.dlo) {
+          uint2 l;
+          l.x = pack_bf16x2(y[0] - __uint_as_float(w.x << 16), y[1] - __uint_as_float(w.x & 0xffff0000u));
+          l.y = pack_bf16x2(y[2] - __uint_as_float(w.y << 16), y[3] - __uint_as_float(w.y & 0xffff0000u));
+          *reinterpret_cast<uint2*>(p.dlo + o) = l;
+        }
+      }
+  }
+}
+
+struct GradParams {
+  const char* w;   // rows of the weight from the piece's first on
+  const char* hz;  // [N, D]
+  const char* d;   // [planes][N, ldd]
+  long plane;      // bytes between the planes of d
+  long w_stride, ldd;  // bytes
+  long N;
+  long vp;         // entries of the piece
+  int D, planes;
+  int m_tiles, n_tiles, splits;
+  long k_per;      // entries per split, a multiple of 64
+  float* acc;      // [splits][N][D]
+  int add;         // the accumulators hold earlier pieces
+  __bf16* gw;      // rows of grad_w from the piece's first on
+  long gw_stride;  // elements
+};
+
+// grad_h, a piece: acc[split][row][c] (+)= sum over the split's entries of d[row][v] w[v][c]
+template <class T>
+__device__ __forceinline__ void head_grad_h_tile(const GradParams& p, char* lds) {
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
+  const int nt = __builtin_amdgcn_readfirstlane((id / p.m_tiles) % p.n_tiles);
+  const int split = __builtin_amdgcn_readfirstlane(id / (p.m_tiles * p.n_tiles));
+  const unsigned lds_base = (unsigned)(size_t)lds;
+  const long k0 = split * p.k_per;
+  long kn = p.vp - k0;
+  kn = kn < 0 ? 0 : (kn < p.k_per ? kn : p.k_per);  // (a last, shorter piece may leave a split without entries)
+  const int steps = (int)((kn + 63) / 64);
+  const int c0 = mt * T::TM;
+  const long r0 = (long)nt * T::TN;
+  const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
+  LoadKS<T::LA, T::TM> la;
+  la.init(p.w + k0 * p.w_stride + 2 * c0, p.w_stride, kn, cols, wave, lane);
+  LoadKC<T::LB> lb;
+  const unsigned kb = 128u * steps;  // d is padded with zeros to whole steps
+  const char* d0 = p.d + r0 * p.ldd + 2 * k0;
+  lb.init(d0, p.N - r0, (unsigned)p.ldd, kb, wave, lane);
+  f32x16 acc[T::MT][T::NT];
+#pragma unroll
+  for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  mainloop_bf16<T, true, false>(acc, steps * p.planes, lds_base, [&](int t, unsigned dst) __attribute__((always_inline)) {
+    const int t1 = t < steps ? t : t - steps;
+    la.issue(t1, dst + wave * (T::LA * 1024));
+    if (t == steps) lb.rebase(d0 + p.plane);
+    lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
+  });
+#pragma unroll
+  for (int j = 0; j < T::NT; ++j) {
+    const long row = r0 + (wn * T::NT + j) * 32 + l32;
+    if (row >= p.N) continue;
+    float* out = p.acc + ((long)split * p.N + row) * p.D;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = c0 + wm * (32 * T::MT) + 32 * i + row_of(4 * q, h);
+        if (c >= p.D) continue;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+        if (p.add) v += *reinterpret_cast<const f32x4*>(out + c);
+        *reinterpret_cast<f32x4*>(out + c) = v;
+      }
+  }
+}
+
+// (a function of its own: the host compiler cannot emit a kernel whose lambda holds a buffer descriptor)
+template <class T>
+__global__ __launch_bounds__(T::THREADS, 2) void head_grad_h_kernel(const GradParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
+  head_grad_h_tile<T>(p, lds);
+}
+
+// grad_h = the splits' accumulators, added in order, rounded once
+__global__ __launch_bounds__(256) void head_grad_h_join_kernel(const float* __restrict__ acc, int splits, long N, int D,
+                                                               __bf16* __restrict__ out, long stride) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= N * D) return;
+  f32x4 v = *reinterpret_cast<const f32x4*>(acc + i);
+  for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(acc + (long)s * N * D + i);
+  const long r = i / D;
+  const uint2 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  *reinterpret_cast<uint2*>(out + r * stride + (i - r * D)) = w;
+}
+
+// grad_w, the rows of a piece: gw[v][c] = sum over rows r of d[r][v] hz[r][c]
+template <class T>
+__global__ __launch_bounds__(T::THREADS, 2) void head_grad_w_kernel(const GradParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
+  const int nt = __builtin_amdgcn_readfirstlane(id / p.m_tiles);
+  const unsigned lds_base = (unsigned)(size_t)lds;
+  const int steps = (int)((p.N + 63) / 64);
+  const int c0 = mt * T::TM;
+  const long v0 = (long)nt * T::TN;
+  const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
+  LoadKS<T::LA, T::TM> la;
+  la.init(p.hz + 2 * c0, 2L * p.D, p.N, cols, wave, lane);
+  LoadKS<T::LB, T::TN> lb;
+  lb.init(p.d + 2 * v0, p.ldd, p.N, 2u * T::TN, wave, lane);  // the rows of d are whole tiles long
+  f32x16 acc[T::MT][T::NT];
+#pragma unroll
+  for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  const char* d0 = lb.base;
+  mainloop_bf16<T, true, true>(acc, steps * p.planes, lds_base, [&](int t, unsigned dst) __attribute__((always_inline)) {
+    const int t1 = t < steps ? t : t - steps;
+    la.issue(t1, dst + wave * (T::LA * 1024));
+    lb.base = t < steps ? d0 : d0 + p.plane;
+    lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
+  });
+#pragma unroll
+  for (int j = 0; j < T::NT; ++j) {
+    const long v = v0 + (wn * T::NT + j) * 32 + l32;
+    if (v >= p.vp) continue;
+    __bf16* out = p.gw + v * p.gw_stride;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = c0 + wm * (32 * T::MT) + 32 * i + row_of(4 * q, h);
+        if (c >= p.D) continue;
+        const uint2 w = {pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
+                         pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
+        *reinterpret_cast<uint2*>(out + c) = w;
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------------------------
+
+namespace {
+
+using TileL = Tile<4, 2, 2, 4, 2>;   // 256 entries x 256 rows, 8 waves
+using TileM = Tile<2, 2, 4, 2, 3>;   // 256 x 128
+using TileS2 = Tile<1, 2, 4, 1, 3>;  // 128 x 64, 4 waves
+using TileS = Tile<1, 1, 4, 1, 4>;   // 128 x 32
+
+constexpr long kMaxRows = 1L << 24;
+constexpr long kMaxVocab = 1L << 30;
+
+// parts of a row in the workspace: the waves of the vocabulary tiles
+int stat_parts(long n, long v) {
+  if (n <= 64) return (int)((v + TileS::TM - 1) / TileS::TM) * TileS::WM;
+  if (n <= 128) return (int)((v + TileM::TM - 1) / TileM::TM) * TileM::WM;
+  return (int)((v + TileL::TM - 1) / TileL::TM) * TileL::WM;
+}
+
+int64_t stats_ws(long n, long v, bool conf) { return (int64_t)stat_parts(n, v) * n * (conf ? 12 : 8) + (conf ? 0 : 4 * n); }
+
+template <class T, bool CONF>
+int launch_stats(HeadParams& p, hipStream_t s) {
+  p.n_voc_tiles = (int)((p.V + T::TM - 1) / T::TM);
+  p.n_tok_tiles = (int)((p.N + T::TN - 1) / T::TN);
+  const long grid = (long)p.n_voc_tiles * p.n_tok_tiles;
+  if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((head_stats_kernel<T, CONF>), dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
+  return launch_status();
+}
+
+int check_head(const void* hidden, int64_t h_stride, const void* weight, int64_t w_stride, int64_t n, int64_t v, int32_t d) {
+  if (n < 0 || v <= 0 || d <= 0 || d % 8 || n > kMaxRows || v > kMaxVocab || d > (1 << 20)) return PDLLM_ERR_SHAPE;
+  if (!weight || (!hidden && n > 0)) return PDLLM_ERR_NULL;
+  if (h_stride < d || w_stride < d || h_stride % 8 || w_stride % 8) return PDLLM_ERR_STRIDE;
+  if ((uintptr_t)hidden % 16 || (uintptr_t)weight % 16) return PDLLM_ERR_STRIDE;
+  if (w_stride * 2 * 256 >= 0x7fffffffL) return PDLLM_ERR_STRIDE;  // a tile's rows lie within 31-bit offsets
+  return PDLLM_OK;
+}
+
+template <bool CONF>
+int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, float* lse_out, long* token_out,
+          hipStream_t s) {
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < stats_ws(p.N, p.V, CONF)) return PDLLM_ERR_WORKSPACE;
+  const int parts = stat_parts(p.N, p.V);
+  p.part = static_cast<float2*>(workspace);
+  float* next = reinterpret_cast<float*>(p.part + (long)parts * p.N);
+  p.part_idx = reinterpret_cast<int*>(next);
+  p.xlab = next;
+  int st;
+  if (p.N <= 32) st = launch_stats<TileS, CONF>(p, s);
+  else if (p.N <= 64) st = launch_stats<TileS2, CONF>(p, s);
+  else if (p.N <= 128) st = launch_stats<TileM, CONF>(p, s);
+  else st = launch_stats<TileL, CONF>(p, s);
+  if (st != PDLLM_OK) return st;
+  hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)((p.N + 15) / 16)), dim3(1024), 0, s, p.part, p.part_idx, p.xlab,
+                     p.labels, parts, p.N, p.V, out, lse_out, token_out);
+  return launch_status();
+}
+
+// ---- gradient: sizes of the workspace's regions ----
+constexpr long kPieceBytes = 256L << 20;  // the piece of d the products read back stays within the last-level cache
+constexpr long kMaxPiece = 1L << 21;        // 256 rows of a piece lie within 31-bit offsets
+constexpr int kPlaneRows = 64;            // up to here the second plane is carried
+
+struct GradPlan {
+  long planes, ldd, vp;  // ldd = entries of a piece (a multiple of 256)
+  int splits, small;     // small: tiles of 64 rows for grad_h
+  int64_t hz, d, acc;    // bytes
+};
+
+int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+bool plan_grad(long n, long v, int d, int64_t have, GradPlan& g) {
+  g.planes = n <= kPlaneRows ? 2 : 1;
+  g.small = n <= 64;
+  const long vall = (v + 255) / 256 * 256;
+  const long tiles = ((d + 255) / 256) * (g.small ? 1 : (n + 255) / 256);
+  long most = 256 / tiles;
+  if (most < 1) most = 1;
+  g.hz = align256(2L * n * d);
+  auto acc_for = [&](long piece) {
+    long s = piece / 512;  // at least eight steps per split
+    s = s < 1 ? 1 : (s < most ? s : most);
+    g.splits = (int)s;
+    return align256(4L * s * n * d);
+  };
+  long piece = kPieceBytes / (2 * n * g.planes) / 256 * 256;
+  piece = piece < kMaxPiece ? piece : kMaxPiece;
+  piece = piece < 256 ? 256 : (piece < vall ? piece : vall);
+  if (have >= 0) {
+    while (piece > 256 && g.hz + align256(2L * n * piece * g.planes) + acc_for(piece) > have) piece = (piece / 2 + 255) / 256 * 256;
+  }
+  // pieces of equal length
+  const long count = (vall + piece - 1) / piece;
+  piece = ((vall + count - 1) / count + 255) / 256 * 256;
+  g.acc = acc_for(piece);
+  g.ldd = g.vp = piece;
+  g.d = align256(2L * n * piece * g.planes);
+  return have < 0 || g.hz + g.d + g.acc <= have;
+}
+
+template <class T>
+int launch_dlogits(HeadParams& p, hipStream_t s) {
+  p.n_tok_tiles = (int)((p.N + T::TN - 1) / T::TN);
+  hipLaunchKernelGGL(head_dlogits_kernel<T>, dim3((unsigned)((long)p.n_voc_tiles * p.n_tok_tiles)), dim3(T::THREADS), 0,
+                     s, p);
+  return launch_status();
+}
+
+using TileH = Tile<4, 2, 2, 4, 2>;   // grad_h: 256 columns x 256 rows
+using TileH2 = Tile<1, 2, 8, 1, 3>;  // 256 columns x 64 rows
+using TileD2 = Tile<1, 2, 8, 1, 3>;  // softmax gradient of up to 64 rows: 256 entries x 64 rows
+
+}  // namespace
+
+}  // namespace pdllm
+
+using namespace pdllm;
+
+extern "C" int64_t pdllm_head_workspace_bytes(int64_t n_rows, int64_t vocab) {
+  if (n_rows < 0 || vocab <= 0 || n_rows > kMaxRows || vocab > kMaxVocab) return PDLLM_ERR_SHAPE;
+  const int64_t a = stats_ws(n_rows, vocab, true), b = stats_ws(n_rows, vocab, false);
+  return a > b ? a : b;
+}
+
+extern "C" int pdllm_head_selfinfo_logprob(const void* hidden, int64_t hidden_stride, const void* weight,
+                                           int64_t weight_stride, const int64_t* labels, int64_t n_rows, int64_t vocab,
+                                           int32_t dim, void* workspace, int64_t workspace_bytes, float* logp_out,
+                                           float* lse_out, pdllm_stream_t stream) {
+  int st = check_head(hidden, hidden_stride, weight, weight_stride, n_rows, vocab, dim);
+  if (st != PDLLM_OK || n_rows == 0) return st;
+  if (!labels || !logp_out) return PDLLM_ERR_NULL;
+  HeadParams p = {};
+  p.w = static_cast<const char*>(weight);
+  p.h = static_cast<const char*>(hidden);
+  p.w_stride = 2 * weight_stride;
+  p.h_stride = 2 * hidden_stride;
+  p.V = vocab;
+  p.N = n_rows;
+  p.D = dim;
+  p.block_len = 1;
+  p.labels = reinterpret_cast<const long*>(labels);
+  return stats<false>(p, workspace, workspace_bytes, logp_out, lse_out, nullptr, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int pdllm_head_conf_argmax(const void* hidden, int64_t hidden_stride, const void* last_hidden,
+                                      int64_t last_hidden_stride, const void* weight, int64_t weight_stride, int64_t n_seqs,
+                                      int64_t block_len, int64_t vocab, int32_t dim, int32_t shift, void* workspace,
+                                      int64_t workspace_bytes, float* conf_out, int64_t* token_out, pdllm_stream_t stream) {
+  if (n_seqs < 0 || block_len <= 0 || block_len > kMaxRows || n_seqs > kMaxRows) return PDLLM_ERR_SHAPE;
+  const int64_t n = n_seqs * block_len;
+  int st = check_head(hidden, hidden_stride, weight, weight_stride, n, vocab, dim);
+  if (st != PDLLM_OK || n == 0) return st;
+  if (!conf_out || !token_out) return PDLLM_ERR_NULL;
+  if (last_hidden && (last_hidden_stride < dim || last_hidden_stride % 8 || (uintptr_t)last_hidden % 16)) return PDLLM_ERR_STRIDE;
+  HeadParams p = {};
+  p.w = static_cast<const char*>(weight);
+  p.h = static_cast<const char*>(hidden);
+  p.last = static_cast<const char*>(last_hidden);
+  p.w_stride = 2 * weight_stride;
+  p.h_stride = 2 * hidden_stride;
+  p.last_stride = 2 * last_hidden_stride;
+  p.V = vocab;
+  p.N = n;
+  p.D = dim;
+  p.block_len = (int)block_len;
+  p.shift = shift ? 1 : 0;
+  return stats<true>(p, workspace, workspace_bytes, conf_out, nullptr, reinterpret_cast<long*>(token_out),
+                     static_cast<hipStream_t>(stream));
+}
+
+extern "C" int pdllm_head_denoise_unmask(const void* hidden, int64_t hidden_stride, const void* last_hidden,
+                                         int64_t last_hidden_stride, const void* weight, int64_t weight_stride,
+                                         int64_t n_seqs, int64_t block_len, int64_t vocab, int32_t dim, int32_t shift,
+                                         int64_t* block_ids, int64_t mask_token_id, float threshold, void* workspace,
+                                         int64_t workspace_bytes, float* conf_out, int64_t* token_out, uint8_t* transfer_out,
+                                         int32_t* n_masked_left, pdllm_stream_t stream) {
+  if (n_seqs > 0 && (!block_ids || !transfer_out)) return PDLLM_ERR_NULL;
+  const int st = pdllm_head_conf_argmax(hidden, hidden_stride, last_hidden, last_hidden_stride, weight, weight_stride, n_seqs,
+                                        block_len, vocab, dim, shift, workspace, workspace_bytes, conf_out, token_out, stream);
+  if (st != PDLLM_OK || n_seqs == 0) return st;
+  return pdllm_threshold_unmask(conf_out, token_out, block_ids, n_seqs, block_len, mask_token_id, threshold, transfer_out,
+                                n_masked_left, stream);
+}
+
+extern "C" int64_t pdllm_head_selfinfo_grad_workspace_bytes(int64_t n_rows, int64_t vocab, int32_t dim) {
+  if (n_rows < 0 || vocab <= 0 || dim <= 0 || dim % 8 || n_rows > kMaxRows || vocab > kMaxVocab || dim > (1 << 20))
+    return PDLLM_ERR_SHAPE;
+  if (n_rows == 0) return 0;
+  GradPlan g;
+  plan_grad(n_rows, vocab, dim, -1, g);
+  return g.hz + g.d + g.acc;
+}
+
+extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
+                                        const int64_t* labels, const float* logp, const float* lse, const float* grad_logp,
+                                        int64_t n_rows, int64_t vocab, int32_t dim, void* workspace, int64_t workspace_bytes,
+                                        void* grad_hidden, int64_t grad_hidden_stride, void* grad_weight,
+                                        int64_t grad_weight_stride, pdllm_stream_t stream) {
+  int st = check_head(hidden, hidden_stride, weight, weight_stride, n_rows, vocab, dim);
+  if (st != PDLLM_OK) return st;
+  if (!grad_weight || (n_rows > 0 && (!labels || !logp || !lse || !grad_logp || !grad_hidden))) return PDLLM_ERR_NULL;
+  if (grad_hidden_stride < dim || grad_hidden_stride % 4 || grad_weight_stride < dim || grad_weight_stride % 4 ||
+      (uintptr_t)grad_hidden % 8 || (uintptr_t)grad_weight % 8)
+    return PDLLM_ERR_STRIDE;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (n_rows == 0) {  // a sum over no rows
+    GradParams q = {};
+    q.D = dim;
+    q.planes = 1;
+    q.m_tiles = (dim + 255) / 256;
+    q.n_tiles = (int)((vocab + 255) / 256);
+    q.vp = vocab;
+    q.gw = static_cast<__bf16*>(grad_weight);
+    q.gw_stride = grad_weight_stride;
+    if ((long)q.m_tiles * q.n_tiles > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(head_grad_w_kernel<TileH>, dim3((unsigned)(q.m_tiles * q.n_tiles)), dim3(TileH::THREADS), 0, s, q);
+    return launch_status();
+  }
+  GradPlan g;
+  if (!workspace || (uintptr_t)workspace % 256 || !plan_grad(n_rows, vocab, dim, workspace_bytes, g)) return PDLLM_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  HeadParams p = {};
+  p.w = static_cast<const char*>(weight);
+  p.h = static_cast<const char*>(hidden);
+  p.w_stride = 2 * weight_stride;
+  p.h_stride = 2 * hidden_stride;
+  p.V = vocab;
+  p.N = n_rows;
+  p.D = dim;
+  p.block_len = 1;
+  p.labels = reinterpret_cast<const long*>(labels);
+  p.lse = lse;
+  p.logp = logp;
+  p.g = grad_logp;
+  p.d = reinterpret_cast<__bf16*>(ws + g.hz);
+  p.dlo = g.planes > 1 ? p.d + n_rows * g.ldd : nullptr;
+  p.ldd = g.ldd;
+  GradParams q = {};
+  q.hz = ws;
+  q.d = ws + g.hz;
+  q.plane = 2 * n_rows * g.ldd;
+  q.w_stride = p.w_stride;
+  q.ldd = 2 * g.ldd;
+  q.N = n_rows;
+  q.D = dim;
+  q.planes = (int)g.planes;
+  q.m_tiles = (dim + 255) / 256;
+  q.acc = reinterpret_cast<float*>(ws + g.hz + g.d);
+  q.gw_stride = grad_weight_stride;
+  for (long v0 = 0; v0 < vocab; v0 += g.vp) {
+    const long vp = vocab - v0 < g.vp ? vocab - v0 : g.vp;
+    p.v0 = v0;
+    p.hz = v0 == 0 ? ws : nullptr;
+    p.n_voc_tiles = (int)((vp + 255) / 256);
+    st = g.small ? launch_dlogits<TileD2>(p, s) : launch_dlogits<TileL>(p, s);
+    if (st != PDLLM_OK) return st;
+    q.w = p.w + v0 * p.w_stride;
+    q.vp = vp;
+    q.add = v0 > 0;
+    q.splits = g.splits;
+    q.k_per = ((vp + g.splits - 1) / g.splits + 63) / 64 * 64;
+    q.gw = static_cast<__bf16*>(grad_weight) + v0 * grad_weight_stride;
+    q.n_tiles = g.small ? 1 : (int)((n_rows + 255) / 256);
+    const long grid = (long)q.m_tiles * q.n_tiles * q.splits;
+    if (g.small) {
+      hipLaunchKernelGGL(head_grad_h_kernel<TileH2>, dim3((unsigned)grid), dim3(TileH2::THREADS), 0, s, q);
+    } else {
+      hipLaunchKernelGGL(head_grad_h_kernel<TileH>, dim3((unsigned)grid), dim3(TileH::THREADS), 0, s, q);
+    }
+    if ((st = launch_status()) != PDLLM_OK) return st;
+    q.n_tiles = (int)((vp + 255) / 256);
+    hipLaunchKernelGGL(head_grad_w_kernel<TileH>, dim3((unsigned)((long)q.m_tiles * q.n_tiles)), dim3(TileH::THREADS),
+                       0, s, q);
+    if ((st = launch_status()) != PDLLM_OK) return st;
+  }
+  const long quads = n_rows * (dim / 4);
+  hipLaunchKernelGGL(head_grad_h_join_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, q.acc, g.splits, n_rows,
+                     dim, static_cast<__bf16*>(grad_hidden), grad_hidden_stride);
+  return launch_status();
+}

@@ -113,6 +113,21 @@ def select_chunks_from_logits(logits: torch.Tensor, labels: torch.Tensor, topk_c
 # token keep set (ENG:903-927)
 # ------------------------------------------------------------------------------------------
 
+def select_chunks_from_hidden(hidden: torch.Tensor, head_weight: torch.Tensor, labels: torch.Tensor, topk_chunks: int,
+                              mean: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Chunk scoring and ranking from the hidden states in front of the head (ENG:1098-1152 and 1199-1204), without the
+    logits: hidden [n_chunks, n_labels, dim] bf16, head_weight [vocab, dim] bf16, labels [n_chunks, n_labels] -> (scores fp32
+    [n_chunks], the indices of the best min(topk_chunks, n_chunks), ascending)."""
+    if hidden.dim() != 3 or tuple(labels.shape) != tuple(hidden.shape[:2]):
+        raise ValueError("hidden must be [n_chunks, n_labels, dim], labels [n_chunks, n_labels]")
+    c, j, dim = hidden.shape
+    if c == 0 or j == 0 or topk_chunks <= 0:
+        raise ValueError("chunks, labels and topk_chunks must be positive")
+    logp = ops.head_selfinfo_logprob(hidden.reshape(c * j, dim), head_weight, labels.reshape(c * j))
+    scores = ops.chunk_score_reduce(logp, c, mean)
+    return scores, ops.topk_lowest_index(scores, topk_chunks)
+
+
 def select_positions_from_token_scores(token_scores: torch.Tensor, *, capacity: int, chunk_len: int,
                                        keep_high: bool = True, force_keep_first: bool = True) -> torch.Tensor:
     """_select_positions_from_token_scores with ties broken by lowest index.  token_scores is one
@@ -460,6 +475,18 @@ def denoise_unmask_step(logits: torch.Tensor, block_ids: torch.Tensor, *, mask_t
     position with confidence >= threshold (ENG:2146-2157).  Returns (transfer mask, masked left)."""
     _, _, transfer, left = ops.denoise_unmask(logits, block_ids, mask_token_id, threshold, shift=shift,
                                               last_logit=last_context_logit)
+    return transfer, left
+
+
+def denoise_unmask_step_from_hidden(hidden: torch.Tensor, head_weight: torch.Tensor, block_ids: torch.Tensor, *,
+                                    mask_token_id: int, threshold: float,
+                                    last_context_hidden: Optional[torch.Tensor] = None,
+                                    shift: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """denoise_unmask_step from the hidden states in front of the head: hidden [n_seqs*block_len, dim] bf16, head_weight
+    [vocab, dim] bf16; the logits are reduced where they are made (ops.head_denoise_unmask).  last_context_hidden [n_seqs,
+    dim] takes the place of last_context_logit.  Returns (transfer mask, masked left)."""
+    _, _, transfer, left = ops.head_denoise_unmask(hidden, head_weight, block_ids, mask_token_id, threshold, shift=shift,
+                                                   last_hidden=last_context_hidden)
     return transfer, left
 
 

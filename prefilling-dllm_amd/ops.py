@@ -7,6 +7,7 @@ PyTorch is used only for device memory and the current stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from typing import Optional, Sequence, Tuple
@@ -537,6 +538,18 @@ def chunk_scores_from_logits(logits: torch.Tensor, labels: torch.Tensor, mean: b
     return out
 
 
+def chunk_score_reduce(logp: torch.Tensor, n_chunks: int, mean: bool = True) -> torch.Tensor:
+    """fp32 log-probabilities [n_chunks * n_labels] -> their mean (or sum) per chunk, added in index order."""
+    _need_cuda(logp)
+    if logp.dtype != torch.float32 or n_chunks <= 0 or logp.numel() % n_chunks or logp.numel() == 0:
+        raise ValueError("logp must be fp32 with the same number of labels, one at least, for every chunk")
+    logp = logp.reshape(-1).contiguous()
+    out = torch.empty(n_chunks, dtype=torch.float32, device=logp.device)
+    check(lib.pdllm_chunk_score_reduce(logp.data_ptr(), n_chunks, logp.numel() // n_chunks, 1 if mean else 0,
+                                       out.data_ptr(), _stream(logp)), "chunk_score_reduce")
+    return out
+
+
 def chunk_select_from_logits(logits: torch.Tensor, labels: torch.Tensor, k: int, mean: bool = True,
                              sorted_ascending: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """chunk_scores_from_logits followed by topk_lowest_index in one library call (two launches):
@@ -936,6 +949,230 @@ class PreparedDenoiseUnmask:
         if st != 0:
             check(st, "PreparedDenoiseUnmask.run")
         return self.transfer, self.left
+
+
+# ----------------------------------------------------------------------------------------
+# the vocabulary head: from hidden states, without logits in memory
+# ----------------------------------------------------------------------------------------
+
+def _on(device: torch.device):
+    """The device a launch goes to, made current where it is not."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _scratch(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
+    """Scratch memory of one call.  It belongs to the current stream's allocator, and under capture to the graph's pool, so
+    no two streams and no two graphs share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _head_args(hidden: torch.Tensor, weight: torch.Tensor) -> Tuple[int, int, int]:
+    """Checks of the states and the head's weight; (rows, vocab, dim)."""
+    _need_cuda(hidden, weight)
+    for name, t in (("hidden", hidden), ("weight", weight)):
+        if t.dtype != torch.bfloat16 or t.dim() != 2 or t.stride(1) != 1:
+            raise ValueError(f"{name} must be bf16 [rows, dim] with contiguous rows")
+    if hidden.device != weight.device:
+        raise ValueError("hidden and weight must be on one device")
+    if hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"hidden has {hidden.shape[1]} columns, weight {weight.shape[1]}")
+    return hidden.shape[0], weight.shape[0], hidden.shape[1]
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """The row stride of a 2-D tensor (a single row may carry any stride)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _head_rows(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, device) -> torch.Tensor:
+    _need_cuda(t)
+    if t.dim() != 1 or t.shape[0] != n or t.device != device:
+        raise ValueError(f"{name} must be a [{n}] tensor on the device of hidden, got {tuple(t.shape)}")
+    return t.to(dtype).contiguous()
+
+
+def head_selfinfo_logprob(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, return_lse: bool = False):
+    """log_softmax(hidden @ weight.T)[row, label[row]] in fp32 from bf16 states [rows, dim] and the head's bf16 weight
+    [vocab, dim]: selfinfo_logprob (fastdllm_engine.py:1148-1152) without the logits in memory.  Labels outside the
+    vocabulary give -inf.  return_lse: also log sum exp of each row, which head_selfinfo_grad takes."""
+    n, vocab, dim = _head_args(hidden, weight)
+    labels = _head_rows(labels, n, torch.int64, "labels", hidden.device)
+    logp = torch.empty(n, dtype=torch.float32, device=hidden.device)
+    lse = torch.empty_like(logp) if return_lse else None
+    with _on(hidden.device):
+        ws = _scratch(hidden.device, int(lib.pdllm_head_workspace_bytes(n, vocab)))
+        check(lib.pdllm_head_selfinfo_logprob(_ptr(hidden), _row_stride(hidden), weight.data_ptr(), _row_stride(weight),
+                                              labels.data_ptr(), n, vocab, dim, _ptr(ws), 0 if ws is None else ws.numel(),
+                                              logp.data_ptr(), _ptr(lse), _stream(hidden)), "head_selfinfo_logprob")
+    return (logp, lse) if return_lse else logp
+
+
+def head_selfinfo_grad(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, logp: torch.Tensor,
+                       lse: torch.Tensor, grad_logp: torch.Tensor, max_workspace_bytes: Optional[int] = None
+                       ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Gradients of (grad_logp * logp).sum() with respect to hidden and weight, for logp, lse =
+    head_selfinfo_logprob(hidden, weight, labels, return_lse=True): bf16 tensors shaped like them.  Rows with a label
+    outside the vocabulary have none.  The vocabulary is taken in pieces that fit the workspace; max_workspace_bytes makes
+    it smaller than the library's choice (256 MB of softmax gradient and the accumulators of grad_hidden)."""
+    n, vocab, dim = _head_args(hidden, weight)
+    dev = hidden.device
+    labels = _head_rows(labels, n, torch.int64, "labels", dev)
+    logp, lse, grad_logp = (_head_rows(t, n, torch.float32, name, dev)
+                            for t, name in ((logp, "logp"), (lse, "lse"), (grad_logp, "grad_logp")))
+    gh = torch.empty((n, dim), dtype=torch.bfloat16, device=dev)
+    gw = torch.empty((vocab, dim), dtype=torch.bfloat16, device=dev)
+    need = int(lib.pdllm_head_selfinfo_grad_workspace_bytes(n, vocab, dim))
+    if need < 0:
+        check(need, "head_selfinfo_grad")
+    if max_workspace_bytes is not None:
+        need = min(need, int(max_workspace_bytes))
+    with _on(dev):
+        ws = _scratch(dev, need)
+        check(lib.pdllm_head_selfinfo_grad(_ptr(hidden), _row_stride(hidden), weight.data_ptr(), _row_stride(weight),
+                                           labels.data_ptr(), logp.data_ptr(), lse.data_ptr(), grad_logp.data_ptr(), n, vocab,
+                                           dim, _ptr(ws), need if ws is not None else 0, gh.data_ptr(), dim, gw.data_ptr(), dim,
+                                           _stream(hidden)), "head_selfinfo_grad")
+    return gh, gw
+
+
+def _head_last(last_hidden: Optional[torch.Tensor], n_seqs: int, dim: int, device) -> Optional[torch.Tensor]:
+    if last_hidden is None:
+        return None
+    _need_cuda(last_hidden)
+    if last_hidden.dtype != torch.bfloat16 or last_hidden.numel() != n_seqs * dim or last_hidden.device != device:
+        raise ValueError(f"last_hidden must be bf16 [{n_seqs}, {dim}] on the device of hidden")
+    return last_hidden.reshape(n_seqs, dim).contiguous()
+
+
+def head_conf_argmax(hidden: torch.Tensor, weight: torch.Tensor, block_len: int, shift: bool = False,
+                     last_hidden: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """conf_argmax from bf16 states [n_seqs*block_len, dim] and the head's weight [vocab, dim], without the logits in
+    memory: (max softmax probability fp32, first index of the largest fp32 logit int64) per row.  shift: row i of a block
+    uses the state of row i - 1, row 0 last_hidden [n_seqs, dim] (the state in front of the block) or, without it, its own."""
+    n, vocab, dim = _head_args(hidden, weight)
+    if block_len <= 0 or n % block_len:
+        raise ValueError("rows must be a multiple of block_len")
+    dev = hidden.device
+    last = _head_last(last_hidden, n // block_len, dim, dev)
+    conf = torch.empty(n, dtype=torch.float32, device=dev)
+    tok = torch.empty(n, dtype=torch.int64, device=dev)
+    with _on(dev):
+        ws = _scratch(dev, int(lib.pdllm_head_workspace_bytes(n, vocab)))
+        check(lib.pdllm_head_conf_argmax(_ptr(hidden), _row_stride(hidden), _ptr(last), dim, weight.data_ptr(),
+                                         _row_stride(weight), n // block_len, block_len, vocab, dim, 1 if shift else 0,
+                                         _ptr(ws), 0 if ws is None else ws.numel(), conf.data_ptr(), tok.data_ptr(),
+                                         _stream(hidden)), "head_conf_argmax")
+    return conf, tok
+
+
+def head_denoise_unmask(hidden: torch.Tensor, weight: torch.Tensor, block_ids: torch.Tensor, mask_token_id: int,
+                        threshold: float, shift: bool = False, last_hidden: Optional[torch.Tensor] = None
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """denoise_unmask from bf16 states [n_seqs*block_len, dim] and the head's weight [vocab, dim], without the logits in
+    memory: head_conf_argmax, then the transfer rule of threshold_unmask on block_ids [n_seqs, block_len] in place.
+    Returns (confidence fp32 [rows], token int64 [rows], transfer bool [n_seqs, block_len], masked left int32 [n_seqs])."""
+    n, vocab, dim = _head_args(hidden, weight)
+    _need_cuda(block_ids)
+    if block_ids.dtype != torch.int64 or not block_ids.is_contiguous() or block_ids.dim() != 2 or \
+            block_ids.device != hidden.device:
+        raise ValueError("block_ids must be contiguous int64 [n_seqs, block_len] on the device of hidden")
+    n_seqs, block_len = block_ids.shape
+    if n != n_seqs * block_len:
+        raise ValueError("hidden rows must equal n_seqs * block_len")
+    dev = hidden.device
+    last = _head_last(last_hidden, n_seqs, dim, dev)
+    conf = torch.empty(n, dtype=torch.float32, device=dev)
+    tok = torch.empty(n, dtype=torch.int64, device=dev)
+    transfer = torch.empty((n_seqs, block_len), dtype=torch.uint8, device=dev)
+    left = torch.empty(n_seqs, dtype=torch.int32, device=dev)
+    if n == 0:
+        return conf, tok, transfer.view(torch.bool), left.zero_()
+    with _on(dev):
+        ws = _scratch(dev, int(lib.pdllm_head_workspace_bytes(n, vocab)))
+        check(lib.pdllm_head_denoise_unmask(_ptr(hidden), _row_stride(hidden), _ptr(last), dim, weight.data_ptr(),
+                                            _row_stride(weight), n_seqs, block_len, vocab, dim, 1 if shift else 0,
+                                            block_ids.data_ptr(), int(mask_token_id), float(threshold), _ptr(ws), ws.numel(),
+                                            conf.data_ptr(), tok.data_ptr(), transfer.data_ptr(), left.data_ptr(),
+                                            _stream(hidden)), "head_denoise_unmask")
+    return conf, tok, transfer.view(torch.bool), left
+
+
+# ----------------------------------------------------------------------------------------
+# products with 8-bit operands and a scale for each block of 128
+# ----------------------------------------------------------------------------------------
+
+def _quantize_arg(x: torch.Tensor, name: str) -> Tuple[int, int]:
+    _need_cuda(x)
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError(f"{name} must be bf16 [rows, k] with contiguous rows")
+    if x.shape[1] == 0 or x.shape[1] % 16:
+        raise ValueError(f"the columns of {name} must be a multiple of 16, got {x.shape[1]}")
+    return x.shape[0], x.shape[1]
+
+
+def quantize_fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16 [rows, k] -> (e4m3 [rows, k], fp32 scale [rows, ceil(k / 128)]): one scale for each row and 128 columns, the
+    smallest power of two with amax / scale <= 448 (1 for zeros, NaN where the block holds an infinity or a NaN).  The
+    scales lie block by block (stride (1, rows)), as fp8_block_linear reads them."""
+    n, k = _quantize_arg(x, "x")
+    q = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(((k + 127) // 128, n), dtype=torch.float32, device=x.device).t()
+    with _on(x.device):
+        check(lib.pdllm_fp8_quantize_rows(_ptr(x), _row_stride(x), n, k, _ptr(q), k, _ptr(scale), 1, n, _stream(x)),
+              "quantize_fp8_rows")
+    return q, scale
+
+
+def quantize_fp8_blocks(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16 weight [n, k] -> (e4m3 [n, k], fp32 scale [ceil(n / 128), ceil(k / 128)]): one scale for each block of 128 x 128,
+    by the rule of quantize_fp8_rows."""
+    n, k = _quantize_arg(weight, "weight")
+    q = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=weight.device)
+    kb = (k + 127) // 128
+    scale = torch.empty(((n + 127) // 128, kb), dtype=torch.float32, device=weight.device)
+    with _on(weight.device):
+        check(lib.pdllm_fp8_quantize_blocks(_ptr(weight), _row_stride(weight), n, k, _ptr(q), k, _ptr(scale), kb, 1,
+                                            _stream(weight)), "quantize_fp8_blocks")
+    return q, scale
+
+
+def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                     x_scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x @ weight.T for an e4m3 weight [n, k] with fp32 scales [ceil(n / 128), ceil(k / 128)], one for each block of
+    128 x 128.  x: bf16 [m, k] (quantised on the way as quantize_fp8_rows does), or e4m3 [m, k] with its scales x_scale
+    [m, ceil(k / 128)].  The result is bf16 [m, n]; `out` receives it where given."""
+    _need_cuda(x, weight, weight_scale, x_scale, out)
+    dev = x.device
+    for t in (weight, weight_scale, x_scale, out):
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
+    if weight.dtype != torch.float8_e4m3fn or weight.dim() != 2 or weight.stride(1) != 1:
+        raise ValueError("weight must be float8_e4m3fn [n, k] with contiguous rows")
+    n, k = weight.shape
+    if x.dim() != 2 or x.shape[1] != k or (k > 0 and x.stride(1) != 1):
+        raise ValueError(f"x must be [m, {k}] with contiguous rows, got {tuple(x.shape)}")
+    m, kb, nb = x.shape[0], (k + 127) // 128, (n + 127) // 128
+    if weight_scale.dtype != torch.float32 or tuple(weight_scale.shape) != (nb, kb):
+        raise ValueError(f"weight_scale must be fp32 [{nb}, {kb}], got {tuple(weight_scale.shape)}")
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be bf16 [{m}, {n}] with contiguous rows")
+    if x.dtype == torch.bfloat16:
+        if x_scale is not None:
+            raise ValueError("x_scale belongs to an e4m3 x")
+        x, x_scale = quantize_fp8_rows(x)
+    elif x.dtype == torch.float8_e4m3fn:
+        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (m, kb):
+            raise ValueError(f"an e4m3 x needs fp32 scales [{m}, {kb}]")
+    else:
+        raise ValueError("x must be bfloat16 or float8_e4m3fn")
+    with _on(dev):
+        check(lib.pdllm_fp8_linear(_ptr(x), _row_stride(x), _ptr(x_scale), x_scale.stride(0), x_scale.stride(1),
+                                   weight.data_ptr(), _row_stride(weight), weight_scale.data_ptr(), weight_scale.stride(0),
+                                   weight_scale.stride(1), m, n, k, _ptr(out), _row_stride(out), _stream(x)),
+              "fp8_block_linear")
+    return out
 
 
 def rope_inplace(x: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor) -> torch.Tensor:
