@@ -55,16 +55,15 @@ __device__ __forceinline__ uint2 to_e4m3(const uint4& v, float inv) {
   return make_uint2(r[0], r[1]);
 }
 
-// One scale for each row and 128 columns; 16 lanes to a block.  HBM-bound: 2 bytes read and 1 written per value.
-__global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const char* __restrict__ x, long x_stride, long M, int K,
+// One scale for each row and 128 columns; 16 lanes to a block, 16 blocks of a row to a workgroup.  HBM-bound: 2 bytes read and 1
+// written per value.
+__global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const char* __restrict__ x, long x_stride, int groups, int K,
                                                                 char* __restrict__ q, long q_stride, float* __restrict__ scale,
                                                                 long s_row, long s_blk) {
-  const int kb = (K + 127) / 128;
-  const long id = ((long)blockIdx.x * 256 + threadIdx.x) >> 4;
-  const long row = id / kb;
-  const int b = (int)(id - row * kb);
-  if (row >= M) return;  // (the 16 lanes of a block leave together)
+  const unsigned row = blockIdx.x / (unsigned)groups;
+  const int b = (int)(blockIdx.x - row * (unsigned)groups) * 16 + (threadIdx.x >> 4);
   const int k = b * 128 + (threadIdx.x & 15) * 8;
+  if (b * 128 >= K) return;  // (the 16 lanes of a block leave together)
   uint4 v = {0, 0, 0, 0};
   if (k < K) v = *reinterpret_cast<const uint4*>(x + row * x_stride + 2L * k);
   unsigned m = max_bits(v);
@@ -161,15 +160,16 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
   const long fw = f0 + wm * (32 * T::MT);
   const long fb = fw < p.N ? fw / 128 : (p.N - 1) / 128;
   const float* sw = p.sw + fb * p.sw_row;
-  const float* sx[T::NT];
+  const float* sx = p.sx + r0 * p.sx_row;
+  unsigned sx_off[T::NT];
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
-    const long row = r0 + (wn * T::NT + j) * 32 + l32;
-    sx[j] = p.sx + (row < p.M ? row : p.M - 1) * p.sx_row;
+    const int row = (wn * T::NT + j) * 32 + l32;
+    sx_off[j] = (unsigned)(r0 + row < p.M ? row : (int)(p.M - 1 - r0)) * (unsigned)p.sx_row;
   }
 
-  Frag<T::MT, false, T::TM> fa;
-  Frag<T::NT, false, T::TN> fb_;
+  Frag<T::MT, false, T::TM, T::KB> fa;
+  Frag<T::NT, false, T::TN, T::KB> fb_;
   fa.init(lds_base, wm * T::MT * 32, lane);
   fb_.init(lds_base + T::A_BYTES, wn * T::NT * 32, lane);
   f32x16 acc[T::MT][T::NT];
@@ -180,86 +180,130 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   const int steps = (p.K + 127) / 128;
-  float sc[T::NT], sn[T::NT];
-  {
-    const float w0 = sw[0];
+  constexpr int COPIES = T::LA + T::LB;
+  // The scales of a stage are fetched ST - 1 stages ahead, right in front of the copies of the stage behind it: loads return in
+  // order, so waiting for them never waits for copies that are not needed yet.
+  constexpr int AHEAD = T::ST - 1;
+  float sc[T::NT], qx[AHEAD][T::NT], qw[AHEAD];
+  auto fetch = [&](int t, float (&x)[T::NT], float& w) __attribute__((always_inline)) {
+    t = t < steps ? t : steps - 1;
+    w = sw[t * p.sw_blk];
 #pragma unroll
-    for (int j = 0; j < T::NT; ++j) sn[j] = sx[j][0] * w0;
-  }
+    for (int j = 0; j < T::NT; ++j) x[j] = (sx + t * p.sx_blk)[sx_off[j]];
+  };
 #pragma unroll
-  for (int s = 0; s < T::ST - 1; ++s)
+  for (int a = 0; a < AHEAD; ++a) fetch(a, qx[a], qw[a]);
+#pragma unroll
+  for (int s = 0; s < T::ST; ++s)
     if (s < steps) issue(s, lds_base + s * T::STAGE);
-  unsigned cur = 0, nxt = (T::ST - 1) * T::STAGE;
+  if (steps >= T::ST) vm_wait<(T::ST - 1) * COPIES>();
+  else vm_wait<0>();
+  wg_barrier();
+  unsigned cur = 0;
   bf16x8 A[2][4], B[T::NT][4];
-  for (int t = 0; t < steps; ++t) {
-    if (T::ST > 2 && t + T::ST - 2 < steps) vm_wait<(T::ST - 2) * (T::LA + T::LB)>();
-    else vm_wait<0>();
-    wg_barrier();
-    fb_.template read<0, 0>(B[0][0], cur);
-    fb_.template read<1, 0>(B[0][1], cur);
-    fb_.template read<2, 0>(B[0][2], cur);
-    fb_.template read<3, 0>(B[0][3], cur);
-    if constexpr (T::NT > 1) {
-      fb_.template read<0, 1>(B[1][0], cur);
-      fb_.template read<1, 1>(B[1][1], cur);
-      fb_.template read<2, 1>(B[1][2], cur);
-      fb_.template read<3, 1>(B[1][3], cur);
-    }
-    fa.template read<0, 0>(A[0][0], cur);
-    fa.template read<1, 0>(A[0][1], cur);
-    fa.template read<2, 0>(A[0][2], cur);
-    fa.template read<3, 0>(A[0][3], cur);
+  auto read_a = [&](auto jt, bf16x8 (&d)[4]) __attribute__((always_inline)) {
+    constexpr int J = decltype(jt)::value;
+    fa.template read<0, J>(d[0], cur);
+    fa.template read<1, J>(d[1], cur);
+    fa.template read<2, J>(d[2], cur);
+    fa.template read<3, J>(d[3], cur);
+  };
+  auto read_b = [&](auto jt, bf16x8 (&d)[4]) __attribute__((always_inline)) {
+    constexpr int J = decltype(jt)::value;
+    fb_.template read<0, J>(d[0], cur);
+    fb_.template read<1, J>(d[1], cur);
+    fb_.template read<2, J>(d[2], cur);
+    fb_.template read<3, J>(d[3], cur);
+  };
+  auto pair = [](const bf16x8& a, const bf16x8& b) __attribute__((always_inline)) {
+    typedef __attribute__((ext_vector_type(4))) int i32x4;
+    return __builtin_shufflevector(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  constexpr std::integral_constant<int, 0> c0{};
+  constexpr std::integral_constant<int, (T::NT > 1 ? 1 : 0)> n1{};
+  constexpr std::integral_constant<int, (T::MT > 1 ? 1 : 0)> m1{};
+  constexpr std::integral_constant<int, (T::MT > 2 ? 2 : 0)> m2{};
+  constexpr std::integral_constant<int, (T::MT > 3 ? 3 : 0)> m3{};
+  read_a(c0, A[0]);
+  read_b(c0, B[0]);
+  if constexpr (T::NT > 1) read_b(n1, B[1]);
+  f32x16 zero;
 #pragma unroll
-    for (int j = 0; j < T::NT; ++j) sc[j] = sn[j];
-    {
-      const int tn = t + 1 < steps ? t + 1 : t;
-      const float w1 = sw[tn * p.sw_blk];
-#pragma unroll
-      for (int j = 0; j < T::NT; ++j) sn[j] = sx[j][tn * p.sx_blk] * w1;
-    }
-    if (t + T::ST - 1 < steps) issue(t + T::ST - 1, lds_base + nxt);
+  for (int e = 0; e < 16; ++e) zero[e] = 0.f;
+
+  auto stage = [&](int t, auto more_tag) __attribute__((always_inline)) {
+    constexpr bool more = decltype(more_tag)::value;  // another stage follows
     lgkm_wait<0>();
 #pragma unroll
-    for (int j = 0; j < T::NT; ++j)
+    for (int j = 0; j < T::NT; ++j) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) tie(B[j][k]);
+      sc[j] = qx[0][j] * qw[0];
+#pragma unroll
+      for (int a = 0; a + 1 < AHEAD; ++a) qx[a][j] = qx[a + 1][j];
+    }
+#pragma unroll
+    for (int a = 0; a + 1 < AHEAD; ++a) qw[a] = qw[a + 1];
+    // Blocks of 32 features in turn.  The products of one block of 32 x 32 are added to the accumulators behind the matrix
+    // instructions of the next one, so that the additions never wait for their result.
+    f32x16 d[2];
 #pragma unroll
     for (int i = 0; i < T::MT; ++i) {
+      if (i > 0) lgkm_wait<0>();
 #pragma unroll
       for (int k = 0; k < 4; ++k) tie(A[i & 1][k]);
-      if (i + 1 < T::MT) {
-        auto next = [&](auto jt) __attribute__((always_inline)) {
-          constexpr int J = decltype(jt)::value;
-          fa.template read<0, J>(A[(i + 1) & 1][0], cur);
-          fa.template read<1, J>(A[(i + 1) & 1][1], cur);
-          fa.template read<2, J>(A[(i + 1) & 1][2], cur);
-          fa.template read<3, J>(A[(i + 1) & 1][3], cur);
-        };
-        if (i == 0) next(std::integral_constant<int, (T::MT > 1 ? 1 : 0)>{});
-        else if (i == 1) next(std::integral_constant<int, (T::MT > 2 ? 2 : 0)>{});
-        else next(std::integral_constant<int, (T::MT > 3 ? 3 : 0)>{});
+      const bool last = i + 1 == T::MT;
+      if (!last) {
+        if (i == 0) read_a(m1, A[1]);
+        else if (i == 1) read_a(m2, A[0]);
+        else read_a(m3, A[1]);
+      } else if (more) {
+        // the stage has been read by this wave; behind the barrier by all, and the next one has landed
+        if (T::ST > 2 && t + T::ST - 1 < steps) vm_wait<(T::ST - 2) * COPIES>();
+        else vm_wait<0>();
+        wg_barrier();
+        fetch(t + AHEAD, qx[AHEAD - 1], qw[AHEAD - 1]);
+        if (t + T::ST < steps) issue(t + T::ST, lds_base + cur);
+        cur = cur == (T::ST - 1) * T::STAGE ? 0u : cur + T::STAGE;
+        if constexpr (T::MT % 2 == 0) read_a(c0, A[0]);
       }
-      f32x16 zero;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) zero[e] = 0.f;
-      auto pair = [](const bf16x8& a, const bf16x8& b) __attribute__((always_inline)) {
-        typedef __attribute__((ext_vector_type(4))) int i32x4;
-        return __builtin_shufflevector(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
-      };
 #pragma unroll
       for (int j = 0; j < T::NT; ++j) {
-        f32x16 d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(A[i & 1][0], A[i & 1][1]), pair(B[j][0], B[j][1]), zero,
-                                                                   0, 0, 0, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(A[i & 1][2], A[i & 1][3]), pair(B[j][2], B[j][3]), d, 0, 0, 0,
-                                                            0, 0, 0);
+        const int n = i * T::NT + j, q = n - 1;
+        auto add = [&](int e0) __attribute__((always_inline)) {
+          if (n > 0)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(d[e], sc[j], acc[i][j][e]);
+            for (int e = e0; e < e0 + 8; ++e)
+              acc[q / T::NT][q % T::NT][e] = __builtin_fmaf(d[q & 1][e], sc[q % T::NT], acc[q / T::NT][q % T::NT][e]);
+          // (pinned here: moved behind the next branch, the additions would keep the products of a whole stage alive)
+          if (n > 0 && e0 == 8) asm volatile("" : "+v"(acc[q / T::NT][q % T::NT]));
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        d[n & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(A[i & 1][0], A[i & 1][1]), pair(B[j][0], B[j][1]), zero,
+                                                                   0, 0, 0, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        add(0);
+        __builtin_amdgcn_sched_barrier(0);
+        d[n & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(A[i & 1][2], A[i & 1][3]), pair(B[j][2], B[j][3]),
+                                                                   d[n & 1], 0, 0, 0, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (last && more) {
+          if (j == 0) read_b(c0, B[0]);
+          else read_b(n1, B[1]);
+        }
+        add(8);
       }
-      if (i + 1 < T::MT) lgkm_wait<0>();
+      if (last && more) {
+        if constexpr (T::MT % 2 != 0) read_a(c0, A[0]);
+      }
     }
-    cur = cur == (T::ST - 1) * T::STAGE ? 0u : cur + T::STAGE;
-    nxt = nxt == (T::ST - 1) * T::STAGE ? 0u : nxt + T::STAGE;
-  }
+    constexpr int q = T::MT * T::NT - 1;
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      acc[q / T::NT][q % T::NT][e] = __builtin_fmaf(d[q & 1][e], sc[q % T::NT], acc[q / T::NT][q % T::NT][e]);
+  };
+  for (int t = 0; t < steps - 1; ++t) stage(t, std::true_type{});
+  stage(steps - 1, std::false_type{});
 
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
@@ -292,12 +336,224 @@ __global__ __launch_bounds__(T::THREADS, 2) void fp8_linear_kernel(const Fp8Para
   fp8_tile<T>(p, lds);
 }
 
+// Up to 32 rows: the weight is read once, straight into registers, and the call waits for memory.  A workgroup takes FT = 16 or
+// 32 features and all rows; its eight waves take every eighth block of k, so that all of the workgroup's weight (FT x K
+// bytes) is on its way at once, and their fp32 sums meet in LDS, added in wave order.  16x16x128 instruction: lane l holds row
+// l & 15 of an operand, bytes 16 (l >> 4) .. + 15 of each half of the block (any order of k that both operands share).
+template <int FT, int TT>
+__global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
+  constexpr int NF = FT / 16, U = 2;  // U blocks of a wave in flight
+  __shared__ float part[8][TT * 16][FT + 1];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long f0 = (long)blockIdx.x * FT;
+  const long nf = p.N - f0 < FT ? p.N - f0 : FT;
+  const int m = (int)p.M;
+  const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.w + f0 * p.w_stride, (unsigned)((nf - 1) * p.w_stride) + (unsigned)p.K);
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, (unsigned)((m - 1) * p.x_stride) + (unsigned)p.K);
+  unsigned wo[NF], xo[TT], so[TT];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) wo[f] = f * 16 + l16 < nf ? (unsigned)(f * 16 + l16) * (unsigned)p.w_stride : kOutOfRange;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int row = t * 16 + l16;
+    xo[t] = row < m ? (unsigned)row * (unsigned)p.x_stride : kOutOfRange;
+    so[t] = (unsigned)(row < m ? row : m - 1) * (unsigned)p.sx_row;
+  }
+  const float* sw = p.sw + f0 / 128 * p.sw_row;
+  f32x4 acc[NF][TT];
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int blocks = (p.K + 127) / 128;
+  typedef __attribute__((ext_vector_type(4))) int i32x4;
+  auto load = [&](const __amdgpu_buffer_rsrc_t& rs, unsigned row, int kb) __attribute__((always_inline)) {
+    const unsigned k0 = kb * 128 + 16 * g, k1 = k0 + 64;
+    const i32x4 a = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, k0 < (unsigned)p.K ? row + k0 : kOutOfRange, 0, 0));
+    const i32x4 b = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, k1 < (unsigned)p.K ? row + k1 : kOutOfRange, 0, 0));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  for (int b0 = wave; b0 < blocks; b0 += 8 * U) {
+    i32x8 w[U][NF], x[U][TT];
+    float s[U][TT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int kb = b0 + 8 * u;  // (behind the last block: zeros)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) w[u][f] = load(wr, wo[f], kb);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int kb = b0 + 8 * u;
+      const int ks = kb < blocks ? kb : b0;
+      const float ws = sw[ks * p.sw_blk];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        x[u][t] = load(xr, xo[t], kb);
+        s[u][t] = kb < blocks ? (p.sx + ks * p.sx_blk)[so[t]] * ws : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          const f32x4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[u][f], x[u][t], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[f][t][e] = __builtin_fmaf(d[e], s[u][t], acc[f][t][e]);
+        }
+  }
+  // lane l of a 16x16 result holds column (row of the output) l & 15, rows (features) 4 (l >> 4) .. + 3
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave][t * 16 + l16][f * 16 + 4 * g + e] = acc[f][t][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < FT * TT * 16; i += 512) {
+    const int f = i % FT, row = i / FT;
+    if (row >= m || f >= nf) continue;
+    float v = part[0][row][f];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) v += part[q][row][f];
+    p.out[row * p.o_stride + f0 + f] = (__bf16)v;
+  }
+}
+
+// Up to 32 rows and many features: one workgroup per compute unit stays, the rows and their scales in its LDS (they would
+// otherwise be read again for every group of features: twice the weight's bytes, through the same L2), and walks over groups
+// of 32 features.  Wave (q, c) takes blocks q, q + 8, ... of k of the 16 features c of the group, so that the group's rows of the
+// weight, which lie side by side in memory, are asked for together; a ring of U blocks in registers runs on from group to
+// group.  The eight partial sums of a result meet in LDS, added in wave order.
+// Rows in LDS: block kb of row r, chunk c at ((kb * R + r) * 8 + (c ^ (r >> 1 & 7))) * 16: 16 rows of one chunk cover all banks.
+constexpr int kResidentPad = 33;
+constexpr int kResidentQ = 8;  // waves that share the features' k
+template <int R>
+constexpr long resident_lds(long blocks, long groups) {
+  return blocks * R * 132 + kResidentQ * R * kResidentPad * 4 + blocks * groups * 4;
+}
+template <int TT, int U>
+__global__ __launch_bounds__(1024, 4) void fp8_resident_kernel(const Fp8Params p) {
+  extern __shared__ __attribute__((aligned(1024))) char xs[];
+  constexpr int R = 16 * TT;
+  typedef __attribute__((ext_vector_type(4))) int i32x4;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kq = wave % kResidentQ, c = wave / kResidentQ;
+  const int m = (int)p.M;
+  const int blocks = (p.K + 127) / 128;  // at least kResidentQ
+  const int tasks = (int)((p.N + 31) / 32), per = (int)gridDim.x;
+  const int first = blockIdx.x;
+  float* scales = reinterpret_cast<float*>(xs + blocks * R * 128);
+  float* part = scales + blocks * R;                   // [kResidentQ][R][kResidentPad]
+  float* wscale = part + kResidentQ * R * kResidentPad;  // [groups of this workgroup][blocks]
+
+  int a_task = first, a_kb = kq;  // the block fetched next
+  i32x4 ring[U][2];
+  auto fetch = [&](i32x4 (&d)[2]) __attribute__((always_inline)) {
+    const long f = 32L * a_task + 16 * c;
+    const int nf = a_task < tasks && f < p.N ? (int)(p.N - f < 16 ? p.N - f : 16) : 0;
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(p.w + (nf > 0 ? f : 0) * p.w_stride, nf > 0 ? (unsigned)((nf - 1) * p.w_stride) + (unsigned)p.K : 0u);
+    const unsigned row = (unsigned)l16 * (unsigned)p.w_stride;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const unsigned k = a_kb * 128 + 64 * q + 16 * g;
+      d[q] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, k < (unsigned)p.K ? row + k : kOutOfRange, 0, 0));
+    }
+    a_kb += kResidentQ;
+    if (a_kb >= blocks) {
+      a_kb = kq;
+      a_task += per;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) fetch(ring[u]);
+  for (int i = threadIdx.x; i < blocks * R * 8; i += 1024) {
+    const int ch = i & 7, r = (i >> 3) % R, kb = (i >> 3) / R;
+    const int k = kb * 128 + 16 * ch;
+    uint4 v = {0, 0, 0, 0};
+    if (r < m && k < p.K) v = *reinterpret_cast<const uint4*>(p.x + (long)r * p.x_stride + k);
+    *reinterpret_cast<uint4*>(xs + (((kb * R + r) * 8 + (ch ^ ((r >> 1) & 7))) << 4)) = v;
+  }
+  for (int i = threadIdx.x; i < blocks * R; i += 1024) {
+    const int r = i % R, kb = i / R;
+    scales[i] = r < m ? p.sx[r * p.sx_row + kb * p.sx_blk] : 0.f;
+  }
+  const int mine = first < tasks ? (tasks - 1 - first) / per + 1 : 0;
+  for (int i = threadIdx.x; i < mine * blocks; i += 1024) {
+    const int t = i / blocks;
+    wscale[i] = p.sw[((first + t * per) >> 2) * p.sw_row + (i - t * blocks) * p.sw_blk];  // (32 features: within one block)
+  }
+  __syncthreads();
+
+  f32x4 acc[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int total = mine * ((blocks - kq + kResidentQ - 1) / kResidentQ);
+  int task = first, kb = kq;
+  const unsigned rd = (unsigned)(l16 * 128);
+  const unsigned ch0 = (unsigned)((g ^ ((l16 >> 1) & 7)) << 4), ch1 = (unsigned)(((4 + g) ^ ((l16 >> 1) & 7)) << 4);
+  for (int n = 0; n < total; n += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (n + u >= total) break;
+      const float ws = wscale[kb];
+      const i32x8 w = __builtin_shufflevector(ring[u][0], ring[u][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      const char* b = xs + kb * (R * 128) + rd;
+      i32x8 x[TT];
+      float sc[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const i32x4 x0 = *reinterpret_cast<const i32x4*>(b + t * 2048 + ch0);
+        const i32x4 x1 = *reinterpret_cast<const i32x4*>(b + t * 2048 + ch1);
+        x[t] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+        sc[t] = scales[kb * R + 16 * t + l16];
+      }
+      f32x4 d[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) d[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x[t], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = __builtin_fmaf(d[t][e], sc[t] * ws, acc[t][e]);
+      fetch(ring[u]);
+      kb += kResidentQ;
+      if (kb >= blocks) {
+        // the group is done: every wave passes these two barriers once per group
+        kb = kq;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[(kq * R + 16 * t + l16) * kResidentPad + 16 * c + 4 * g + e] = acc[t][e];
+          acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        lgkm_wait<0>();
+        wg_barrier();
+        for (int i = threadIdx.x; i < R * 32; i += 1024) {
+          const int f = i & 31, row = i >> 5;
+          const float* q = part + row * kResidentPad + f;
+          float v = q[0];
+#pragma unroll
+          for (int o = 1; o < kResidentQ; ++o) v += q[o * R * kResidentPad];
+          if (row < m && 32L * task + f < p.N) p.out[row * p.o_stride + 32L * task + f] = (__bf16)v;
+        }
+        lgkm_wait<0>();
+        wg_barrier();
+        task += per;
+        wscale += blocks;
+      }
+    }
+  }
+}
+
 namespace {
 
 using TileL = Tile<4, 2, 2, 4, 2>;   // 256 features x 256 rows, 8 waves
 using TileM = Tile<2, 2, 4, 2, 3>;   // 256 x 128
 using TileS2 = Tile<1, 2, 4, 1, 3>;  // 128 x 64, 4 waves
-using TileS = Tile<1, 1, 4, 1, 4>;   // 128 x 32
 
 constexpr long kMaxRows = 1L << 24;
 
@@ -308,6 +564,33 @@ int launch_fp8(Fp8Params& p, hipStream_t s) {
   const long grid = (long)p.m_tiles * p.n_tiles;
   if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(fp8_linear_kernel<T>, dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
+  return launch_status();
+}
+
+template <int TT>
+int launch_resident(Fp8Params& p, hipStream_t s) {
+  const long blocks = (p.K + 127) / 128, groups = ((p.N + 31) / 32 + 255) / 256;
+  hipLaunchKernelGGL((fp8_resident_kernel<TT, 4>), dim3(256), dim3(1024), (unsigned)resident_lds<16 * TT>(blocks, groups), s, p);
+  return launch_status();
+}
+
+int launch_stream(Fp8Params& p, hipStream_t s) {
+  const long blocks = (p.K + 127) / 128, groups = ((p.N + 31) / 32 + 255) / 256;
+  // (measured, K = 3584, 152064 features: 1 row 91 us resident, 88 us streamed; 16 rows 100 and 110; 32 rows 107 and 140)
+  if (p.M > 4 && p.N >= 16384 && blocks >= kResidentQ) {
+    if (p.M <= 16 && resident_lds<16>(blocks, groups) <= 160 * 1024) return launch_resident<1>(p, s);
+    if (p.M > 16 && resident_lds<32>(blocks, groups) <= 160 * 1024) return launch_resident<2>(p, s);
+  }
+  // 32 features to a workgroup read the rows half as often; 16 where 32 would leave compute units idle
+  const bool wide = (p.N + 31) / 32 >= 512;
+  const unsigned grid = (unsigned)((p.N + (wide ? 31 : 15)) / (wide ? 32 : 16));
+  if (p.M <= 16) {
+    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 1>), dim3(grid), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fp8_stream_kernel<16, 1>), dim3(grid), dim3(512), 0, s, p);
+  } else {
+    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 2>), dim3(grid), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fp8_stream_kernel<16, 2>), dim3(grid), dim3(512), 0, s, p);
+  }
   return launch_status();
 }
 
@@ -333,10 +616,10 @@ extern "C" int pdllm_fp8_quantize_rows(const void* x, int64_t x_stride, int64_t 
                                        pdllm_stream_t stream) {
   const int st = check_quantize(x, x_stride, n_rows, k, q, q_stride, scale, scale_row_stride, scale_block_stride);
   if (st != PDLLM_OK || n_rows == 0) return st;
-  const long blocks = n_rows * ((k + 127) / 128);
-  if ((blocks + 15) / 16 > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(fp8_quantize_rows_kernel, dim3((unsigned)((blocks + 15) / 16)), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), static_cast<const char*>(x), 2L * x_stride, (long)n_rows, k,
+  const int groups = (k + 2047) / 2048;
+  if (n_rows * groups > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(fp8_quantize_rows_kernel, dim3((unsigned)(n_rows * groups)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const char*>(x), 2L * x_stride, groups, k,
                      static_cast<char*>(q), (long)q_stride, scale, (long)scale_row_stride, (long)scale_block_stride);
   return launch_status();
 }
@@ -364,7 +647,7 @@ extern "C" int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_
   if (!x || !x_scale || !weight || !weight_scale || !out) return PDLLM_ERR_NULL;
   if (x_stride < k || x_stride % 16 || weight_stride < k || weight_stride % 16 || (uintptr_t)x % 16 || (uintptr_t)weight % 16 ||
       x_stride * 256 >= 0x7fffffffL || weight_stride * 256 >= 0x7fffffffL || out_stride < n || x_scale_row_stride < 0 ||
-      x_scale_block_stride < 0 || weight_scale_row_stride < 0 || weight_scale_block_stride < 0 ||
+      x_scale_row_stride >= (1 << 22) || x_scale_block_stride < 0 || weight_scale_row_stride < 0 || weight_scale_block_stride < 0 ||
       (uintptr_t)out % 2)
     return PDLLM_ERR_STRIDE;
   Fp8Params p = {};
@@ -385,8 +668,10 @@ extern "C" int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_
   p.o_stride = out_stride;
   p.vec = out_stride % 4 == 0 && (uintptr_t)out % 8 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (m <= 32) return launch_fp8<TileS>(p, s);
-  if (m <= 64) return launch_fp8<TileS2>(p, s);
-  if (m <= 128) return launch_fp8<TileM>(p, s);
-  return launch_fp8<TileL>(p, s);
+  if (m <= 32) return launch_stream(p, s);
+  // The largest tile that still gives most of the 256 compute units one: tiles re-read their operands less the larger they are
+  const auto tiles = [&](long tm, long tn) { return ((n + tm - 1) / tm) * ((m + tn - 1) / tn); };
+  if (m > 128 && tiles(256, 256) >= 160) return launch_fp8<TileL>(p, s);
+  if (m > 64 && tiles(256, 128) >= 160) return launch_fp8<TileM>(p, s);
+  return launch_fp8<TileS2>(p, s);
 }

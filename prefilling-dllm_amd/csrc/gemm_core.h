@@ -6,12 +6,16 @@
 // and 16 of its columns in registers, so softmax statistics of a row are sums over a lane's own registers and
 // stores are groups of four neighbouring columns.
 //
-// LDS.  A stage holds 128 bytes of k per row of A and of B (64 bf16 or 128 fp8 values).  Operands that lie with k
-// contiguous ("KC") are kept as rows of 128 bytes, 16-byte chunk c of row r at position c ^ ((r >> 1) & 7): 16
-// consecutive rows of one chunk cover all 64 banks.  Operands that lie with k as their row index ("KS", bf16 only)
-// are kept as 64 rows of TM * 2 bytes, chunk c of row r at c ^ ((r & 3) << 2), and read through the transposing
-// 64-bit reads (four rows of four neighbouring chunks per half wave, again all banks).  Copies go straight from memory to
-// LDS, ST - 1 stages ahead; operand reads are hand-issued with counted waits so that they do not wait for the copies.
+// LDS.  A stage holds KB = 64 or 128 bytes of k per row of A and of B.  Operands that lie with k contiguous ("KC") are kept as
+// rows of KB bytes, 16-byte chunk c of row r at position c ^ x(r) with x(r) = (r >> 1) & 7 (KB = 128) or (r >> 2) & 3 (KB = 64):
+// 16 consecutive rows of one chunk cover all 64 banks.  Operands that lie with k as their row index ("KS", bf16 only) are kept
+// as KB / 2 rows of TM * 2 bytes, chunk c of row r at c ^ ((r & 3) << 2), and read through the transposing 64-bit reads
+// (four rows of four neighbouring chunks per half wave, again all banks).  Copies go straight from memory to LDS, up to ST
+// stages ahead; operand reads are hand-issued with counted waits so that they do not wait for the copies.
+//
+// KB = 128 reads whole cache lines of a row at a time and is what the tiles of few rows use, which wait for memory; KB = 64
+// gives the large tiles four stages in 128 KB, so that the copies can be issued two at a time between groups of matrix
+// instructions instead of eight in a row, which kept the matrix unit waiting behind the address unit.
 #pragma once
 
 #include <type_traits>
@@ -32,6 +36,12 @@ __device__ __forceinline__ void wg_barrier() {
   asm volatile("s_barrier" ::: "memory");
 }
 
+// position of a row's chunks in LDS (see above)
+template <int KB>
+__device__ __forceinline__ constexpr unsigned chunk_xor(unsigned row) {
+  return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
 typedef __attribute__((address_space(3))) void lds_void;
 __device__ __forceinline__ lds_void* lds_at(unsigned a) { return (lds_void*)(size_t)a; }
 
@@ -46,31 +56,38 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, un
 }
 
 // Rows of k-contiguous data, through a buffer whose size ends with the last valid row: rows and k behind the end read
-// as zero.  L 1-KB copies per wave and stage.
-template <int L>
+// as zero.  L copies of 1024 / KB rows per wave and stage; a lane's offset inside them takes one of two values (KB = 128: the
+// chunk positions of even and odd groups of 8 rows), the group goes through the buffer's base.
+template <int L, int KB = 128>
 struct LoadKC {
-  __amdgpu_buffer_rsrc_t rs;
-  unsigned off[L], kc[L], kbytes, bytes;
-  __device__ __forceinline__ void init(const void* base, long rows_left, unsigned stride, unsigned kb, int wave, int lane) {
-    const unsigned rows = rows_left <= 0 ? 0u : (rows_left < 4096 ? (unsigned)rows_left : 4096u);
-    bytes = rows ? (rows - 1) * stride + kb : 0u;
-    rs = make_rsrc(base, bytes);
+  static constexpr int R = 1024 / KB, LANES = KB / 16;  // rows of a copy, lanes of a row
+  const char* base;  // first row of the wave
+  int bytes;         // from there to the end of the last valid row; not positive: none
+  unsigned stride, kbytes, off[2], kc[2];
+  __device__ __forceinline__ void init(const void* b, long rows_left, unsigned row_bytes, unsigned kb, int wave, int lane) {
+    base = static_cast<const char*>(b) + (long)(R * wave * L) * row_bytes;
+    rows_left -= R * wave * L;
+    const int rows = rows_left < 0 ? 0 : (rows_left < R * L ? (int)rows_left : R * L);
+    bytes = rows > 0 ? (int)((rows - 1) * row_bytes + kb) : 0;
+    stride = row_bytes;
     kbytes = kb;
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const unsigned row = 8 * (wave * L + i) + (lane >> 3);
-      const unsigned c = (lane & 7) ^ ((row >> 1) & 7);
-      kc[i] = 16 * c;
-      off[i] = row < rows ? row * stride + 16 * c : kOutOfRange;
+    for (int q = 0; q < 2; ++q) {
+      const unsigned c = (lane % LANES) ^ chunk_xor<KB>(R * (wave * L + q) + lane / LANES);
+      kc[q] = 16 * c;
+      off[q] = (lane / LANES) * row_bytes + 16 * c;
     }
   }
-  __device__ __forceinline__ void rebase(const void* base) { rs = make_rsrc(base, bytes); }
   __device__ __forceinline__ void issue(int t, unsigned dst) const {
-    const unsigned k = 128u * t;
+    const unsigned k = (unsigned)KB * t;
+    unsigned o[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) o[q] = k + kc[q] < kbytes ? off[q] + k : kOutOfRange;
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const unsigned o = k + kc[i] < kbytes ? off[i] + k : kOutOfRange;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, o, 0, 0, 0);
+      const int left = bytes - (int)(R * i * stride);
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (long)(R * i) * stride, left > 0 ? left : 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, o[KB == 128 ? i & 1 : 0], 0, 0, 0);
     }
   }
 };
@@ -78,56 +95,56 @@ struct LoadKC {
 // Rows of k-contiguous data at a 64-bit address per row (rows gathered from two tensors).  Rows past the end repeat a
 // valid row (their results are dropped); k behind the end repeats the row's first bytes (the other operand is zero
 // there).
-template <int L>
+template <int L, int KB = 128>
 struct LoadRows {
+  static constexpr int R = 1024 / KB, LANES = KB / 16;
   const char* p[L];
-  unsigned kc[L], kbytes;
+  unsigned kc[2], kbytes;
   template <typename F>
   __device__ __forceinline__ void init(F&& row_ptr, unsigned kb, int wave, int lane) {
     kbytes = kb;
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const unsigned row = 8 * (wave * L + i) + (lane >> 3);
-      kc[i] = 16 * ((lane & 7) ^ ((row >> 1) & 7));
-      p[i] = row_ptr(row);
-    }
+    for (int i = 0; i < L; ++i) p[i] = row_ptr((unsigned)(R * (wave * L + i) + lane / LANES));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) kc[q] = 16 * ((lane % LANES) ^ chunk_xor<KB>(R * (wave * L + q) + lane / LANES));
   }
   __device__ __forceinline__ void issue(int t, unsigned dst) const {
-    const unsigned k = 128u * t;
+    const unsigned k = (unsigned)KB * t;
+    unsigned o[2];
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const unsigned o = k + kc[i] < kbytes ? k + kc[i] : 0u;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[i] + o), lds_at(dst + 1024 * i),
-                                       16, 0, 0);
-    }
+    for (int q = 0; q < 2; ++q) o[q] = k + kc[q] < kbytes ? k + kc[q] : 0u;
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[i] + o[KB == 128 ? i & 1 : 0]),
+                                       lds_at(dst + 1024 * i), 16, 0, 0);
   }
 };
 
-// 64 rows of k per stage, W columns (bf16) of each: base = first row, first column.  Rows from k_rows on read as zero;
+// KB / 2 rows of k per stage, W columns (bf16) of each: base = first row, first column.  Rows from k_rows on read as zero;
 // so do columns from col_bytes on.
-template <int L, int W>
+template <int L, int W, int KB = 128>
 struct LoadKS {
+  static constexpr int ROWS = KB / 2, CH = W / 8;  // rows of a stage, chunks of a row
   const char* base;
-  long stride;   // bytes
+  long stride;  // bytes
   long k_rows;
   unsigned off[L], colb;
   __device__ __forceinline__ void init(const void* b, long stride_bytes, long rows, unsigned col_bytes, int wave, int lane) {
-    constexpr int CH = W / 8;  // chunks per row
     base = static_cast<const char*>(b);
     stride = stride_bytes;
     k_rows = rows;
+    colb = col_bytes;
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       const unsigned q = 64 * (wave * L + i) + lane;
       const unsigned row = q / CH, c = (q % CH) ^ ((row & 3) << 2);
       off[i] = 16 * c < col_bytes ? row * (unsigned)stride_bytes + 16 * c : kOutOfRange;
     }
-    colb = col_bytes;
   }
   __device__ __forceinline__ void issue(int t, unsigned dst) const {
-    const long r0 = 64L * t;
+    const long r0 = (long)ROWS * t;
     const long left = k_rows - r0;
-    const unsigned rows = left <= 0 ? 0u : (left < 64 ? (unsigned)left : 64u);
+    const unsigned rows = left <= 0 ? 0u : (left < ROWS ? (unsigned)left : (unsigned)ROWS);
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + r0 * stride, rows ? (rows - 1) * (unsigned)stride + colb : 0u);
 #pragma unroll
     for (int i = 0; i < L; ++i)
@@ -135,12 +152,12 @@ struct LoadKS {
   }
 };
 
-template <int MT_, int NT_, int WM_, int WN_, int ST_>
+template <int MT_, int NT_, int WM_, int WN_, int ST_, int KB_ = 128>
 struct Tile {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, ST = ST_;
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, ST = ST_, KB = KB_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN;
-  static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int A_BYTES = TM * KB, B_BYTES = TN * KB, STAGE = A_BYTES + B_BYTES;
   static constexpr int LA = A_BYTES / 1024 / NW, LB = B_BYTES / 1024 / NW;
   static_assert(LA * NW * 1024 == A_BYTES && LB * NW * 1024 == B_BYTES, "every wave copies the same number of pieces");
   static constexpr int LDS = ST * STAGE;
@@ -150,29 +167,29 @@ struct Tile {
 // A wave's operand fragments: N_ blocks of 32 rows (KC) or columns (KS), the first one at `first` of the tile.  A fragment of
 // step ks holds, in lane half h, the k values 16 ks + 8 h .. + 7 (bf16) of its row; for fp8 two fragments make one operand
 // (the k values of both operands are permuted alike, which a sum over k does not see).
-template <int N_, bool KS, int W>
+template <int N_, bool KS, int W, int KB>
 struct Frag;
-template <int N_, int W>
-struct Frag<N_, false, W> {
-  unsigned a[4];
+template <int N_, int W, int KB>
+struct Frag<N_, false, W, KB> {
+  unsigned a[KB / 32];
   typedef bf16x8 raw;
   static constexpr int READS = 1;  // LDS operations per fragment
   __device__ __forceinline__ void init(unsigned lds_base, int first, int lane) {
     const int l32 = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) a[ks] = lds_base + (first + l32) * 128 + (((2 * ks + h) ^ ((l32 >> 1) & 7)) << 4);
+    for (int ks = 0; ks < KB / 32; ++ks) a[ks] = lds_base + (first + l32) * KB + (((2 * ks + h) ^ chunk_xor<KB>(l32)) << 4);
   }
   template <int KS_, int J>
   __device__ __forceinline__ void read(raw& d, unsigned stage) const {
-    lds_read_b128<J * 4096>(d, a[KS_] + stage);
+    lds_read_b128<J * 32 * KB>(d, a[KS_] + stage);
   }
   static __device__ __forceinline__ bf16x8 value(const raw& r) { return r; }
 };
 struct TrPair {
   s16x4 lo, hi;
 };
-template <int N_, int W>
-struct Frag<N_, true, W> {
+template <int N_, int W, int KB>
+struct Frag<N_, true, W, KB> {
   unsigned a[N_];
   typedef TrPair raw;
   static constexpr int READS = 2;
@@ -200,67 +217,89 @@ struct Frag<N_, true, W> {
 __device__ __forceinline__ void tie(bf16x8& r) { asm volatile("" : "+v"(r)::"memory"); }
 __device__ __forceinline__ void tie(TrPair& r) { asm volatile("" : "+v"(r.lo), "+v"(r.hi)::"memory"); }
 
-// The bf16 loop over T stages.  issue(t, lds address of the stage) starts the copies of stage t (T::LA + T::LB per wave);
-// every wave passes one barrier per stage: behind it stage t has landed for all waves and stage t - 1 has been read by all
-// of them, so its buffer takes the copies of stage t + ST - 1.
+// The bf16 loop over `steps` stages.  issue(t, lds address of the stage, part) starts half of the copies of stage t (part 0
+// or 1; T::LA + T::LB per wave in all).  One barrier per stage, in front of the stage's last group of matrix instructions: by
+// then every wave has read all of the stage and its own part of the next one has landed, so behind the barrier the
+// stage's buffer takes the copies of stage t + ST, half of them at once and half behind the next group, and the first
+// fragments of the next stage are read while the last group runs.
 template <class T, bool AKS, bool BKS, class Issue>
 __device__ __forceinline__ void mainloop_bf16(f32x16 (&acc)[T::MT][T::NT], int steps, unsigned lds_base, Issue&& issue) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
-  Frag<T::MT, AKS, T::TM> fa;
-  Frag<T::NT, BKS, T::TN> fb;
+  constexpr int COPIES = T::LA + T::LB, GROUPS = T::KB / 32;
+  typedef Frag<T::MT, AKS, T::TM, T::KB> FA;
+  typedef Frag<T::NT, BKS, T::TN, T::KB> FB;
+  FA fa;
+  FB fb;
   fa.init(lds_base, wm * T::MT * 32, lane);
   fb.init(lds_base + T::A_BYTES, wn * T::NT * 32, lane);
-  typename Frag<T::MT, AKS, T::TM>::raw A[2][T::MT];
-  typename Frag<T::NT, BKS, T::TN>::raw B[2][T::NT];
-  constexpr int READS = T::MT * Frag<T::MT, AKS, T::TM>::READS + T::NT * Frag<T::NT, BKS, T::TN>::READS;
+  typename FA::raw A[2][T::MT];
+  typename FB::raw B[2][T::NT];
+  constexpr int READS = T::MT * FA::READS + T::NT * FB::READS;
   static_assert(READS <= 15, "the wait counts 15 LDS operations at most");
+  static_assert(GROUPS == 2 || GROUPS == 4, "fragments alternate between two sets");
+  if (steps <= 0) return;
+  unsigned cur = 0, old = 0;
+  auto read = [&](auto ks_tag, int set) __attribute__((always_inline)) {
+    constexpr int KS = decltype(ks_tag)::value;
+    fb.template read<KS, 0>(B[set][0], cur);
+    if constexpr (T::NT > 1) fb.template read<KS, 1>(B[set][1], cur);
+    fa.template read<KS, 0>(A[set][0], cur);
+    if constexpr (T::MT > 1) fa.template read<KS, 1>(A[set][1], cur);
+    if constexpr (T::MT > 2) fa.template read<KS, 2>(A[set][2], cur);
+    if constexpr (T::MT > 3) fa.template read<KS, 3>(A[set][3], cur);
+  };
+  auto mul = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
-  for (int s = 0; s < T::ST - 1; ++s)
-    if (s < steps) issue(s, lds_base + s * T::STAGE);
-  unsigned cur = 0, nxt = (T::ST - 1) * T::STAGE;
-  for (int t = 0; t < steps; ++t) {
-    if (T::ST > 2 && t + T::ST - 2 < steps) vm_wait<(T::ST - 2) * (T::LA + T::LB)>();
-    else vm_wait<0>();
-    wg_barrier();
-    auto read = [&](auto ks_tag, int set) __attribute__((always_inline)) {
-      constexpr int KS = decltype(ks_tag)::value;
-      fb.template read<KS, 0>(B[set][0], cur);
-      if constexpr (T::NT > 1) fb.template read<KS, 1>(B[set][1], cur);
-      fa.template read<KS, 0>(A[set][0], cur);
-      if constexpr (T::MT > 1) fa.template read<KS, 1>(A[set][1], cur);
-      if constexpr (T::MT > 2) fa.template read<KS, 2>(A[set][2], cur);
-      if constexpr (T::MT > 3) fa.template read<KS, 3>(A[set][3], cur);
-    };
-    auto mul = [&](int set) __attribute__((always_inline)) {
+    for (int i = 0; i < T::MT; ++i) tie(A[set][i]);
 #pragma unroll
-      for (int i = 0; i < T::MT; ++i) tie(A[set][i]);
+    for (int j = 0; j < T::NT; ++j) tie(B[set][j]);
 #pragma unroll
-      for (int j = 0; j < T::NT; ++j) tie(B[set][j]);
+    for (int i = 0; i < T::MT; ++i)
 #pragma unroll
-      for (int i = 0; i < T::MT; ++i)
+      for (int j = 0; j < T::NT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FA::value(A[set][i]), FB::value(B[set][j]), acc[i][j], 0, 0, 0);
+  };
 #pragma unroll
-        for (int j = 0; j < T::NT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Frag<T::MT, AKS, T::TM>::value(A[set][i]),
-                                                              Frag<T::NT, BKS, T::TN>::value(B[set][j]), acc[i][j], 0, 0, 0);
-    };
-    read(std::integral_constant<int, 0>{}, 0);
-    if (t + T::ST - 1 < steps) issue(t + T::ST - 1, lds_base + nxt);
+  for (int s = 0; s < T::ST; ++s)
+    if (s < steps) {
+      issue(s, lds_base + s * T::STAGE, 0);
+      issue(s, lds_base + s * T::STAGE, 1);
+    }
+  if (steps >= T::ST) vm_wait<(T::ST - 1) * COPIES>();
+  else vm_wait<0>();
+  wg_barrier();
+  read(std::integral_constant<int, 0>{}, 0);
+  // all groups of a stage but the last; behind the first one the second half of the copies that the barrier before allowed
+  auto groups = [&](int t) __attribute__((always_inline)) {
     read(std::integral_constant<int, 1>{}, 1);
     lgkm_wait<READS>();
+    if (t > 0 && t + T::ST - 1 < steps) issue(t + T::ST - 1, lds_base + old, 1);
     mul(0);
-    read(std::integral_constant<int, 2>{}, 0);
-    lgkm_wait<READS>();
-    mul(1);
-    read(std::integral_constant<int, 3>{}, 1);
-    lgkm_wait<READS>();
-    mul(0);
+    if constexpr (GROUPS == 4) {
+      read(std::integral_constant<int, 2>{}, 0);
+      lgkm_wait<READS>();
+      mul(1);
+      read(std::integral_constant<int, 3>{}, 1);
+      lgkm_wait<READS>();
+      mul(0);
+    }
     lgkm_wait<0>();
-    mul(1);
+  };
+  for (int t = 0; t < steps - 1; ++t) {
+    groups(t);
+    if (T::ST > 2 && t + T::ST - 1 < steps) vm_wait<(T::ST - 2) * COPIES>();
+    else vm_wait<0>();
+    wg_barrier();
+    old = cur;
     cur = cur == (T::ST - 1) * T::STAGE ? 0u : cur + T::STAGE;
-    nxt = nxt == (T::ST - 1) * T::STAGE ? 0u : nxt + T::STAGE;
+    read(std::integral_constant<int, 0>{}, 0);
+    if (t + T::ST < steps) issue(t + T::ST, lds_base + old, 0);
+    mul(1);
   }
+  groups(steps - 1);
+  mul(1);
 }
 
 }  // namespace pdllm

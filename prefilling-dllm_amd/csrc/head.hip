@@ -58,9 +58,9 @@ __device__ __forceinline__ void head_logits(const HeadParams& p, int vt, int nt,
   const unsigned lds_base = (unsigned)(size_t)lds;
   const long v0 = p.v0 + (long)vt * T::TM;
   const unsigned kbytes = 2u * p.D;
-  LoadKC<T::LA> la;
+  LoadKC<T::LA, T::KB> la;
   la.init(p.w + v0 * p.w_stride, p.V - v0, (unsigned)p.w_stride, kbytes, wave, lane);
-  LoadRows<T::LB> lb;
+  LoadRows<T::LB, T::KB> lb;
   lb.init(
       [&](unsigned row) __attribute__((always_inline)) {
         long t = (long)nt * T::TN + row;
@@ -79,16 +79,32 @@ __device__ __forceinline__ void head_logits(const HeadParams& p, int vt, int nt,
     for (int j = 0; j < T::NT; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  mainloop_bf16<T, false, false>(acc, (p.D + 63) / 64, lds_base, [&](int t, unsigned dst) __attribute__((always_inline)) {
-    la.issue(t, dst + wave * (T::LA * 1024));
-    lb.issue(t, dst + T::A_BYTES + wave * (T::LB * 1024));
-  });
+  mainloop_bf16<T, false, false>(
+      acc, (int)(kbytes + T::KB - 1) / T::KB, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
+        if (part == 0) la.issue(t, dst + wave * (T::LA * 1024));
+        else lb.issue(t, dst + T::A_BYTES + wave * (T::LB * 1024));
+      });
 }
 
 // register e of a 32x32 result of lane half h holds row 8 (e / 4) + 4 h + e % 4
 __device__ __forceinline__ constexpr int row_of(int e, int h) { return 8 * (e >> 2) + 4 * h + (e & 3); }
 
-// exp(x - m) sums of a lane's 16 MT values; m = the maximum over them
+struct Stat {
+  float m, s;
+  int idx;
+};
+__device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
+  Stat r;
+  r.m = fmaxf(a.m, b.m);
+  const float ref = r.m == -INFINITY ? 0.f : r.m;
+  r.s = a.s * __builtin_amdgcn_exp2f((a.m - ref) * kLog2eH) + b.s * __builtin_amdgcn_exp2f((b.m - ref) * kLog2eH);
+  const int ia = a.m == r.m ? a.idx : 0x7fffffff, ib = b.m == r.m ? b.idx : 0x7fffffff;
+  r.idx = ia < ib ? ia : ib;
+  return r;
+}
+
+// A tile of logits and its statistics per row: a lane's own values first (their maximum, then the sum of exp(x - max)), the other
+// half of the wave, the other waves of the row.
 template <class T, bool CONF>
 __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
@@ -110,10 +126,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadPar
 #pragma unroll
           for (int j = 0; j < T::NT; ++j) acc[i][j][e] = -INFINITY;
   }
+  __syncthreads();  // the tile's operands are done with: their place takes the statistics
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
-    const long row = (long)nt * T::TN + (wn * T::NT + j) * 32 + l32;
     if constexpr (!CONF) {
+      const long row = (long)nt * T::TN + (wn * T::NT + j) * 32 + l32;
       const long lab = row < p.N ? p.labels[row] : -1;
       const long rel = lab - vw;
       const bool mine = rel >= 0 && rel < 32 * T::MT && lab < p.V;
@@ -162,52 +179,60 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadPar
       cand = other < cand ? other : cand;
       idx = cand == 0x7fffffff ? cand : cand + (int)vw;
     }
-    if (h == 0 && row < p.N) {
-      const long o = ((long)vt * T::WM + wm) * p.N + row;
-      p.part[o] = make_float2(m2, s);
-      if constexpr (CONF) p.part_idx[o] = idx;
+    if (h == 0) {
+      Stat* sh = reinterpret_cast<Stat*>(lds) + wm * T::TN + (wn * T::NT + j) * 32 + l32;
+      *sh = {m2, s, idx};
     }
+  }
+  __syncthreads();
+  const int c = threadIdx.x;
+  const long row = (long)nt * T::TN + c;
+  if (c < T::TN && row < p.N) {
+    const Stat* sh = reinterpret_cast<const Stat*>(lds) + c;
+    Stat a = sh[0];
+#pragma unroll
+    for (int q = 1; q < T::WM; ++q) a = stat_join(a, sh[q * T::TN]);
+    const long o = (long)vt * p.N + row;
+    p.part[o] = make_float2(a.m, a.s);
+    if constexpr (CONF) p.part_idx[o] = a.idx;
   }
 }
 
-struct Stat {
-  float m, s;
-  int idx;
-};
-__device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
-  Stat r;
-  r.m = fmaxf(a.m, b.m);
-  const float ref = r.m == -INFINITY ? 0.f : r.m;
-  r.s = a.s * __builtin_amdgcn_exp2f((a.m - ref) * kLog2eH) + b.s * __builtin_amdgcn_exp2f((b.m - ref) * kLog2eH);
-  const int ia = a.m == r.m ? a.idx : 0x7fffffff, ib = b.m == r.m ? b.idx : 0x7fffffff;
-  r.idx = ia < ib ? ia : ib;
-  return r;
-}
-
-// Joins the parts of 16 rows per workgroup, 64 threads to a row, in a fixed order.
+// Joins the parts of 8 rows per workgroup, 128 threads to a row, in a fixed order; four parts of a thread are fetched at a
+// time (one after the other their latency was the kernel's time: 32 rows x 1188 parts 12.8 -> TODO us).
 template <bool CONF>
 __global__ __launch_bounds__(1024) void head_join_kernel(const float2* __restrict__ part, const int* __restrict__ part_idx,
                                                          const float* __restrict__ xlab, const long* __restrict__ labels,
                                                          int parts, long N, long V, float* __restrict__ out,
                                                          float* __restrict__ lse_out, long* __restrict__ token_out) {
-  __shared__ Stat sh[16][16];
-  const int r = threadIdx.x & 15;
-  const long row = (long)blockIdx.x * 16 + r;
+  __shared__ Stat sh[16][8];
+  const int r = threadIdx.x & 7;
+  const long row = (long)blockIdx.x * 8 + r;
   Stat a = {-INFINITY, 0.f, 0x7fffffff};
   if (row < N) {
-    for (int q = threadIdx.x >> 4; q < parts; q += 64) {
-      const float2 v = part[(long)q * N + row];
-      a = stat_join(a, {v.x, v.y, CONF ? part_idx[(long)q * N + row] : 0});
+    for (int q = threadIdx.x >> 3; q < parts; q += 512) {
+      float2 v[4];
+      int idx[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool on = q + 128 * u < parts;
+        const long at = (long)(on ? q + 128 * u : q) * N + row;
+        v[u] = part[at];
+        idx[u] = CONF ? part_idx[at] : 0;
+        if (!on) v[u] = make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a = stat_join(a, {v[u].x, v[u].y, idx[u]});
     }
   }
 #pragma unroll
-  for (int o = 16; o < 64; o <<= 1) {
+  for (int o = 8; o < 64; o <<= 1) {
     const Stat b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.idx, o, 64)};
     a = stat_join(a, b);
   }
-  if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][r] = a;
+  if ((threadIdx.x & 63) < 8) sh[threadIdx.x >> 6][r] = a;
   __syncthreads();
-  if (threadIdx.x >= 16 || row >= N) return;
+  if (threadIdx.x >= 8 || row >= N) return;
   a = sh[0][r];
   for (int q = 1; q < 16; ++q) a = stat_join(a, sh[q][r]);
   if constexpr (CONF) {
@@ -326,16 +351,18 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, char* lds)
   const long k0 = split * p.k_per;
   long kn = p.vp - k0;
   kn = kn < 0 ? 0 : (kn < p.k_per ? kn : p.k_per);  // (a last, shorter piece may leave a split without entries)
-  const int steps = (int)((kn + 63) / 64);
+  constexpr int SK = T::KB / 2;  // entries per stage
+  const int steps = (int)((kn + SK - 1) / SK);
   const int c0 = mt * T::TM;
   const long r0 = (long)nt * T::TN;
   const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
-  LoadKS<T::LA, T::TM> la;
+  LoadKS<T::LA, T::TM, T::KB> la;
   la.init(p.w + k0 * p.w_stride + 2 * c0, p.w_stride, kn, cols, wave, lane);
-  LoadKC<T::LB> lb;
-  const unsigned kb = 128u * steps;  // d is padded with zeros to whole steps
+  LoadKC<T::LB, T::KB> lb;
+  const unsigned kb = (unsigned)T::KB * steps;  // d is padded with zeros to whole stages
   const char* d0 = p.d + r0 * p.ldd + 2 * k0;
   lb.init(d0, p.N - r0, (unsigned)p.ldd, kb, wave, lane);
+  d0 = lb.base;
   f32x16 acc[T::MT][T::NT];
 #pragma unroll
   for (int i = 0; i < T::MT; ++i)
@@ -343,12 +370,16 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, char* lds)
     for (int j = 0; j < T::NT; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  mainloop_bf16<T, true, false>(acc, steps * p.planes, lds_base, [&](int t, unsigned dst) __attribute__((always_inline)) {
-    const int t1 = t < steps ? t : t - steps;
-    la.issue(t1, dst + wave * (T::LA * 1024));
-    if (t == steps) lb.rebase(d0 + p.plane);
-    lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
-  });
+  mainloop_bf16<T, true, false>(
+      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
+        const int t1 = t < steps ? t : t - steps;
+        if (part == 0) {
+          la.issue(t1, dst + wave * (T::LA * 1024));
+        } else {
+          lb.base = t < steps ? d0 : d0 + p.plane;
+          lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
+        }
+      });
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
     const long row = r0 + (wn * T::NT + j) * 32 + l32;
@@ -399,13 +430,14 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_grad_w_kernel(const GradPa
   const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
   const int nt = __builtin_amdgcn_readfirstlane(id / p.m_tiles);
   const unsigned lds_base = (unsigned)(size_t)lds;
-  const int steps = (int)((p.N + 63) / 64);
+  constexpr int SK = T::KB / 2;  // rows per stage
+  const int steps = (int)((p.N + SK - 1) / SK);
   const int c0 = mt * T::TM;
   const long v0 = (long)nt * T::TN;
   const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
-  LoadKS<T::LA, T::TM> la;
+  LoadKS<T::LA, T::TM, T::KB> la;
   la.init(p.hz + 2 * c0, 2L * p.D, p.N, cols, wave, lane);
-  LoadKS<T::LB, T::TN> lb;
+  LoadKS<T::LB, T::TN, T::KB> lb;
   lb.init(p.d + 2 * v0, p.ldd, p.N, 2u * T::TN, wave, lane);  // the rows of d are whole tiles long
   f32x16 acc[T::MT][T::NT];
 #pragma unroll
@@ -415,12 +447,16 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_grad_w_kernel(const GradPa
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   const char* d0 = lb.base;
-  mainloop_bf16<T, true, true>(acc, steps * p.planes, lds_base, [&](int t, unsigned dst) __attribute__((always_inline)) {
-    const int t1 = t < steps ? t : t - steps;
-    la.issue(t1, dst + wave * (T::LA * 1024));
-    lb.base = t < steps ? d0 : d0 + p.plane;
-    lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
-  });
+  mainloop_bf16<T, true, true>(
+      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
+        const int t1 = t < steps ? t : t - steps;
+        if (part == 0) {
+          la.issue(t1, dst + wave * (T::LA * 1024));
+        } else {
+          lb.base = t < steps ? d0 : d0 + p.plane;
+          lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
+        }
+      });
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
     const long v = v0 + (wn * T::NT + j) * 32 + l32;
@@ -453,11 +489,11 @@ using TileS = Tile<1, 1, 4, 1, 4>;   // 128 x 32
 constexpr long kMaxRows = 1L << 24;
 constexpr long kMaxVocab = 1L << 30;
 
-// parts of a row in the workspace: the waves of the vocabulary tiles
+// parts of a row in the workspace: the vocabulary tiles
 int stat_parts(long n, long v) {
-  if (n <= 64) return (int)((v + TileS::TM - 1) / TileS::TM) * TileS::WM;
-  if (n <= 128) return (int)((v + TileM::TM - 1) / TileM::TM) * TileM::WM;
-  return (int)((v + TileL::TM - 1) / TileL::TM) * TileL::WM;
+  const int tm = n <= 64 ? TileS::TM : TileL::TM;
+  static_assert(TileS::TM == TileS2::TM && TileM::TM == TileL::TM, "two heights of tiles");
+  return (int)((v + tm - 1) / tm);
 }
 
 int64_t stats_ws(long n, long v, bool conf) { return (int64_t)stat_parts(n, v) * n * (conf ? 12 : 8) + (conf ? 0 : 4 * n); }
@@ -496,7 +532,7 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
   else if (p.N <= 128) st = launch_stats<TileM, CONF>(p, s);
   else st = launch_stats<TileL, CONF>(p, s);
   if (st != PDLLM_OK) return st;
-  hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)((p.N + 15) / 16)), dim3(1024), 0, s, p.part, p.part_idx, p.xlab,
+  hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)((p.N + 7) / 8)), dim3(1024), 0, s, p.part, p.part_idx, p.xlab,
                      p.labels, parts, p.N, p.V, out, lse_out, token_out);
   return launch_status();
 }
@@ -551,7 +587,7 @@ int launch_dlogits(HeadParams& p, hipStream_t s) {
   return launch_status();
 }
 
-using TileH = Tile<4, 2, 2, 4, 2>;   // grad_h: 256 columns x 256 rows
+using TileH = Tile<4, 2, 2, 4, 2>;  // grad_h, grad_w: 256 columns x 256 rows or entries
 using TileH2 = Tile<1, 2, 8, 1, 3>;  // 256 columns x 64 rows
 using TileD2 = Tile<1, 2, 8, 1, 3>;  // softmax gradient of up to 64 rows: 256 entries x 64 rows
 
