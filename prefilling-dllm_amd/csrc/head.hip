@@ -23,7 +23,8 @@ struct HeadParams {
   int D;
   int block_len, shift;
   const long* labels;
-  int n_tok_tiles, n_voc_tiles;
+  // tiles (see head_grid): n_full whole tiles, n_cut pieces of 64 rows of whole tiles, then the rows behind the whole columns
+  int n_tok_tiles, n_voc_tiles, n_full, n_cut, rest_cols;
   // statistics
   float2* part;   // [parts][N]: maximum and sum over the part's entries (the label's excluded when labels are given)
   int* part_idx;  // [parts][N]: position of the maximum
@@ -39,9 +40,8 @@ struct HeadParams {
   char* hz;       // [N, D]: h with the rows of labels outside the vocabulary cleared
 };
 
-// workgroup -> tile: four neighbouring token tiles share a strip of the weight in the L2 of one XCD
-__device__ __forceinline__ void head_tile(const HeadParams& p, int& vt, int& nt) {
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
+// tile number -> tile: four neighbouring token tiles share a strip of the weight in the L2 of one XCD
+__device__ __forceinline__ void head_tile(const HeadParams& p, int id, int& vt, int& nt) {
   const int per = 4 * p.n_voc_tiles;
   const int g = id / per;
   const int left = p.n_tok_tiles - 4 * g;
@@ -52,7 +52,7 @@ __device__ __forceinline__ void head_tile(const HeadParams& p, int& vt, int& nt)
 }
 
 template <class T>
-__device__ __forceinline__ void head_logits(const HeadParams& p, int vt, int nt, f32x16 (&acc)[T::MT][T::NT], char* lds) {
+__device__ __forceinline__ void head_logits(const HeadParams& p, int vt, long row0, f32x16 (&acc)[T::MT][T::NT], char* lds) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned lds_base = (unsigned)(size_t)lds;
@@ -63,7 +63,7 @@ __device__ __forceinline__ void head_logits(const HeadParams& p, int vt, int nt,
   LoadRows<T::LB, T::KB> lb;
   lb.init(
       [&](unsigned row) __attribute__((always_inline)) {
-        long t = (long)nt * T::TN + row;
+        long t = row0 + row;
         t = t < p.N ? t : p.N - 1;
         if (p.shift) {
           const long b = t / p.block_len;
@@ -106,12 +106,9 @@ __device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
 // A tile of logits and its statistics per row: a lane's own values first (their maximum, then the sum of exp(x - max)), the other
 // half of the wave, the other waves of the row.
 template <class T, bool CONF>
-__global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
-  int vt, nt;
-  head_tile(p, vt, nt);
+__device__ __forceinline__ void head_stats_tile(const HeadParams& p, int vt, long row0, char* lds) {
   f32x16 acc[T::MT][T::NT];
-  head_logits<T>(p, vt, nt, acc, lds);
+  head_logits<T>(p, vt, row0, acc, lds);
 
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -130,7 +127,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadPar
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
     if constexpr (!CONF) {
-      const long row = (long)nt * T::TN + (wn * T::NT + j) * 32 + l32;
+      const long row = row0 + (wn * T::NT + j) * 32 + l32;
       const long lab = row < p.N ? p.labels[row] : -1;
       const long rel = lab - vw;
       const bool mine = rel >= 0 && rel < 32 * T::MT && lab < p.V;
@@ -186,7 +183,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadPar
   }
   __syncthreads();
   const int c = threadIdx.x;
-  const long row = (long)nt * T::TN + c;
+  const long row = row0 + c;
   if (c < T::TN && row < p.N) {
     const Stat* sh = reinterpret_cast<const Stat*>(lds) + c;
     Stat a = sh[0];
@@ -196,6 +193,36 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadPar
     p.part[o] = make_float2(a.m, a.s);
     if constexpr (CONF) p.part_idx[o] = a.idx;
   }
+}
+
+// A workgroup's tile: T for the whole tiles, then pieces of 64 rows (TS) of those that would be an almost empty last round of
+// the compute units, and of the rows behind the last whole column.
+template <class T, class TS, class F>
+__device__ __forceinline__ void head_dispatch(const HeadParams& p, F&& tile) {
+  int vt, nt;
+  if ((int)blockIdx.x < p.n_full) {
+    head_tile(p, xcd_remap(blockIdx.x, p.n_full), vt, nt);
+    tile(static_cast<T*>(nullptr), vt, (long)nt * T::TN);
+    return;
+  }
+  const int id = xcd_remap(blockIdx.x - p.n_full, gridDim.x - p.n_full);
+  if (id < p.n_cut) {
+    constexpr int Q = T::TN / TS::TN;
+    head_tile(p, p.n_full + id / Q, vt, nt);
+    tile(static_cast<TS*>(nullptr), vt, (long)nt * T::TN + (id % Q) * TS::TN);
+  } else {
+    const int r = id - p.n_cut;
+    vt = __builtin_amdgcn_readfirstlane(r / p.rest_cols);
+    tile(static_cast<TS*>(nullptr), vt, (long)p.n_tok_tiles * T::TN + (r - vt * p.rest_cols) * TS::TN);
+  }
+}
+
+template <class T, class TS, bool CONF>
+__global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS > TS::LDS ? T::LDS : TS::LDS];
+  head_dispatch<T, TS>(p, [&](auto* t, int vt, long row0) __attribute__((always_inline)) {
+    head_stats_tile<std::remove_pointer_t<decltype(t)>, CONF>(p, vt, row0, lds);
+  });
 }
 
 // Joins the parts of 8 rows per workgroup, 128 threads to a row, in a fixed order; four parts of a thread are fetched at a
@@ -263,31 +290,16 @@ __global__ __launch_bounds__(1024) void head_join_kernel(const float2* __restric
 // most 2^-8 of itself).  For few rows, where few entries make up a result and the products wait for memory anyway, the
 // second plane carries the remainder of the rounding.
 template <class T>
-__global__ __launch_bounds__(T::THREADS, 2) void head_dlogits_kernel(const HeadParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
-  int vt, nt;
-  head_tile(p, vt, nt);
-  if (p.hz) {
-    // grad_w must not see the rows without a label (their states may hold anything): a copy with those rows cleared
-    const int chunks = p.D / 8;
-    for (long i = (long)blockIdx.x * T::THREADS + threadIdx.x; i < p.N * chunks; i += (long)gridDim.x * T::THREADS) {
-      const long r = i / chunks;
-      const int c = (int)(i - r * chunks);
-      const long lab = p.labels[r];
-      uint4 v = {0, 0, 0, 0};
-      if (lab >= 0 && lab < p.V) v = *reinterpret_cast<const uint4*>(p.h + r * p.h_stride + 16 * c);
-      *reinterpret_cast<uint4*>(p.hz + i * 16) = v;
-    }
-  }
+__device__ __forceinline__ void head_dlogits_tile(const HeadParams& p, int vt, long row0, char* lds) {
   f32x16 acc[T::MT][T::NT];
-  head_logits<T>(p, vt, nt, acc, lds);
+  head_logits<T>(p, vt, row0, acc, lds);
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   const long vl = (long)vt * T::TM + wm * (32 * T::MT);  // first entry of the wave, in the piece
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
-    const long row = (long)nt * T::TN + (wn * T::NT + j) * 32 + l32;
+    const long row = row0 + (wn * T::NT + j) * 32 + l32;
     if (row >= p.N) continue;
     const long lab = p.labels[row];
     const bool in = lab >= 0 && lab < p.V;
@@ -320,6 +332,26 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_dlogits_kernel(const HeadP
   }
 }
 
+template <class T, class TS>
+__global__ __launch_bounds__(T::THREADS, 2) void head_dlogits_kernel(const HeadParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS > TS::LDS ? T::LDS : TS::LDS];
+  if (p.hz) {
+    // grad_w must not see the rows without a label (their states may hold anything): a copy with those rows cleared
+    const int chunks = p.D / 8;
+    for (long i = (long)blockIdx.x * T::THREADS + threadIdx.x; i < p.N * chunks; i += (long)gridDim.x * T::THREADS) {
+      const long r = i / chunks;
+      const int c = (int)(i - r * chunks);
+      const long lab = p.labels[r];
+      uint4 v = {0, 0, 0, 0};
+      if (lab >= 0 && lab < p.V) v = *reinterpret_cast<const uint4*>(p.h + r * p.h_stride + 16 * c);
+      *reinterpret_cast<uint4*>(p.hz + i * 16) = v;
+    }
+  }
+  head_dispatch<T, TS>(p, [&](auto* t, int vt, long row0) __attribute__((always_inline)) {
+    head_dlogits_tile<std::remove_pointer_t<decltype(t)>>(p, vt, row0, lds);
+  });
+}
+
 struct GradParams {
   const char* w;   // rows of the weight from the piece's first on
   const char* hz;  // [N, D]
@@ -329,7 +361,7 @@ struct GradParams {
   long N;
   long vp;         // entries of the piece
   int D, planes;
-  int m_tiles, n_tiles, splits;
+  int m_tiles, n_tiles, splits;  // of grad_h: column tiles, row tiles, splits of the entries
   long k_per;      // entries per split, a multiple of 64
   float* acc;      // [splits][N][D]
   int add;         // the accumulators hold earlier pieces
@@ -337,13 +369,12 @@ struct GradParams {
   long gw_stride;  // elements
 };
 
-// grad_h, a piece: acc[split][row][c] (+)= sum over the split's entries of d[row][v] w[v][c]
+// grad_h of a piece: acc[split][row][c] (+)= sum over the split's entries of d[row][v] w[v][c]
 template <class T>
-__device__ __forceinline__ void head_grad_h_tile(const GradParams& p, char* lds) {
+__device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, char* lds) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
   const int nt = __builtin_amdgcn_readfirstlane((id / p.m_tiles) % p.n_tiles);
   const int split = __builtin_amdgcn_readfirstlane(id / (p.m_tiles * p.n_tiles));
@@ -400,20 +431,20 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, char* lds)
   }
 }
 
-// (a function of its own: the host compiler cannot emit a kernel whose lambda holds a buffer descriptor)
-template <class T>
-__global__ __launch_bounds__(T::THREADS, 2) void head_grad_h_kernel(const GradParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
-  head_grad_h_tile<T>(p, lds);
-}
-
 // grad_h = the splits' accumulators, added in order, rounded once
 __global__ __launch_bounds__(256) void head_grad_h_join_kernel(const float* __restrict__ acc, int splits, long N, int D,
                                                                __bf16* __restrict__ out, long stride) {
   const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= N * D) return;
-  f32x4 v = *reinterpret_cast<const f32x4*>(acc + i);
-  for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(acc + (long)s * N * D + i);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; s += 4) {
+    f32x4 a[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) a[u] = *reinterpret_cast<const f32x4*>(acc + (long)(s + u < splits ? s + u : s) * N * D + i);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s + u < splits) v += a[u];
+  }
   const long r = i / D;
   const uint2 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
   *reinterpret_cast<uint2*>(out + r * stride + (i - r * D)) = w;
@@ -421,12 +452,10 @@ __global__ __launch_bounds__(256) void head_grad_h_join_kernel(const float* __re
 
 // grad_w, the rows of a piece: gw[v][c] = sum over rows r of d[r][v] hz[r][c]
 template <class T>
-__global__ __launch_bounds__(T::THREADS, 2) void head_grad_w_kernel(const GradParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
+__device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, char* lds) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
   const int nt = __builtin_amdgcn_readfirstlane(id / p.m_tiles);
   const unsigned lds_base = (unsigned)(size_t)lds;
@@ -475,6 +504,19 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_grad_w_kernel(const GradPa
   }
 }
 
+// Both products of a piece in one launch: the tiles of grad_h first (few, with the whole piece to sum over), those of grad_w
+// (many, with the rows to sum over) fill the compute units they leave.
+template <class TH, class TW>
+__global__ __launch_bounds__(TW::THREADS, 2) void head_grad_kernel(const GradParams p) {
+  static_assert(TH::THREADS == TW::THREADS, "");
+  __shared__ __attribute__((aligned(1024))) char lds[TH::LDS > TW::LDS ? TH::LDS : TW::LDS];
+#ifdef __HIP_DEVICE_COMPILE__  // (the host compiler cannot resolve the calls: their lambdas hold buffer descriptors)
+  const int n_h = p.m_tiles * p.n_tiles * p.splits;
+  if ((int)blockIdx.x < n_h) head_grad_h_tile<TH>(p, xcd_remap(blockIdx.x, n_h), lds);
+  else head_grad_w_tile<TW>(p, xcd_remap(blockIdx.x - n_h, gridDim.x - n_h), lds);
+#endif
+}
+
 // ------------------------------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------------------------------
@@ -482,6 +524,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void head_grad_w_kernel(const GradPa
 namespace {
 
 using TileL = Tile<4, 2, 2, 4, 2>;   // 256 entries x 256 rows, 8 waves
+using TileR = Tile<2, 1, 4, 2, 3>;   // 256 x 64, 8 waves: pieces of 256 x 256
 using TileM = Tile<2, 2, 4, 2, 3>;   // 256 x 128
 using TileS2 = Tile<1, 2, 4, 1, 3>;  // 128 x 64, 4 waves
 using TileS = Tile<1, 1, 4, 1, 4>;   // 128 x 32
@@ -498,13 +541,30 @@ int stat_parts(long n, long v) {
 
 int64_t stats_ws(long n, long v, bool conf) { return (int64_t)stat_parts(n, v) * n * (conf ? 12 : 8) + (conf ? 0 : 4 * n); }
 
-template <class T, bool CONF>
+// The grid over n_voc_tiles x N rows: whole tiles of T, pieces of TS where fewer than 96 tiles would be the last round of the
+// 256 compute units (their four pieces take about half a tile's time each: 784 tiles of 1000 rows x 50021 entries were four rounds,
+// 148 us, and are three and a half), and for up to 128 rows behind the last whole column.
+template <class T, class TS>
+long head_grid(HeadParams& p) {
+  constexpr int Q = T::TN / TS::TN;
+  const long rest = p.N % T::TN;
+  const bool cut_rest = Q > 1 && rest > 0 && rest <= T::TN / 2;
+  p.n_tok_tiles = (int)(p.N / T::TN + (rest > 0 && !cut_rest));
+  p.rest_cols = cut_rest ? (int)((rest + TS::TN - 1) / TS::TN) : 0;
+  const long whole = (long)p.n_voc_tiles * p.n_tok_tiles, last = whole % 256;
+  const long full = Q > 1 && last <= 96 ? whole - last : whole;
+  const long grid = full + Q * (whole - full) + (long)p.n_voc_tiles * p.rest_cols;
+  p.n_full = (int)full;
+  p.n_cut = (int)(Q * (whole - full));
+  return grid <= 0x7fffffffL ? grid : -1;
+}
+
+template <class T, class TS, bool CONF>
 int launch_stats(HeadParams& p, hipStream_t s) {
   p.n_voc_tiles = (int)((p.V + T::TM - 1) / T::TM);
-  p.n_tok_tiles = (int)((p.N + T::TN - 1) / T::TN);
-  const long grid = (long)p.n_voc_tiles * p.n_tok_tiles;
-  if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((head_stats_kernel<T, CONF>), dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
+  const long grid = head_grid<T, TS>(p);
+  if (grid < 0) return PDLLM_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((head_stats_kernel<T, TS, CONF>), dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
   return launch_status();
 }
 
@@ -527,10 +587,10 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
   p.part_idx = reinterpret_cast<int*>(next);
   p.xlab = next;
   int st;
-  if (p.N <= 32) st = launch_stats<TileS, CONF>(p, s);
-  else if (p.N <= 64) st = launch_stats<TileS2, CONF>(p, s);
-  else if (p.N <= 128) st = launch_stats<TileM, CONF>(p, s);
-  else st = launch_stats<TileL, CONF>(p, s);
+  if (p.N <= 32) st = launch_stats<TileS, TileS, CONF>(p, s);
+  else if (p.N <= 64) st = launch_stats<TileS2, TileS2, CONF>(p, s);
+  else if (p.N <= 128 && p.V >= 32768) st = launch_stats<TileM, TileM, CONF>(p, s);
+  else st = launch_stats<TileL, TileR, CONF>(p, s);
   if (st != PDLLM_OK) return st;
   hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)((p.N + 7) / 8)), dim3(1024), 0, s, p.part, p.part_idx, p.xlab,
                      p.labels, parts, p.N, p.V, out, lse_out, token_out);
@@ -550,40 +610,35 @@ struct GradPlan {
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
+// Pieces as long as the workspace allows, up to kPieceBytes of d: of 4096 rows 32768 entries, 128 x 16 tiles of logits and 128 x 14 of
+// grad_w (3584 columns), whole rounds of the 256 compute units.  have < 0: the size that is asked for.
 bool plan_grad(long n, long v, int d, int64_t have, GradPlan& g) {
   g.planes = n <= kPlaneRows ? 2 : 1;
   g.small = n <= 64;
   const long vall = (v + 255) / 256 * 256;
   const long tiles = ((d + 255) / 256) * (g.small ? 1 : (n + 255) / 256);
-  long most = 256 / tiles;
-  if (most < 1) most = 1;
+  const long most = tiles < 256 ? 256 / tiles : 1;
   g.hz = align256(2L * n * d);
-  auto acc_for = [&](long piece) {
-    long s = piece / 512;  // at least eight steps per split
-    s = s < 1 ? 1 : (s < most ? s : most);
-    g.splits = (int)s;
-    return align256(4L * s * n * d);
-  };
-  long piece = kPieceBytes / (2 * n * g.planes) / 256 * 256;
-  piece = piece < kMaxPiece ? piece : kMaxPiece;
-  piece = piece < 256 ? 256 : (piece < vall ? piece : vall);
-  if (have >= 0) {
-    while (piece > 256 && g.hz + align256(2L * n * piece * g.planes) + acc_for(piece) > have) piece = (piece / 2 + 255) / 256 * 256;
+  for (long piece = kPieceBytes / (2 * n * g.planes);; piece = g.vp / 2) {
+    piece = piece < kMaxPiece ? piece : kMaxPiece;
+    piece = piece >= 8192 ? piece / 4096 * 4096 : piece / 256 * 256;
+    piece = piece < 256 ? 256 : (piece < vall ? piece : vall);
+    // grad_h: enough splits of the piece for every compute unit, at least four stages each
+    const long s = piece / 256;
+    g.splits = (int)(s < 1 ? 1 : (s < most ? s : most));
+    g.ldd = g.vp = piece;
+    g.d = align256(2L * n * piece * g.planes);
+    g.acc = align256(4L * g.splits * n * d);
+    if (have < 0 || g.hz + g.d + g.acc <= have) return true;
+    if (piece <= 256) return false;
   }
-  // pieces of equal length
-  const long count = (vall + piece - 1) / piece;
-  piece = ((vall + count - 1) / count + 255) / 256 * 256;
-  g.acc = acc_for(piece);
-  g.ldd = g.vp = piece;
-  g.d = align256(2L * n * piece * g.planes);
-  return have < 0 || g.hz + g.d + g.acc <= have;
 }
 
-template <class T>
+template <class T, class TS>
 int launch_dlogits(HeadParams& p, hipStream_t s) {
-  p.n_tok_tiles = (int)((p.N + T::TN - 1) / T::TN);
-  hipLaunchKernelGGL(head_dlogits_kernel<T>, dim3((unsigned)((long)p.n_voc_tiles * p.n_tok_tiles)), dim3(T::THREADS), 0,
-                     s, p);
+  const long grid = head_grid<T, TS>(p);
+  if (grid < 0) return PDLLM_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((head_dlogits_kernel<T, TS>), dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
   return launch_status();
 }
 
@@ -688,13 +743,13 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     GradParams q = {};
     q.D = dim;
     q.planes = 1;
-    q.m_tiles = (dim + 255) / 256;
-    q.n_tiles = (int)((vocab + 255) / 256);
+    q.m_tiles = (dim + 255) / 256;  // (no tiles of grad_h: n_tiles is 0)
+    const long tiles = q.m_tiles * ((vocab + 255) / 256);
     q.vp = vocab;
     q.gw = static_cast<__bf16*>(grad_weight);
     q.gw_stride = grad_weight_stride;
-    if ((long)q.m_tiles * q.n_tiles > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(head_grad_w_kernel<TileH>, dim3((unsigned)(q.m_tiles * q.n_tiles)), dim3(TileH::THREADS), 0, s, q);
+    if (tiles > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((head_grad_kernel<TileH, TileH>), dim3((unsigned)tiles), dim3(TileH::THREADS), 0, s, q);
     return launch_status();
   }
   GradPlan g;
@@ -733,7 +788,7 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     p.v0 = v0;
     p.hz = v0 == 0 ? ws : nullptr;
     p.n_voc_tiles = (int)((vp + 255) / 256);
-    st = g.small ? launch_dlogits<TileD2>(p, s) : launch_dlogits<TileL>(p, s);
+    st = g.small ? launch_dlogits<TileD2, TileD2>(p, s) : launch_dlogits<TileL, TileR>(p, s);
     if (st != PDLLM_OK) return st;
     q.w = p.w + v0 * p.w_stride;
     q.vp = vp;
@@ -742,16 +797,10 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     q.k_per = ((vp + g.splits - 1) / g.splits + 63) / 64 * 64;
     q.gw = static_cast<__bf16*>(grad_weight) + v0 * grad_weight_stride;
     q.n_tiles = g.small ? 1 : (int)((n_rows + 255) / 256);
-    const long grid = (long)q.m_tiles * q.n_tiles * q.splits;
-    if (g.small) {
-      hipLaunchKernelGGL(head_grad_h_kernel<TileH2>, dim3((unsigned)grid), dim3(TileH2::THREADS), 0, s, q);
-    } else {
-      hipLaunchKernelGGL(head_grad_h_kernel<TileH>, dim3((unsigned)grid), dim3(TileH::THREADS), 0, s, q);
-    }
-    if ((st = launch_status()) != PDLLM_OK) return st;
-    q.n_tiles = (int)((vp + 255) / 256);
-    hipLaunchKernelGGL(head_grad_w_kernel<TileH>, dim3((unsigned)((long)q.m_tiles * q.n_tiles)), dim3(TileH::THREADS),
-                       0, s, q);
+    const long grid = (long)q.m_tiles * q.n_tiles * q.splits + (long)q.m_tiles * ((vp + 255) / 256);
+    if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+    if (g.small) hipLaunchKernelGGL((head_grad_kernel<TileH2, TileH>), dim3((unsigned)grid), dim3(TileH::THREADS), 0, s, q);
+    else hipLaunchKernelGGL((head_grad_kernel<TileH, TileH>), dim3((unsigned)grid), dim3(TileH::THREADS), 0, s, q);
     if ((st = launch_status()) != PDLLM_OK) return st;
   }
   const long quads = n_rows * (dim / 4);
