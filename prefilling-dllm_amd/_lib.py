@@ -101,6 +101,8 @@ SIGNATURES = {
     "pdllm_fp8_quantize_rows": (C.c_int, [vp, i64, i64, i32, vp, i64, vp, i64, i64, vp]),
     "pdllm_fp8_quantize_blocks": (C.c_int, [vp, i64, i64, i32, vp, i64, vp, i64, i64, vp]),
     "pdllm_fp8_linear": (C.c_int, [vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, i64, i64, i32, vp, i64, vp]),
+    "pdllm_fp8_linear_bf16_workspace_bytes": (i64, [i64, i32]),
+    "pdllm_fp8_linear_bf16": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, i64, i64, i32, vp, i64, vp, i64, vp]),
     "pdllm_anchor_delta_add": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, vp, vp, i64, vp, i64, i64, i64, i64, i32, i32,
                                          i32, i32, i32, f32, f32, i32, vp]),
 }

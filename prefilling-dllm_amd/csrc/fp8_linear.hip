@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_blocks_kernel(const char* __
 // ---- the product ---------------------------------------------------------------------------------------------------
 
 struct Fp8Params {
-  const char* x;  // [M, K] e4m3
+  const char* x;  // [M, K] e4m3 (bf16 where a kernel quantises on the way)
   const char* w;  // [N, K]
   const float* sx;
   const float* sw;
@@ -128,13 +128,12 @@ struct Fp8Params {
   int K;
   __bf16* out;
   long o_stride;  // elements
-  int vec;        // rows of the output are 8-byte aligned
   int m_tiles, n_tiles;  // tiles of output features, of rows
 };
 
 template <class T>
 __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   const unsigned lds_base = (unsigned)(size_t)lds;
@@ -305,28 +304,12 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
   for (int t = 0; t < steps - 1; ++t) stage(t, std::true_type{});
   stage(steps - 1, std::false_type{});
 
-#pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
-    const long row = r0 + (wn * T::NT + j) * 32 + l32;
-    if (row >= p.M) continue;
-#pragma unroll
-    for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const long f = fw + 32 * i + 8 * q + 4 * h;
-        if (f >= p.N) continue;
-        const long o = row * p.o_stride + f;
-        if (p.vec && f + 4 <= p.N) {
-          const uint2 v = {pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
-                           pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
-          *reinterpret_cast<uint2*>(p.out + o) = v;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (f + e < p.N) p.out[o + e] = (__bf16)acc[i][j][4 * q + e];
-        }
-      }
-  }
+  store_tile<T>(
+      lds,
+      [&](int i, int j, int q) __attribute__((always_inline)) {
+        return make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+      },
+      p.out + r0 * p.o_stride + f0, p.o_stride, p.M - r0, p.N - f0);
 }
 
 // (a function of its own: the host compiler cannot emit a kernel whose lambda holds a buffer descriptor)
@@ -340,9 +323,9 @@ __global__ __launch_bounds__(T::THREADS, 2) void fp8_linear_kernel(const Fp8Para
 // 32 features and all rows; its eight waves take every eighth block of k, so that all of the workgroup's weight (FT x K
 // bytes) is on its way at once, and their fp32 sums meet in LDS, added in wave order.  16x16x128 instruction: lane l holds row
 // l & 15 of an operand, bytes 16 (l >> 4) .. + 15 of each half of the block (any order of k that both operands share).
-template <int FT, int TT>
+template <int FT, int TT, bool BF>
 __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
-  constexpr int NF = FT / 16, U = 2;  // U blocks of a wave in flight
+  constexpr int NF = FT / 16, U = BF && TT == 2 ? 1 : 2;  // U blocks of a wave in flight (as many as the registers hold)
   __shared__ float part[8][TT * 16][FT + 1];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -350,7 +333,7 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
   const long nf = p.N - f0 < FT ? p.N - f0 : FT;
   const int m = (int)p.M;
   const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.w + f0 * p.w_stride, (unsigned)((nf - 1) * p.w_stride) + (unsigned)p.K);
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, (unsigned)((m - 1) * p.x_stride) + (unsigned)p.K);
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, (unsigned)((m - 1) * p.x_stride) + (unsigned)(BF ? 2 * p.K : p.K));
   unsigned wo[NF], xo[TT], so[TT];
 #pragma unroll
   for (int f = 0; f < NF; ++f) wo[f] = f * 16 + l16 < nf ? (unsigned)(f * 16 + l16) * (unsigned)p.w_stride : kOutOfRange;
@@ -374,6 +357,34 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
     const i32x4 b = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, k1 < (unsigned)p.K ? row + k1 : kOutOfRange, 0, 0));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   };
+  // bf16 rows: a lane's 32 values of the block, the block's scale from the four lanes that share it
+  auto load_quantized = [&](unsigned row, int kb, float& scale) __attribute__((always_inline)) {
+    uint4 v[4];
+    unsigned amax = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const unsigned k = kb * 128 + (c >> 1) * 64 + 16 * g + (c & 1) * 8;
+      v[c] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(xr, k < (unsigned)p.K ? row + 2 * k : kOutOfRange, 0, 0));
+      const unsigned b = max_bits(v[c]);
+      amax = amax > b ? amax : b;
+    }
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {
+      const unsigned b = __shfl_xor(amax, o, 64);
+      amax = amax > b ? amax : b;
+    }
+    const unsigned sb = block_scale_bits(amax);
+    scale = __uint_as_float(sb);
+    const float inv = inverse_scale(sb);
+    i32x8 r;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint2 q = to_e4m3(v[c], inv);
+      r[2 * c] = (int)q.x;
+      r[2 * c + 1] = (int)q.y;
+    }
+    return r;
+  };
   for (int b0 = wave; b0 < blocks; b0 += 8 * U) {
     i32x8 w[U][NF], x[U][TT];
     float s[U][TT];
@@ -390,8 +401,13 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
       const float ws = sw[ks * p.sw_blk];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        x[u][t] = load(xr, xo[t], kb);
-        s[u][t] = kb < blocks ? (p.sx + ks * p.sx_blk)[so[t]] * ws : 0.f;
+        if constexpr (BF) {
+          x[u][t] = load_quantized(xo[t], kb, s[u][t]);
+          s[u][t] = kb < blocks ? s[u][t] * ws : 0.f;
+        } else {
+          x[u][t] = load(xr, xo[t], kb);
+          s[u][t] = kb < blocks ? (p.sx + ks * p.sx_blk)[so[t]] * ws : 0.f;
+        }
       }
     }
 #pragma unroll
@@ -435,7 +451,7 @@ template <int R>
 constexpr long resident_lds(long blocks, long groups) {
   return blocks * R * 132 + kResidentQ * R * kResidentPad * 4 + blocks * groups * 4;
 }
-template <int TT, int U>
+template <int TT, int U, bool BF>
 __global__ __launch_bounds__(1024, 4) void fp8_resident_kernel(const Fp8Params p) {
   extern __shared__ __attribute__((aligned(1024))) char xs[];
   constexpr int R = 16 * TT;
@@ -471,16 +487,45 @@ __global__ __launch_bounds__(1024, 4) void fp8_resident_kernel(const Fp8Params p
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) fetch(ring[u]);
-  for (int i = threadIdx.x; i < blocks * R * 8; i += 1024) {
-    const int ch = i & 7, r = (i >> 3) % R, kb = (i >> 3) / R;
-    const int k = kb * 128 + 16 * ch;
-    uint4 v = {0, 0, 0, 0};
-    if (r < m && k < p.K) v = *reinterpret_cast<const uint4*>(p.x + (long)r * p.x_stride + k);
-    *reinterpret_cast<uint4*>(xs + (((kb * R + r) * 8 + (ch ^ ((r >> 1) & 7))) << 4)) = v;
-  }
-  for (int i = threadIdx.x; i < blocks * R; i += 1024) {
-    const int r = i % R, kb = i / R;
-    scales[i] = r < m ? p.sx[r * p.sx_row + kb * p.sx_blk] : 0.f;
+  if constexpr (BF) {
+    // bf16 rows: 16 lanes to a block, as the quantising kernel does it; four blocks of a lane are fetched together
+    const int l = threadIdx.x & 15, all = blocks * R;
+    for (int i0 = threadIdx.x >> 4; i0 < all; i0 += 4 * 64) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u, r = i % R, k = i / R * 128 + 8 * l;
+        v[u] = uint4{0, 0, 0, 0};
+        if (i < all && r < m && k < p.K) v[u] = *reinterpret_cast<const uint4*>(p.x + (long)r * p.x_stride + 2 * k);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u, r = i % R, kb = i / R;
+        unsigned amax = max_bits(v[u]);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+          const unsigned t = __shfl_xor(amax, o, 64);
+          amax = amax > t ? amax : t;
+        }
+        const unsigned sb = block_scale_bits(amax);
+        if (i < all) {
+          *reinterpret_cast<uint2*>(xs + (((kb * R + r) * 8 + ((l >> 1) ^ ((r >> 1) & 7))) << 4) + 8 * (l & 1)) = to_e4m3(v[u], inverse_scale(sb));
+          if (l == 0) scales[i] = __uint_as_float(sb);
+        }
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < blocks * R * 8; i += 1024) {
+      const int ch = i & 7, r = (i >> 3) % R, kb = (i >> 3) / R;
+      const int k = kb * 128 + 16 * ch;
+      uint4 v = {0, 0, 0, 0};
+      if (r < m && k < p.K) v = *reinterpret_cast<const uint4*>(p.x + (long)r * p.x_stride + k);
+      *reinterpret_cast<uint4*>(xs + (((kb * R + r) * 8 + (ch ^ ((r >> 1) & 7))) << 4)) = v;
+    }
+    for (int i = threadIdx.x; i < blocks * R; i += 1024) {
+      const int r = i % R, kb = i / R;
+      scales[i] = r < m ? p.sx[r * p.sx_row + kb * p.sx_blk] : 0.f;
+    }
   }
   const int mine = first < tasks ? (tasks - 1 - first) / per + 1 : 0;
   for (int i = threadIdx.x; i < mine * blocks; i += 1024) {
@@ -567,32 +612,44 @@ int launch_fp8(Fp8Params& p, hipStream_t s) {
   return launch_status();
 }
 
-template <int TT>
+template <int TT, bool BF>
 int launch_resident(Fp8Params& p, hipStream_t s) {
   const long blocks = (p.K + 127) / 128, groups = ((p.N + 31) / 32 + 255) / 256;
-  hipLaunchKernelGGL((fp8_resident_kernel<TT, 4>), dim3(256), dim3(1024), (unsigned)resident_lds<16 * TT>(blocks, groups), s, p);
+  hipLaunchKernelGGL((fp8_resident_kernel<TT, 4, BF>), dim3(256), dim3(1024), (unsigned)resident_lds<16 * TT>(blocks, groups), s, p);
   return launch_status();
 }
 
-int launch_stream(Fp8Params& p, hipStream_t s) {
+// up to 32 rows
+template <bool BF>
+int launch_few(Fp8Params& p, hipStream_t s) {
   const long blocks = (p.K + 127) / 128, groups = ((p.N + 31) / 32 + 255) / 256;
   // (measured, K = 3584, 152064 features: 1 row 91 us resident, 88 us streamed; 16 rows 100 and 110; 32 rows 107 and 140)
   if (p.M > 4 && p.N >= 16384 && blocks >= kResidentQ) {
-    if (p.M <= 16 && resident_lds<16>(blocks, groups) <= 160 * 1024) return launch_resident<1>(p, s);
-    if (p.M > 16 && resident_lds<32>(blocks, groups) <= 160 * 1024) return launch_resident<2>(p, s);
+    if (p.M <= 16 && resident_lds<16>(blocks, groups) <= 160 * 1024) return launch_resident<1, BF>(p, s);
+    if (p.M > 16 && resident_lds<32>(blocks, groups) <= 160 * 1024) return launch_resident<2, BF>(p, s);
   }
   // 32 features to a workgroup read the rows half as often; 16 where 32 would leave compute units idle
   const bool wide = (p.N + 31) / 32 >= 512;
   const unsigned grid = (unsigned)((p.N + (wide ? 31 : 15)) / (wide ? 32 : 16));
   if (p.M <= 16) {
-    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 1>), dim3(grid), dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fp8_stream_kernel<16, 1>), dim3(grid), dim3(512), 0, s, p);
+    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 1, BF>), dim3(grid), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fp8_stream_kernel<16, 1, BF>), dim3(grid), dim3(512), 0, s, p);
   } else {
-    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 2>), dim3(grid), dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fp8_stream_kernel<16, 2>), dim3(grid), dim3(512), 0, s, p);
+    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 2, BF>), dim3(grid), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fp8_stream_kernel<16, 2, BF>), dim3(grid), dim3(512), 0, s, p);
   }
   return launch_status();
 }
+
+int launch_many(Fp8Params& p, hipStream_t s) {
+  // The largest tile that still gives most of the 256 compute units one: tiles re-read their operands less the larger they are
+  const auto tiles = [&](long tm, long tn) { return ((p.N + tm - 1) / tm) * ((p.M + tn - 1) / tn); };
+  if (p.M > 128 && tiles(256, 256) >= 160) return launch_fp8<TileL>(p, s);
+  if (p.M > 64 && tiles(256, 128) >= 160) return launch_fp8<TileM>(p, s);
+  return launch_fp8<TileS2>(p, s);
+}
+
+constexpr int kFewRows = 32;
 
 int check_quantize(const void* x, int64_t x_stride, int64_t rows, int32_t K, const void* q, int64_t q_stride, const void* scale,
                    int64_t s_row, int64_t s_blk) {
@@ -637,41 +694,91 @@ extern "C" int pdllm_fp8_quantize_blocks(const void* w, int64_t w_stride, int64_
   return launch_status();
 }
 
-extern "C" int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_scale, int64_t x_scale_row_stride,
-                                int64_t x_scale_block_stride, const void* weight, int64_t weight_stride,
-                                const float* weight_scale, int64_t weight_scale_row_stride,
-                                int64_t weight_scale_block_stride, int64_t m, int64_t n, int32_t k, void* out,
-                                int64_t out_stride, pdllm_stream_t stream) {
-  if (m < 0 || n <= 0 || k <= 0 || k % 16 || k > (1 << 20) || m > kMaxRows || n > (1L << 30)) return PDLLM_ERR_SHAPE;
-  if (m == 0) return PDLLM_OK;
-  if (!x || !x_scale || !weight || !weight_scale || !out) return PDLLM_ERR_NULL;
-  if (x_stride < k || x_stride % 16 || weight_stride < k || weight_stride % 16 || (uintptr_t)x % 16 || (uintptr_t)weight % 16 ||
-      x_stride * 256 >= 0x7fffffffL || weight_stride * 256 >= 0x7fffffffL || out_stride < n || x_scale_row_stride < 0 ||
-      x_scale_row_stride >= (1 << 22) || x_scale_block_stride < 0 || weight_scale_row_stride < 0 || weight_scale_block_stride < 0 ||
-      (uintptr_t)out % 2)
+namespace pdllm {
+namespace {
+
+int check_linear(int64_t m, int64_t n, int32_t k) {
+  return m < 0 || n <= 0 || k <= 0 || k % 16 || k > (1 << 20) || m > kMaxRows || n > (1L << 30) ? PDLLM_ERR_SHAPE : PDLLM_OK;
+}
+// operands of elem bytes per value of x
+int check_linear_strides(const void* x, int64_t x_stride, int elem, const void* weight, int64_t weight_stride, int64_t sw_row,
+                         int64_t sw_blk, int64_t n, int32_t k, const void* out, int64_t out_stride) {
+  if (x_stride < k || (elem * x_stride) % 16 || weight_stride < k || weight_stride % 16 || (uintptr_t)x % 16 ||
+      (uintptr_t)weight % 16 || elem * x_stride * 256 >= 0x7fffffffL || weight_stride * 256 >= 0x7fffffffL || out_stride < n ||
+      sw_row < 0 || sw_blk < 0 || (uintptr_t)out % 2)
     return PDLLM_ERR_STRIDE;
+  return PDLLM_OK;
+}
+Fp8Params linear_params(const void* x, int64_t x_bytes, const void* weight, int64_t weight_stride, const float* weight_scale,
+                        int64_t sw_row, int64_t sw_blk, int64_t m, int64_t n, int32_t k, void* out, int64_t out_stride) {
   Fp8Params p = {};
   p.x = static_cast<const char*>(x);
   p.w = static_cast<const char*>(weight);
-  p.sx = x_scale;
   p.sw = weight_scale;
-  p.x_stride = x_stride;
+  p.x_stride = x_bytes;
   p.w_stride = weight_stride;
-  p.sx_row = x_scale_row_stride;
-  p.sx_blk = x_scale_block_stride;
-  p.sw_row = weight_scale_row_stride;
-  p.sw_blk = weight_scale_block_stride;
+  p.sw_row = sw_row;
+  p.sw_blk = sw_blk;
   p.M = m;
   p.N = n;
   p.K = k;
   p.out = static_cast<__bf16*>(out);
   p.o_stride = out_stride;
-  p.vec = out_stride % 4 == 0 && (uintptr_t)out % 8 == 0;
+  return p;
+}
+
+}  // namespace
+}  // namespace pdllm
+
+extern "C" int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_scale, int64_t x_scale_row_stride,
+                                int64_t x_scale_block_stride, const void* weight, int64_t weight_stride,
+                                const float* weight_scale, int64_t weight_scale_row_stride,
+                                int64_t weight_scale_block_stride, int64_t m, int64_t n, int32_t k, void* out,
+                                int64_t out_stride, pdllm_stream_t stream) {
+  int st = check_linear(m, n, k);
+  if (st != PDLLM_OK || m == 0) return st;
+  if (!x || !x_scale || !weight || !weight_scale || !out) return PDLLM_ERR_NULL;
+  st = check_linear_strides(x, x_stride, 1, weight, weight_stride, weight_scale_row_stride, weight_scale_block_stride, n, k, out,
+                            out_stride);
+  if (st != PDLLM_OK) return st;
+  if (x_scale_row_stride < 0 || x_scale_row_stride >= (1 << 22) || x_scale_block_stride < 0) return PDLLM_ERR_STRIDE;
+  Fp8Params p = linear_params(x, x_stride, weight, weight_stride, weight_scale, weight_scale_row_stride,
+                              weight_scale_block_stride, m, n, k, out, out_stride);
+  p.sx = x_scale;
+  p.sx_row = x_scale_row_stride;
+  p.sx_blk = x_scale_block_stride;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (m <= 32) return launch_stream(p, s);
-  // The largest tile that still gives most of the 256 compute units one: tiles re-read their operands less the larger they are
-  const auto tiles = [&](long tm, long tn) { return ((n + tm - 1) / tm) * ((m + tn - 1) / tn); };
-  if (m > 128 && tiles(256, 256) >= 160) return launch_fp8<TileL>(p, s);
-  if (m > 64 && tiles(256, 128) >= 160) return launch_fp8<TileM>(p, s);
-  return launch_fp8<TileS2>(p, s);
+  return m <= kFewRows ? launch_few<false>(p, s) : launch_many(p, s);
+}
+
+extern "C" int64_t pdllm_fp8_linear_bf16_workspace_bytes(int64_t m, int32_t k) {
+  if (check_linear(m, 1, k) != PDLLM_OK) return PDLLM_ERR_SHAPE;
+  return m <= kFewRows ? 0 : m * k + 4 * m * ((k + 127) / 128);
+}
+
+extern "C" int pdllm_fp8_linear_bf16(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                     const float* weight_scale, int64_t weight_scale_row_stride,
+                                     int64_t weight_scale_block_stride, int64_t m, int64_t n, int32_t k, void* workspace,
+                                     int64_t workspace_bytes, void* out, int64_t out_stride, pdllm_stream_t stream) {
+  int st = check_linear(m, n, k);
+  if (st != PDLLM_OK || m == 0) return st;
+  if (!x || !weight || !weight_scale || !out) return PDLLM_ERR_NULL;
+  st = check_linear_strides(x, x_stride, 2, weight, weight_stride, weight_scale_row_stride, weight_scale_block_stride, n, k, out,
+                            out_stride);
+  if (st != PDLLM_OK) return st;
+  Fp8Params p = linear_params(x, 2 * x_stride, weight, weight_stride, weight_scale, weight_scale_row_stride,
+                              weight_scale_block_stride, m, n, k, out, out_stride);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (m <= kFewRows) return launch_few<true>(p, s);  // quantised where they are read: one launch
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < pdllm_fp8_linear_bf16_workspace_bytes(m, k)) return PDLLM_ERR_WORKSPACE;
+  char* q = static_cast<char*>(workspace);
+  float* scale = reinterpret_cast<float*>(q + m * k);
+  st = pdllm_fp8_quantize_rows(x, x_stride, m, k, q, k, scale, 1, m, stream);
+  if (st != PDLLM_OK) return st;
+  p.x = q;
+  p.x_stride = k;
+  p.sx = scale;
+  p.sx_row = 1;
+  p.sx_blk = m;
+  return launch_many(p, s);
 }

@@ -302,4 +302,71 @@ __device__ __forceinline__ void mainloop_bf16(f32x16 (&acc)[T::MT][T::NT], int s
   mul(1);
 }
 
+// A tile of bf16 results to memory through LDS, so that a row's columns leave in one piece (a lane's four columns at a time,
+// straight from the registers, every store touches 32 rows).  get(i, j, q): columns 32 i + 8 q + 4 h .. + 3 of the wave's
+// block, row block j, packed.  out: row 0, column 0 of the tile; rows, cols: how much of it exists.  Chunk c of row r lies at
+// c ^ (r & 15).
+template <class T, class Get>
+__device__ __forceinline__ void store_tile(char* lds, Get&& get, __bf16* out, long stride, long rows, long cols) {
+  constexpr int CH = T::TM / 8;  // chunks of a row
+  static_assert(T::TM * T::TN * 2 <= T::LDS && CH >= 16, "the results take the place of the operands");
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  __syncthreads();  // the tile's operands are done with
+#pragma unroll
+  for (int j = 0; j < T::NT; ++j) {
+    const int r = (wn * T::NT + j) * 32 + l32;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = (wm * T::MT + i) * 4 + q;
+        *reinterpret_cast<uint2*>(lds + (r * CH + (c ^ (r & 15))) * 16 + 8 * h) = get(i, j, q);
+      }
+  }
+  __syncthreads();
+  const int nr = rows < T::TN ? (int)rows : T::TN, nc = cols < T::TM ? (int)cols : T::TM;
+  const unsigned odd = (unsigned)(uintptr_t)out | (unsigned)(2 * stride);
+  if (odd % 16 == 0) {
+    for (int k = threadIdx.x; k < nr * CH; k += T::THREADS) {
+      const int r = k / CH, c = k % CH;
+      const uint4 v = *reinterpret_cast<const uint4*>(lds + (r * CH + (c ^ (r & 15))) * 16);
+      __bf16* o = out + r * stride + 8 * c;
+      if (8 * c + 8 <= nc) {
+        *reinterpret_cast<uint4*>(o) = v;
+      } else {
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (8 * c + e < nc) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  } else if (odd % 4 == 0) {
+    for (int k = threadIdx.x; k < nr * (T::TM / 2); k += T::THREADS) {
+      const int r = k / (T::TM / 2), c = k % (T::TM / 2);
+      const unsigned v = *reinterpret_cast<const unsigned*>(lds + (r * CH + ((c >> 2) ^ (r & 15))) * 16 + 4 * (c & 3));
+      __bf16* o = out + r * stride + 2 * c;
+      if (2 * c + 2 <= nc) *reinterpret_cast<unsigned*>(o) = v;
+      else if (2 * c < nc) *reinterpret_cast<unsigned short*>(o) = (unsigned short)v;
+    }
+  } else {
+    // rows that begin between two words: word k of a row holds its elements 2 k - p and 2 k - p + 1, p = the row's parity
+    constexpr int WORDS = T::TM / 2 + 1;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nr * WORDS; i += T::THREADS) {
+      const int r = i / WORDS, k = i % WORDS;
+      unsigned short* o = reinterpret_cast<unsigned short*>(out + r * stride);
+      const int c = 2 * k - ((int)((uintptr_t)o >> 1) & 1);
+      auto at = [&](int e) __attribute__((always_inline)) {
+        return *reinterpret_cast<const unsigned short*>(lds + (r * CH + ((e >> 3) ^ (r & 15))) * 16 + 2 * (e & 7));
+      };
+      const unsigned lo = c >= 0 ? at(c) : 0u, hi = c + 1 < T::TM ? at(c + 1) : 0u;
+      if (c >= 0 && c + 1 < nc) *reinterpret_cast<unsigned*>(o + c) = lo | hi << 16;
+      else if (c >= 0 && c < nc) o[c] = (unsigned short)lo;
+      else if (c < 0) o[0] = (unsigned short)hi;
+    }
+  }
+}
+
 }  // namespace pdllm

@@ -9,6 +9,7 @@
 //   d[r, v] = -g[r] exp(z[r, v] - lse[r]) (v != l),  d[r, l] = -g[r] expm1(logp[r]);  grad_h = d w,  grad_w = d^T h.
 
 #include "gemm_core.h"
+#include "unmask_rule.h"
 
 namespace pdllm {
 
@@ -26,9 +27,11 @@ struct HeadParams {
   // tiles (see head_grid): n_full whole tiles, n_cut pieces of 64 rows of whole tiles, then the rows behind the whole columns
   int n_tok_tiles, n_voc_tiles, n_full, n_cut, rest_cols;
   // statistics
-  float2* part;   // [parts][N]: maximum and sum over the part's entries (the label's excluded when labels are given)
-  int* part_idx;  // [parts][N]: position of the maximum
+  float2* part;   // [N][parts]: maximum and sum over the part's entries (the label's excluded when labels are given)
+  int* part_idx;  // [N][parts]: position of the maximum
+  int parts;
   float* xlab;    // [N]: logit of the label
+  int* joined;    // workgroups of the joining kernel that are done (cleared by this one), or NULL
   // gradient
   const float* lse;
   const float* logp;
@@ -189,7 +192,7 @@ __device__ __forceinline__ void head_stats_tile(const HeadParams& p, int vt, lon
     Stat a = sh[0];
 #pragma unroll
     for (int q = 1; q < T::WM; ++q) a = stat_join(a, sh[q * T::TN]);
-    const long o = (long)vt * p.N + row;
+    const long o = row * p.parts + vt;
     p.part[o] = make_float2(a.m, a.s);
     if constexpr (CONF) p.part_idx[o] = a.idx;
   }
@@ -220,52 +223,81 @@ __device__ __forceinline__ void head_dispatch(const HeadParams& p, F&& tile) {
 template <class T, class TS, bool CONF>
 __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS > TS::LDS ? T::LDS : TS::LDS];
+  if (CONF && p.joined && blockIdx.x == 0 && threadIdx.x == 0) *p.joined = 0;
   head_dispatch<T, TS>(p, [&](auto* t, int vt, long row0) __attribute__((always_inline)) {
     head_stats_tile<std::remove_pointer_t<decltype(t)>, CONF>(p, vt, row0, lds);
   });
 }
 
-// Joins the parts of 8 rows per workgroup, 128 threads to a row, in a fixed order; four parts of a thread are fetched at a
-// time (one after the other their latency was the kernel's time: 32 rows x 1188 parts 12.8 -> TODO us).
+// Joins the parts of a row in a fixed order: a workgroup's 256 threads for one row, or a wave where a row has few parts.  The parts of
+// a row lie side by side and are fetched four at a time by a thread (32 rows x 1188 parts: 12.8 us with the parts of 16
+// rows interleaved and one fetch after the other, 7.9 us so).
+struct UnmaskParams {
+  long* block_ids;  // NULL: no transfer
+  long n_seqs, block_len, mask_token_id;
+  float threshold;
+  uint8_t* transfer;
+  int* n_left;
+  int* joined;
+};
+
 template <bool CONF>
-__global__ __launch_bounds__(1024) void head_join_kernel(const float2* __restrict__ part, const int* __restrict__ part_idx,
+__global__ __launch_bounds__(256) void head_join_kernel(const float2* __restrict__ part, const int* __restrict__ part_idx,
                                                          const float* __restrict__ xlab, const long* __restrict__ labels,
-                                                         int parts, long N, long V, float* __restrict__ out,
-                                                         float* __restrict__ lse_out, long* __restrict__ token_out) {
-  __shared__ Stat sh[16][8];
-  const int r = threadIdx.x & 7;
-  const long row = (long)blockIdx.x * 8 + r;
+                                                         int parts, long N, long V, float* out, float* __restrict__ lse_out,
+                                                         long* token_out, const UnmaskParams un) {
+  __shared__ Stat sh[4];
+  const int per = parts > 256 ? 256 : 64;  // threads of a row
+  const int at = threadIdx.x & (per - 1);
+  const long row = (long)blockIdx.x * (256 / per) + threadIdx.x / per;
   Stat a = {-INFINITY, 0.f, 0x7fffffff};
   if (row < N) {
-    for (int q = threadIdx.x >> 3; q < parts; q += 512) {
-      float2 v[4];
+    const float2* v = part + row * parts;
+    const int* vi = part_idx + row * parts;
+    for (int q = at; q < parts; q += 4 * per) {
+      float2 x[4];
       int idx[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const bool on = q + 128 * u < parts;
-        const long at = (long)(on ? q + 128 * u : q) * N + row;
-        v[u] = part[at];
-        idx[u] = CONF ? part_idx[at] : 0;
-        if (!on) v[u] = make_float2(-INFINITY, 0.f);
+        const bool on = q + per * u < parts;
+        x[u] = v[on ? q + per * u : q];
+        idx[u] = CONF ? vi[on ? q + per * u : q] : 0;
+        if (!on) x[u] = make_float2(-INFINITY, 0.f);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) a = stat_join(a, {v[u].x, v[u].y, idx[u]});
+      for (int u = 0; u < 4; ++u) a = stat_join(a, {x[u].x, x[u].y, idx[u]});
     }
   }
 #pragma unroll
-  for (int o = 8; o < 64; o <<= 1) {
+  for (int o = 1; o < 64; o <<= 1) {
     const Stat b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.idx, o, 64)};
     a = stat_join(a, b);
   }
-  if ((threadIdx.x & 63) < 8) sh[threadIdx.x >> 6][r] = a;
-  __syncthreads();
-  if (threadIdx.x >= 8 || row >= N) return;
-  a = sh[0][r];
-  for (int q = 1; q < 16; ++q) a = stat_join(a, sh[q][r]);
+  if (per == 256) {
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = sh[0];
+    for (int q = 1; q < 4; ++q) a = stat_join(a, sh[q]);
+  }
+  const bool writes = at == 0 && row < N;
   if constexpr (CONF) {
-    out[row] = 1.f / a.s;
-    token_out[row] = a.idx == 0x7fffffff ? 0 : a.idx;  // a row of NaN alone has no maximum
+    if (writes) {
+      out[row] = 1.f / a.s;
+      token_out[row] = a.idx == 0x7fffffff ? 0 : a.idx;  // a row of NaN alone has no maximum
+    }
+    if (!un.block_ids) return;
+    // the workgroup that is done last makes the step's transfers (its order decides nothing: it sees every row's result)
+    __shared__ int last;
+    if (writes) __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(un.joined, 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (long b = threadIdx.x >> 6; b < un.n_seqs; b += 4)
+      unmask_block(out, token_out, un.block_ids, b, un.block_len, un.mask_token_id, un.threshold, un.transfer, un.n_left);
   } else {
+    if (!writes) return;
     const float L = a.m + logf(a.s);
     const long lab = labels[row];
     if (lab < 0 || lab >= V) {
@@ -296,40 +328,57 @@ __device__ __forceinline__ void head_dlogits_tile(const HeadParams& p, int vt, l
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const long vl = (long)vt * T::TM + wm * (32 * T::MT);  // first entry of the wave, in the piece
+  const long vl = (long)vt * T::TM + wm * (32 * T::MT);                             // first entry of the wave, in the piece
+  const long left = p.V - p.v0 - vl;                                               // entries of the vocabulary from there on
+  const int end = left < 0 ? 0 : left < 32 * T::MT ? (int)left : 32 * T::MT;
 #pragma unroll
   for (int j = 0; j < T::NT; ++j) {
     const long row = row0 + (wn * T::NT + j) * 32 + l32;
-    if (row >= p.N) continue;
-    const long lab = p.labels[row];
+    const long lab = row < p.N ? p.labels[row] : -1;
     const bool in = lab >= 0 && lab < p.V;
-    const float lse = p.lse[row], g = p.g[row];
-    const float at_label = -g * expm1f(p.logp[row]);
-    const long rel = in ? lab - p.v0 - vl : -1;
-    const long left = p.V - p.v0 - vl;  // entries of the vocabulary from the wave's first on
+    const float lse = in ? p.lse[row] : 0.f, g = in ? p.g[row] : 0.f;
 #pragma unroll
     for (int i = 0; i < T::MT; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at = 32 * i + row_of(4 * q + e, h);
-          float v = -g * __builtin_amdgcn_exp2f((acc[i][j][4 * q + e] - lse) * kLog2eH);
-          v = at == rel ? at_label : v;
-          y[e] = in && at < left ? v : 0.f;
-        }
-        const long o = row * p.ldd + vl + 32 * i + row_of(4 * q, h);
-        uint2 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-        *reinterpret_cast<uint2*>(p.d + o) = w;
-        if (p.dlo) {
-          uint2 l;
-          l.x = pack_bf16x2(y[0] - __uint_as_float(w.x << 16), y[1] - __uint_as_float(w.x & 0xffff0000u));
-          l.y = pack_bf16x2(y[2] - __uint_as_float(w.y << 16), y[3] - __uint_as_float(w.y & 0xffff0000u));
-          *reinterpret_cast<uint2*>(p.dlo + o) = l;
-        }
+      for (int e = 0; e < 16; ++e) {
+        const float y = -g * __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * kLog2eH);
+        acc[i][j][e] = in ? y : 0.f;  // (a row without a label may hold anything)
       }
+    const long rel = lab - p.v0 - vl;
+    const bool mine = in && rel >= 0 && rel < 32 * T::MT;
+    if (__builtin_amdgcn_ballot_w64(mine) != 0) {
+      const int at = mine ? (int)rel : -1;
+      const float y = mine ? -g * expm1f(p.logp[row]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (at == 32 * i + row_of(e, h)) acc[i][j][e] = y;
+    }
   }
+  if (end < 32 * T::MT) {  // entries behind the vocabulary: zeros, which the products read
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (32 * i + row_of(e, h) >= end)
+#pragma unroll
+          for (int j = 0; j < T::NT; ++j) acc[i][j][e] = 0.f;
+  }
+  auto hi = [&](int i, int j, int q) __attribute__((always_inline)) {
+    return make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+  };
+  const long o = row0 * p.ldd + (long)vt * T::TM;
+  store_tile<T>(lds, hi, p.d + o, p.ldd, p.N - row0, T::TM);
+  if (p.dlo)
+    store_tile<T>(
+        lds,
+        [&](int i, int j, int q) __attribute__((always_inline)) {
+          const uint2 w = hi(i, j, q);
+          return make_uint2(pack_bf16x2(acc[i][j][4 * q] - __uint_as_float(w.x << 16), acc[i][j][4 * q + 1] - __uint_as_float(w.x & 0xffff0000u)),
+                            pack_bf16x2(acc[i][j][4 * q + 2] - __uint_as_float(w.y << 16), acc[i][j][4 * q + 3] - __uint_as_float(w.y & 0xffff0000u)));
+        },
+        p.dlo + o, p.ldd, p.N - row0, T::TM);
 }
 
 template <class T, class TS>
@@ -362,8 +411,11 @@ struct GradParams {
   long vp;         // entries of the piece
   int D, planes;
   int m_tiles, n_tiles, splits;  // of grad_h: column tiles, row tiles, splits of the entries
+  int w_tiles;                   // of grad_w: column tiles
   long k_per;      // entries per split, a multiple of 64
   float* acc;      // [splits][N][D]
+  __bf16* gh;      // written directly when the one split of the one piece is all of the sum
+  long gh_stride;  // elements
   int add;         // the accumulators hold earlier pieces
   __bf16* gw;      // rows of grad_w from the piece's first on
   long gw_stride;  // elements
@@ -425,6 +477,10 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, ch
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+        if (p.gh) {
+          *reinterpret_cast<uint2*>(p.gh + row * p.gh_stride + c) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+          continue;
+        }
         if (p.add) v += *reinterpret_cast<const f32x4*>(out + c);
         *reinterpret_cast<f32x4*>(out + c) = v;
       }
@@ -453,11 +509,10 @@ __global__ __launch_bounds__(256) void head_grad_h_join_kernel(const float* __re
 // grad_w, the rows of a piece: gw[v][c] = sum over rows r of d[r][v] hz[r][c]
 template <class T>
 __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, char* lds) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / T::WN, wn = wave % T::WN;
-  const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
-  const int nt = __builtin_amdgcn_readfirstlane(id / p.m_tiles);
+  const int mt = __builtin_amdgcn_readfirstlane(id % p.w_tiles);
+  const int nt = __builtin_amdgcn_readfirstlane(id / p.w_tiles);
   const unsigned lds_base = (unsigned)(size_t)lds;
   constexpr int SK = T::KB / 2;  // rows per stage
   const int steps = (int)((p.N + SK - 1) / SK);
@@ -486,28 +541,20 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
           lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
         }
       });
-#pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
-    const long v = v0 + (wn * T::NT + j) * 32 + l32;
-    if (v >= p.vp) continue;
-    __bf16* out = p.gw + v * p.gw_stride;
-#pragma unroll
-    for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = c0 + wm * (32 * T::MT) + 32 * i + row_of(4 * q, h);
-        if (c >= p.D) continue;
-        const uint2 w = {pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
-                         pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
-        *reinterpret_cast<uint2*>(out + c) = w;
-      }
-  }
+  store_tile<T>(
+      lds,
+      [&](int i, int j, int q) __attribute__((always_inline)) {
+        return make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+      },
+      p.gw + v0 * p.gw_stride + c0, p.gw_stride, p.vp - v0, p.D - c0);
 }
 
 // Both products of a piece in one launch: the tiles of grad_h first (few, with the whole piece to sum over), those of grad_w
 // (many, with the rows to sum over) fill the compute units they leave.
+// The small tiles (80 KB of LDS, at most 128 registers) leave room for two workgroups on a compute unit, which hide each other's
+// start and end: with few rows a tile of grad_w is two or three stages and then 64 KB of results.
 template <class TH, class TW>
-__global__ __launch_bounds__(TW::THREADS, 2) void head_grad_kernel(const GradParams p) {
+__global__ __launch_bounds__(TW::THREADS, TW::MT * TW::NT <= 2 ? 4 : 2) void head_grad_kernel(const GradParams p) {
   static_assert(TH::THREADS == TW::THREADS, "");
   __shared__ __attribute__((aligned(1024))) char lds[TH::LDS > TW::LDS ? TH::LDS : TW::LDS];
 #ifdef __HIP_DEVICE_COMPILE__  // (the host compiler cannot resolve the calls: their lambdas hold buffer descriptors)
@@ -539,7 +586,7 @@ int stat_parts(long n, long v) {
   return (int)((v + tm - 1) / tm);
 }
 
-int64_t stats_ws(long n, long v, bool conf) { return (int64_t)stat_parts(n, v) * n * (conf ? 12 : 8) + (conf ? 0 : 4 * n); }
+int64_t stats_ws(long n, long v, bool conf) { return (int64_t)stat_parts(n, v) * n * (conf ? 12 : 8) + (conf ? 4 : 4 * n); }
 
 // The grid over n_voc_tiles x N rows: whole tiles of T, pieces of TS where fewer than 96 tiles would be the last round of the
 // 256 compute units (their four pieces take about half a tile's time each: 784 tiles of 1000 rows x 50021 entries were four rounds,
@@ -579,21 +626,22 @@ int check_head(const void* hidden, int64_t h_stride, const void* weight, int64_t
 
 template <bool CONF>
 int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, float* lse_out, long* token_out,
-          hipStream_t s) {
+          UnmaskParams un, hipStream_t s) {
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < stats_ws(p.N, p.V, CONF)) return PDLLM_ERR_WORKSPACE;
-  const int parts = stat_parts(p.N, p.V);
+  const int parts = p.parts = stat_parts(p.N, p.V);
   p.part = static_cast<float2*>(workspace);
   float* next = reinterpret_cast<float*>(p.part + (long)parts * p.N);
   p.part_idx = reinterpret_cast<int*>(next);
   p.xlab = next;
+  if (un.block_ids) p.joined = un.joined = p.part_idx + (long)parts * p.N;
   int st;
   if (p.N <= 32) st = launch_stats<TileS, TileS, CONF>(p, s);
   else if (p.N <= 64) st = launch_stats<TileS2, TileS2, CONF>(p, s);
   else if (p.N <= 128 && p.V >= 32768) st = launch_stats<TileM, TileM, CONF>(p, s);
   else st = launch_stats<TileL, TileR, CONF>(p, s);
   if (st != PDLLM_OK) return st;
-  hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)((p.N + 7) / 8)), dim3(1024), 0, s, p.part, p.part_idx, p.xlab,
-                     p.labels, parts, p.N, p.V, out, lse_out, token_out);
+  hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)(parts > 256 ? p.N : (p.N + 3) / 4)), dim3(256), 0, s, p.part, p.part_idx, p.xlab,
+                     p.labels, parts, p.N, p.V, out, lse_out, token_out, un);
   return launch_status();
 }
 
@@ -604,7 +652,8 @@ constexpr int kPlaneRows = 64;            // up to here the second plane is carr
 
 struct GradPlan {
   long planes, ldd, vp;  // ldd = entries of a piece (a multiple of 256)
-  int splits, small;     // small: tiles of 64 rows for grad_h
+  int splits, small;     // small: the small tiles
+  int direct;            // grad_h needs no accumulators
   int64_t hz, d, acc;    // bytes
 };
 
@@ -614,10 +663,12 @@ int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 // grad_w (3584 columns), whole rounds of the 256 compute units.  have < 0: the size that is asked for.
 bool plan_grad(long n, long v, int d, int64_t have, GradPlan& g) {
   g.planes = n <= kPlaneRows ? 2 : 1;
-  g.small = n <= 64;
   const long vall = (v + 255) / 256 * 256;
-  const long tiles = ((d + 255) / 256) * (g.small ? 1 : (n + 255) / 256);
-  const long most = tiles < 256 ? 256 / tiles : 1;
+  // the small tiles where the sums over rows are short or the large ones would leave compute units idle
+  g.small = n <= 256 || ((d + 255) / 256) * (vall / 256) < 192;
+  const long tiles = ((d + 255) / 256) * (g.small ? (n + 63) / 64 : (n + 255) / 256);
+  const long slots = g.small ? 512 : 256;  // workgroups at a time
+  const long most = tiles < slots ? slots / tiles : 1;
   g.hz = align256(2L * n * d);
   for (long piece = kPieceBytes / (2 * n * g.planes);; piece = g.vp / 2) {
     piece = piece < kMaxPiece ? piece : kMaxPiece;
@@ -628,7 +679,10 @@ bool plan_grad(long n, long v, int d, int64_t have, GradPlan& g) {
     g.splits = (int)(s < 1 ? 1 : (s < most ? s : most));
     g.ldd = g.vp = piece;
     g.d = align256(2L * n * piece * g.planes);
-    g.acc = align256(4L * g.splits * n * d);
+    // a short sum is not split: the launch that would join the splits costs more than 16 stages
+    g.direct = piece >= vall && (g.splits == 1 || vall <= 1024);
+    if (g.direct) g.splits = 1;
+    g.acc = g.direct ? 0 : align256(4L * g.splits * n * d);
     if (have < 0 || g.hz + g.d + g.acc <= have) return true;
     if (piece <= 256) return false;
   }
@@ -643,8 +697,8 @@ int launch_dlogits(HeadParams& p, hipStream_t s) {
 }
 
 using TileH = Tile<4, 2, 2, 4, 2>;  // grad_h, grad_w: 256 columns x 256 rows or entries
-using TileH2 = Tile<1, 2, 8, 1, 3>;  // 256 columns x 64 rows
-using TileD2 = Tile<1, 2, 8, 1, 3>;  // softmax gradient of up to 64 rows: 256 entries x 64 rows
+using TileH2 = Tile<1, 2, 8, 1, 2>;  // grad_h of small problems: 256 columns x 64 rows
+using TileW2 = Tile<1, 2, 4, 2, 2>;  // grad_w of small problems: 128 columns x 128 entries
 
 }  // namespace
 
@@ -654,6 +708,7 @@ using namespace pdllm;
 
 extern "C" int64_t pdllm_head_workspace_bytes(int64_t n_rows, int64_t vocab) {
   if (n_rows < 0 || vocab <= 0 || n_rows > kMaxRows || vocab > kMaxVocab) return PDLLM_ERR_SHAPE;
+  if (n_rows == 0) return 0;
   const int64_t a = stats_ws(n_rows, vocab, true), b = stats_ws(n_rows, vocab, false);
   return a > b ? a : b;
 }
@@ -675,13 +730,16 @@ extern "C" int pdllm_head_selfinfo_logprob(const void* hidden, int64_t hidden_st
   p.D = dim;
   p.block_len = 1;
   p.labels = reinterpret_cast<const long*>(labels);
-  return stats<false>(p, workspace, workspace_bytes, logp_out, lse_out, nullptr, static_cast<hipStream_t>(stream));
+  return stats<false>(p, workspace, workspace_bytes, logp_out, lse_out, nullptr, {}, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int pdllm_head_conf_argmax(const void* hidden, int64_t hidden_stride, const void* last_hidden,
-                                      int64_t last_hidden_stride, const void* weight, int64_t weight_stride, int64_t n_seqs,
-                                      int64_t block_len, int64_t vocab, int32_t dim, int32_t shift, void* workspace,
-                                      int64_t workspace_bytes, float* conf_out, int64_t* token_out, pdllm_stream_t stream) {
+namespace pdllm {
+namespace {
+
+int conf_argmax(const void* hidden, int64_t hidden_stride, const void* last_hidden, int64_t last_hidden_stride,
+                const void* weight, int64_t weight_stride, int64_t n_seqs, int64_t block_len, int64_t vocab, int32_t dim,
+                int32_t shift, void* workspace, int64_t workspace_bytes, float* conf_out, int64_t* token_out,
+                const UnmaskParams& un, pdllm_stream_t stream) {
   if (n_seqs < 0 || block_len <= 0 || block_len > kMaxRows || n_seqs > kMaxRows) return PDLLM_ERR_SHAPE;
   const int64_t n = n_seqs * block_len;
   int st = check_head(hidden, hidden_stride, weight, weight_stride, n, vocab, dim);
@@ -700,8 +758,19 @@ extern "C" int pdllm_head_conf_argmax(const void* hidden, int64_t hidden_stride,
   p.D = dim;
   p.block_len = (int)block_len;
   p.shift = shift ? 1 : 0;
-  return stats<true>(p, workspace, workspace_bytes, conf_out, nullptr, reinterpret_cast<long*>(token_out),
+  return stats<true>(p, workspace, workspace_bytes, conf_out, nullptr, reinterpret_cast<long*>(token_out), un,
                      static_cast<hipStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace pdllm
+
+extern "C" int pdllm_head_conf_argmax(const void* hidden, int64_t hidden_stride, const void* last_hidden,
+                                      int64_t last_hidden_stride, const void* weight, int64_t weight_stride, int64_t n_seqs,
+                                      int64_t block_len, int64_t vocab, int32_t dim, int32_t shift, void* workspace,
+                                      int64_t workspace_bytes, float* conf_out, int64_t* token_out, pdllm_stream_t stream) {
+  return conf_argmax(hidden, hidden_stride, last_hidden, last_hidden_stride, weight, weight_stride, n_seqs, block_len, vocab, dim,
+                     shift, workspace, workspace_bytes, conf_out, token_out, {}, stream);
 }
 
 extern "C" int pdllm_head_denoise_unmask(const void* hidden, int64_t hidden_stride, const void* last_hidden,
@@ -711,9 +780,13 @@ extern "C" int pdllm_head_denoise_unmask(const void* hidden, int64_t hidden_stri
                                          int64_t workspace_bytes, float* conf_out, int64_t* token_out, uint8_t* transfer_out,
                                          int32_t* n_masked_left, pdllm_stream_t stream) {
   if (n_seqs > 0 && (!block_ids || !transfer_out)) return PDLLM_ERR_NULL;
-  const int st = pdllm_head_conf_argmax(hidden, hidden_stride, last_hidden, last_hidden_stride, weight, weight_stride, n_seqs,
-                                        block_len, vocab, dim, shift, workspace, workspace_bytes, conf_out, token_out, stream);
-  if (st != PDLLM_OK || n_seqs == 0) return st;
+  // up to 32 blocks the last workgroup of the joining kernel makes the transfers (one launch less); more of them are quicker
+  // done by a launch of their own
+  UnmaskParams un = {};
+  if (n_seqs <= 32) un = {reinterpret_cast<long*>(block_ids), (long)n_seqs, (long)block_len, (long)mask_token_id, threshold, transfer_out, n_masked_left, nullptr};
+  const int st = conf_argmax(hidden, hidden_stride, last_hidden, last_hidden_stride, weight, weight_stride, n_seqs, block_len, vocab,
+                             dim, shift, workspace, workspace_bytes, conf_out, token_out, un, stream);
+  if (st != PDLLM_OK || n_seqs <= 32) return st;
   return pdllm_threshold_unmask(conf_out, token_out, block_ids, n_seqs, block_len, mask_token_id, threshold, transfer_out,
                                 n_masked_left, stream);
 }
@@ -743,8 +816,8 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     GradParams q = {};
     q.D = dim;
     q.planes = 1;
-    q.m_tiles = (dim + 255) / 256;  // (no tiles of grad_h: n_tiles is 0)
-    const long tiles = q.m_tiles * ((vocab + 255) / 256);
+    q.w_tiles = (dim + 255) / 256;  // (no tiles of grad_h)
+    const long tiles = q.w_tiles * ((vocab + 255) / 256);
     q.vp = vocab;
     q.gw = static_cast<__bf16*>(grad_weight);
     q.gw_stride = grad_weight_stride;
@@ -781,14 +854,21 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
   q.D = dim;
   q.planes = (int)g.planes;
   q.m_tiles = (dim + 255) / 256;
+  const int tw = g.small ? TileW2::TM : TileH::TM;
+  static_assert(TileW2::TM == TileW2::TN && TileH::TM == TileH::TN, "square tiles");
+  q.w_tiles = (dim + tw - 1) / tw;
+  q.n_tiles = (int)(g.small ? (n_rows + TileH2::TN - 1) / TileH2::TN : (n_rows + TileH::TN - 1) / TileH::TN);
   q.acc = reinterpret_cast<float*>(ws + g.hz + g.d);
   q.gw_stride = grad_weight_stride;
+  q.gh = g.direct ? static_cast<__bf16*>(grad_hidden) : nullptr;
+  q.gh_stride = grad_hidden_stride;
+  const bool few = n_rows <= 64;
   for (long v0 = 0; v0 < vocab; v0 += g.vp) {
     const long vp = vocab - v0 < g.vp ? vocab - v0 : g.vp;
     p.v0 = v0;
     p.hz = v0 == 0 ? ws : nullptr;
-    p.n_voc_tiles = (int)((vp + 255) / 256);
-    st = g.small ? launch_dlogits<TileD2, TileD2>(p, s) : launch_dlogits<TileL, TileR>(p, s);
+    p.n_voc_tiles = (int)((vp + (few ? TileS2::TM : TileL::TM) - 1) / (few ? TileS2::TM : TileL::TM));
+    st = few ? launch_dlogits<TileS2, TileS2>(p, s) : launch_dlogits<TileL, TileR>(p, s);
     if (st != PDLLM_OK) return st;
     q.w = p.w + v0 * p.w_stride;
     q.vp = vp;
@@ -796,13 +876,13 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     q.splits = g.splits;
     q.k_per = ((vp + g.splits - 1) / g.splits + 63) / 64 * 64;
     q.gw = static_cast<__bf16*>(grad_weight) + v0 * grad_weight_stride;
-    q.n_tiles = g.small ? 1 : (int)((n_rows + 255) / 256);
-    const long grid = (long)q.m_tiles * q.n_tiles * q.splits + (long)q.m_tiles * ((vp + 255) / 256);
+    const long grid = (long)q.m_tiles * q.n_tiles * q.splits + (long)q.w_tiles * ((vp + tw - 1) / tw);
     if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
-    if (g.small) hipLaunchKernelGGL((head_grad_kernel<TileH2, TileH>), dim3((unsigned)grid), dim3(TileH::THREADS), 0, s, q);
+    if (g.small) hipLaunchKernelGGL((head_grad_kernel<TileH2, TileW2>), dim3((unsigned)grid), dim3(TileW2::THREADS), 0, s, q);
     else hipLaunchKernelGGL((head_grad_kernel<TileH, TileH>), dim3((unsigned)grid), dim3(TileH::THREADS), 0, s, q);
     if ((st = launch_status()) != PDLLM_OK) return st;
   }
+  if (g.direct) return PDLLM_OK;
   const long quads = n_rows * (dim / 4);
   hipLaunchKernelGGL(head_grad_h_join_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, q.acc, g.splits, n_rows,
                      dim, static_cast<__bf16*>(grad_hidden), grad_hidden_stride);

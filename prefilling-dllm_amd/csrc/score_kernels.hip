@@ -10,7 +10,7 @@
 
 #include <mutex>
 
-#include "pdllm_common.h"
+#include "unmask_rule.h"
 
 namespace pdllm {
 
@@ -297,39 +297,7 @@ __global__ __launch_bounds__(64) void threshold_unmask_kernel(
     const float* __restrict__ conf, const long* __restrict__ token, long* __restrict__ block_ids,
     long block_len, long mask_token_id, float threshold, uint8_t* __restrict__ transfer,
     int* __restrict__ n_left) {
-  const long b = blockIdx.x;
-  const int lane = threadIdx.x;
-  const long base = b * block_len;
-  // pass 1: most confident masked position (lowest index on ties)
-  float best = -INFINITY;
-  long besti = 0x7fffffffffffffffL;
-  int n_masked = 0;
-  for (long i = lane; i < block_len; i += 64) {
-    if (block_ids[base + i] == mask_token_id) {
-      ++n_masked;
-      const float c = conf[base + i];
-      if (c > best || besti == 0x7fffffffffffffffL) { best = c; besti = i; }
-    }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ob = __shfl_xor(best, o, 64);
-    const long oi = __shfl_xor(besti, o, 64);
-    n_masked += __shfl_xor(n_masked, o, 64);
-    const bool o_valid = oi != 0x7fffffffffffffffL, s_valid = besti != 0x7fffffffffffffffL;
-    const bool take = o_valid && (!s_valid || ob > best || (ob == best && oi < besti));
-    if (take) { best = ob; besti = oi; }
-  }
-  int moved = 0;
-  for (long i = lane; i < block_len; i += 64) {
-    const bool masked = block_ids[base + i] == mask_token_id;
-    const bool t = masked && (i == besti || conf[base + i] >= threshold);
-    transfer[base + i] = t ? 1 : 0;
-    if (t) { block_ids[base + i] = token[base + i]; ++moved; }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) moved += __shfl_xor(moved, o, 64);
-  if (lane == 0 && n_left) n_left[b] = n_masked - moved;
+  unmask_block(conf, token, block_ids, blockIdx.x, block_len, mask_token_id, threshold, transfer, n_left);
 }
 
 // one rotation in fp32 with every product and sum rounded on its own, as the unfused torch expression

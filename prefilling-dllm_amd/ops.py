@@ -20,7 +20,13 @@ from ._lib import AttnDesc, check, lib
 PAGE_SIZE = 256  # reference default, config.py:39
 
 
+# (the raw handle without the Stream object around it: 0.1 instead of 1.9 us of a call's 10 to 20)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -1161,12 +1167,19 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     if x.dtype == torch.bfloat16:
         if x_scale is not None:
             raise ValueError("x_scale belongs to an e4m3 x")
-        x, x_scale = quantize_fp8_rows(x)
-    elif x.dtype == torch.float8_e4m3fn:
-        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (m, kb):
-            raise ValueError(f"an e4m3 x needs fp32 scales [{m}, {kb}]")
-    else:
+        need = int(lib.pdllm_fp8_linear_bf16_workspace_bytes(m, k))
+        if need < 0:
+            check(need, "fp8_block_linear")
+        with _on(dev):
+            ws = _scratch(dev, need)
+            check(lib.pdllm_fp8_linear_bf16(_ptr(x), _row_stride(x), weight.data_ptr(), _row_stride(weight),
+                                            weight_scale.data_ptr(), weight_scale.stride(0), weight_scale.stride(1), m, n, k,
+                                            _ptr(ws), need, _ptr(out), _row_stride(out), _stream(x)), "fp8_block_linear")
+        return out
+    if x.dtype != torch.float8_e4m3fn:
         raise ValueError("x must be bfloat16 or float8_e4m3fn")
+    if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (m, kb):
+        raise ValueError(f"an e4m3 x needs fp32 scales [{m}, {kb}]")
     with _on(dev):
         check(lib.pdllm_fp8_linear(_ptr(x), _row_stride(x), _ptr(x_scale), x_scale.stride(0), x_scale.stride(1),
                                    weight.data_ptr(), _row_stride(weight), weight_scale.data_ptr(), weight_scale.stride(0),

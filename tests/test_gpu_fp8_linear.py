@@ -51,7 +51,10 @@ def operands(dev, m, n, k, seed=0):
 # every tile (32, 64, 128, 256 rows), one row to several tiles, blocks and vectors that end early, one feature
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 4096, 4096), (3, 127, 128), (32, 129, 272), (33, 300, 144), (64, 1000, 1168),
                                    (65, 2201, 400), (128, 256, 2048), (129, 513, 1024), (333, 2201, 1168), (600, 130, 5120),
-                                   (17, 40, 18944), (2, 20001, 64)])
+                                   (17, 40, 18944), (2, 20001, 64),
+                                   # up to 32 rows: kept in shared memory beside many features, or streamed with them
+                                   (5, 16400, 1040), (17, 20001, 1168), (32, 16385, 2064), (4, 16384, 1024), (9, 16384, 896),
+                                   (20, 8200, 272)])
 def test_linear(dev, m, n, k):
     from prefilling_dllm_amd import ops
     x, wq, ws = operands(dev, m, n, k, seed=m + n + k)

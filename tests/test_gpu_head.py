@@ -72,7 +72,9 @@ def check_grad(gh, gw, h, w, d):
 
 # every tile of the kernels (32, 64, 128, 256 rows), one row to several tiles, ragged in every direction, one entry
 SHAPES = [(1, 1, 8), (1, 300, 64), (5, 1000, 520), (31, 127, 72), (32, 129, 64), (33, 2570, 136), (64, 3000, 256),
-          (65, 257, 8), (128, 1025, 1032), (129, 3001, 512), (300, 2571, 136), (1030, 700, 200), (2, 40000, 64)]
+          (65, 257, 8), (128, 1025, 1032), (129, 3001, 512), (300, 2571, 136), (1030, 700, 200), (2, 40000, 64),
+          # one piece of few entries (no sum of partial results), just more than that, the last row of the small tiles
+          (20, 1024, 520), (20, 1030, 520), (256, 2000, 264), (257, 2001, 264), (200, 20000, 72)]
 
 
 @pytest.mark.parametrize("n,v,d", SHAPES)
@@ -219,7 +221,9 @@ def plain_shift(h, block, last):
 
 @pytest.mark.parametrize("n_seqs,block,v,d,shift,with_last",
                          [(1, 1, 50, 8, True, True), (1, 32, 5000, 512, True, True), (3, 33, 4001, 264, True, False),
-                          (2, 32, 1000, 64, False, False), (5, 64, 2000, 136, True, True), (1, 7, 1, 64, True, True)])
+                          (2, 32, 1000, 64, False, False), (5, 64, 2000, 136, True, True), (1, 7, 1, 64, True, True),
+                          (1, 3, 40000, 64, True, True), (32, 5, 300, 64, True, False), (40, 33, 1500, 64, True, True),
+                          (33, 1, 40001, 72, False, False)])
 def test_denoise_step(dev, n_seqs, block, v, d, shift, with_last):
     from prefilling_dllm_amd import ops
     n = n_seqs * block

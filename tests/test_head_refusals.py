@@ -36,9 +36,9 @@ def test_head_sizes_and_pointers(lib, p):
         assert call(**kw) == st, kw
     assert lib.pdllm_head_workspace_bytes(-1, 10) == -2 and lib.pdllm_head_workspace_bytes(1, 0) == -2
     assert lib.pdllm_head_workspace_bytes(0, 10) == 0
-    # enough for every tile size: the parts of a row, the label's logit or the position
+    # a row's parts: 8 bytes and a position each, of 128 entries up to 64 rows and of 256 above
     for n in (1, 32, 33, 64, 65, 128, 129, 5000):
-        assert lib.pdllm_head_workspace_bytes(n, 152064) >= n * (152064 // 128) * 12
+        assert lib.pdllm_head_workspace_bytes(n, 152064) >= n * (152064 // (128 if n <= 64 else 256)) * 12
 
 
 def test_gradient_sizes_and_pointers(lib, p):
@@ -93,6 +93,24 @@ def test_fp8_sizes_and_pointers(lib, p):
                    (dict(xs=48), -3), (dict(ws=72), -3), (dict(x=p + 8), -3), (dict(w=p + 4), -3), (dict(os=7), -3),
                    (dict(out=p + 1), -3), (dict(sxr=-1), -3), (dict(swb=-1), -3), (dict(ws=1 << 23), -3)):
         assert call(**kw) == st, kw
+    g = lib.pdllm_fp8_linear_bf16
+    need = lib.pdllm_fp8_linear_bf16_workspace_bytes(40, 64)
+    assert need == 40 * 64 + 4 * 40 and lib.pdllm_fp8_linear_bf16_workspace_bytes(32, 64) == 0
+    for bad in ((-1, 64), (4, 0), (4, 40), (4, (1 << 20) + 16), ((1 << 24) + 1, 64)):
+        assert lib.pdllm_fp8_linear_bf16_workspace_bytes(*bad) == -2
+    ok.update(m=40, ws_p=p, ws_n=need)
+
+    def call16(**kw):
+        a = {**ok, **kw}
+        return g(a["x"], a["xs"], a["w"], a["ws"], a["sw"], a["swr"], a["swb"], a["m"], a["n"], a["k"], a["ws_p"], a["ws_n"],
+                 a["out"], a["os"], None)
+
+    assert call16(m=0) == 0
+    for kw, st in ((dict(x=None), -1), (dict(w=None), -1), (dict(sw=None), -1), (dict(out=None), -1), (dict(m=-1), -2),
+                   (dict(n=0), -2), (dict(k=40), -2), (dict(xs=48), -3), (dict(xs=68), -3), (dict(x=p + 8), -3), (dict(ws=72), -3),
+                   (dict(os=7), -3), (dict(swr=-1), -3), (dict(xs=1 << 22), -3), (dict(ws_p=None), -5), (dict(ws_p=p + 4), -5),
+                   (dict(ws_n=need - 1), -5)):
+        assert call16(**kw) == st, kw
     for q in (lib.pdllm_fp8_quantize_rows, lib.pdllm_fp8_quantize_blocks):
         assert q(p, 64, 0, 64, p, 64, p, 1, 1, None) == 0
         assert q(None, 64, 2, 64, p, 64, p, 1, 1, None) == -1 and q(p, 64, 2, 64, None, 64, p, 1, 1, None) == -1
