@@ -131,6 +131,21 @@ struct Fp8Params {
   int m_tiles, n_tiles;  // tiles of output features, of rows
 };
 
+// A wave's operand fragments, blocks of 32 rows: step ks holds, in lane half h, the 16 bytes of k at 32 ks + 16 h of its row; two
+// steps make one operand of the 32x32x64 instruction (k is permuted alike in both operands, which a sum over k does not see).
+struct Frag8 {
+  unsigned a[4];
+  __device__ __forceinline__ void init(unsigned lds_base, int first, int lane) {
+    const int l32 = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) a[ks] = lds_base + (first + l32) * KB + (((2 * ks + h) ^ kc_xor(l32)) << 4);
+  }
+  template <int KS, int J>
+  __device__ __forceinline__ void read(bf16x8& d, unsigned stage) const {
+    lds_read_b128<J * 32 * KB>(d, a[KS] + stage);
+  }
+};
+
 template <class T>
 __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
   const int lane = threadIdx.x & 63, l32 = lane & 31;
@@ -167,8 +182,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
     sx_off[j] = (unsigned)(r0 + row < p.M ? row : (int)(p.M - 1 - r0)) * (unsigned)p.sx_row;
   }
 
-  Frag<T::MT, false, T::TM, T::KB> fa;
-  Frag<T::NT, false, T::TN, T::KB> fb_;
+  Frag8 fa, fb_;
   fa.init(lds_base, wm * T::MT * 32, lane);
   fb_.init(lds_base + T::A_BYTES, wn * T::NT * 32, lane);
   f32x16 acc[T::MT][T::NT];
@@ -306,8 +320,15 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
 
   store_tile<T>(
       lds,
-      [&](int i, int j, int q) __attribute__((always_inline)) {
-        return make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+      [&](auto&& put) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < T::NT; ++j)
+#pragma unroll
+          for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              put((wn * T::NT + j) * 32 + l32, (wm * T::MT + i) * 32 + 8 * q + 4 * (lane >> 5),
+                  make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])));
       },
       p.out + r0 * p.o_stride + f0, p.o_stride, p.M - r0, p.N - f0);
 }

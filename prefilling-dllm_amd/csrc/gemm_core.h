@@ -2,23 +2,19 @@
 // C[m][n] = sum_k A[m][k] B[n][k] on the matrix cores, fp32 accumulation.
 //
 // Orientation.  A is the operand whose index is contiguous in the output (vocabulary entries, output features, state
-// columns), B the one over rows (tokens): in the 32x32 result layout a lane then owns ONE row of the output (lane & 31)
-// and 16 of its columns in registers, so softmax statistics of a row are sums over a lane's own registers and
-// stores are groups of four neighbouring columns.
+// columns), B the one over rows (tokens): in the result layouts of the matrix instructions a lane then owns ONE row of the output
+// and groups of four neighbouring columns, so softmax statistics of a row are sums over a lane's own registers.
 //
-// LDS.  A stage holds KB = 64 or 128 bytes of k per row of A and of B.  Operands that lie with k contiguous ("KC") are kept as
-// rows of KB bytes, 16-byte chunk c of row r at position c ^ x(r) with x(r) = (r >> 1) & 7 (KB = 128) or (r >> 2) & 3 (KB = 64):
-// 16 consecutive rows of one chunk cover all 64 banks.  Operands that lie with k as their row index ("KS", bf16 only) are kept
-// as KB / 2 rows of TM * 2 bytes, chunk c of row r at c ^ ((r & 3) << 2), and read through the transposing 64-bit reads
-// (four rows of four neighbouring chunks per half wave, again all banks).  Copies go straight from memory to LDS, up to ST
-// stages ahead; operand reads are hand-issued with counted waits so that they do not wait for the copies.
-//
-// KB = 128 reads whole cache lines of a row at a time and is what the tiles of few rows use, which wait for memory; KB = 64
-// gives the large tiles four stages in 128 KB, so that the copies can be issued two at a time between groups of matrix
-// instructions instead of eight in a row, which kept the matrix unit waiting behind the address unit.
+// LDS.  A stage holds KB = 128 bytes of k (a cache line) per row of A and of B.  Operands that lie with k contiguous ("KC") are
+// kept as rows of 128 bytes, 16-byte chunk c of row r at position c ^ ((r >> 1) & 7): 16 consecutive rows of one chunk cover all 64
+// banks.  Operands that lie with k as their row index ("KS", bf16 only) are kept as 64 rows of TM * 2 bytes, chunk c of row
+// r at c ^ ks_xor(r), and read through the transposing 64-bit reads (half a wave takes four rows and the four 8 rows further on,
+// two neighbouring chunks of each: again all banks).  Copies go straight from memory to LDS, up to ST stages ahead; operand
+// reads are hand-issued with counted waits so that they do not wait for the copies.
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "attn_common.h"
 
@@ -37,10 +33,9 @@ __device__ __forceinline__ void wg_barrier() {
 }
 
 // position of a row's chunks in LDS (see above)
-template <int KB>
-__device__ __forceinline__ constexpr unsigned chunk_xor(unsigned row) {
-  return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
-}
+constexpr int KB = 128;  // bytes of k in a stage
+__device__ __forceinline__ constexpr unsigned kc_xor(unsigned row) { return (row >> 1) & 7; }
+__device__ __forceinline__ constexpr unsigned ks_xor(unsigned row) { return (row & 3) << 2 | ((row >> 2) & 2); }
 
 typedef __attribute__((address_space(3))) void lds_void;
 __device__ __forceinline__ lds_void* lds_at(unsigned a) { return (lds_void*)(size_t)a; }
@@ -56,9 +51,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, un
 }
 
 // Rows of k-contiguous data, through a buffer whose size ends with the last valid row: rows and k behind the end read
-// as zero.  L copies of 1024 / KB rows per wave and stage; a lane's offset inside them takes one of two values (KB = 128: the
-// chunk positions of even and odd groups of 8 rows), the group goes through the buffer's base.
-template <int L, int KB = 128>
+// as zero.  L copies of 8 rows per wave and stage; a lane's offset inside them takes one of two values (the chunk positions of even
+// and odd groups of 8 rows), the group goes through the buffer's base.
+template <int L>
 struct LoadKC {
   static constexpr int R = 1024 / KB, LANES = KB / 16;  // rows of a copy, lanes of a row
   const char* base;  // first row of the wave
@@ -73,7 +68,7 @@ struct LoadKC {
     kbytes = kb;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const unsigned c = (lane % LANES) ^ chunk_xor<KB>(R * (wave * L + q) + lane / LANES);
+      const unsigned c = (lane % LANES) ^ kc_xor(R * (wave * L + q) + lane / LANES);
       kc[q] = 16 * c;
       off[q] = (lane / LANES) * row_bytes + 16 * c;
     }
@@ -87,7 +82,7 @@ struct LoadKC {
     for (int i = 0; i < L; ++i) {
       const int left = bytes - (int)(R * i * stride);
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (long)(R * i) * stride, left > 0 ? left : 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, o[KB == 128 ? i & 1 : 0], 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, o[i & 1], 0, 0, 0);
     }
   }
 };
@@ -95,7 +90,7 @@ struct LoadKC {
 // Rows of k-contiguous data at a 64-bit address per row (rows gathered from two tensors).  Rows past the end repeat a
 // valid row (their results are dropped); k behind the end repeats the row's first bytes (the other operand is zero
 // there).
-template <int L, int KB = 128>
+template <int L>
 struct LoadRows {
   static constexpr int R = 1024 / KB, LANES = KB / 16;
   const char* p[L];
@@ -106,7 +101,7 @@ struct LoadRows {
 #pragma unroll
     for (int i = 0; i < L; ++i) p[i] = row_ptr((unsigned)(R * (wave * L + i) + lane / LANES));
 #pragma unroll
-    for (int q = 0; q < 2; ++q) kc[q] = 16 * ((lane % LANES) ^ chunk_xor<KB>(R * (wave * L + q) + lane / LANES));
+    for (int q = 0; q < 2; ++q) kc[q] = 16 * ((lane % LANES) ^ kc_xor(R * (wave * L + q) + lane / LANES));
   }
   __device__ __forceinline__ void issue(int t, unsigned dst) const {
     const unsigned k = (unsigned)KB * t;
@@ -115,14 +110,14 @@ struct LoadRows {
     for (int q = 0; q < 2; ++q) o[q] = k + kc[q] < kbytes ? k + kc[q] : 0u;
 #pragma unroll
     for (int i = 0; i < L; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[i] + o[KB == 128 ? i & 1 : 0]),
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[i] + o[i & 1]),
                                        lds_at(dst + 1024 * i), 16, 0, 0);
   }
 };
 
 // KB / 2 rows of k per stage, W columns (bf16) of each: base = first row, first column.  Rows from k_rows on read as zero;
 // so do columns from col_bytes on.
-template <int L, int W, int KB = 128>
+template <int L, int W>
 struct LoadKS {
   static constexpr int ROWS = KB / 2, CH = W / 8;  // rows of a stage, chunks of a row
   const char* base;
@@ -137,7 +132,7 @@ struct LoadKS {
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       const unsigned q = 64 * (wave * L + i) + lane;
-      const unsigned row = q / CH, c = (q % CH) ^ ((row & 3) << 2);
+      const unsigned row = q / CH, c = (q % CH) ^ ks_xor(row);
       off[i] = 16 * c < col_bytes ? row * (unsigned)stride_bytes + 16 * c : kOutOfRange;
     }
   }
@@ -152,9 +147,9 @@ struct LoadKS {
   }
 };
 
-template <int MT_, int NT_, int WM_, int WN_, int ST_, int KB_ = 128>
+template <int MT_, int NT_, int WM_, int WN_, int ST_>
 struct Tile {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, ST = ST_, KB = KB_;
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, ST = ST_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN;
   static constexpr int A_BYTES = TM * KB, B_BYTES = TN * KB, STAGE = A_BYTES + B_BYTES;
@@ -164,48 +159,55 @@ struct Tile {
   static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
 };
 
-// A wave's operand fragments: N_ blocks of 32 rows (KC) or columns (KS), the first one at `first` of the tile.  A fragment of
-// step ks holds, in lane half h, the k values 16 ks + 8 h .. + 7 (bf16) of its row; for fp8 two fragments make one operand
-// (the k values of both operands are permuted alike, which a sum over k does not see).
-template <int N_, bool KS, int W, int KB>
+template <class F, int... I>
+__device__ __forceinline__ void unroll_over(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+// f(0), f(1), ... f(N - 1), each with its number as a constant
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  unroll_over(f, std::make_integer_sequence<int, N>{});
+}
+
+// A wave's bf16 operand fragments for the 16x16x32 instruction: blocks of 16 rows (KC) or columns (KS), the first one at `first` of
+// the tile.  A fragment of step ks holds, in lanes 16 g .. 16 g + 15, the k values 32 ks + 8 g .. + 7 of its 16 rows.
+template <bool KS, int W>
 struct Frag;
-template <int N_, int W, int KB>
-struct Frag<N_, false, W, KB> {
-  unsigned a[KB / 32];
+template <int W>
+struct Frag<false, W> {
+  unsigned a[2];
   typedef bf16x8 raw;
   static constexpr int READS = 1;  // LDS operations per fragment
   __device__ __forceinline__ void init(unsigned lds_base, int first, int lane) {
-    const int l32 = lane & 31, h = lane >> 5;
+    const int l16 = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int ks = 0; ks < KB / 32; ++ks) a[ks] = lds_base + (first + l32) * KB + (((2 * ks + h) ^ chunk_xor<KB>(l32)) << 4);
+    for (int ks = 0; ks < 2; ++ks) a[ks] = lds_base + (first + l16) * KB + (((4 * ks + g) ^ kc_xor(l16)) << 4);
   }
   template <int KS_, int J>
   __device__ __forceinline__ void read(raw& d, unsigned stage) const {
-    lds_read_b128<J * 32 * KB>(d, a[KS_] + stage);
+    lds_read_b128<J * 16 * KB>(d, a[KS_] + stage);
   }
   static __device__ __forceinline__ bf16x8 value(const raw& r) { return r; }
 };
 struct TrPair {
   s16x4 lo, hi;
 };
-template <int N_, int W, int KB>
-struct Frag<N_, true, W, KB> {
-  unsigned a[N_];
+template <int W>
+struct Frag<true, W> {
+  static_assert(W >= 128, "the chunks of a row change places in groups of 16");
+  unsigned a;
   typedef TrPair raw;
   static constexpr int READS = 2;
   __device__ __forceinline__ void init(unsigned lds_base, int first, int lane) {
-    const int l32 = lane & 31, h = lane >> 5, i16 = lane & 15, g = l32 >> 4;
-    const int row = 8 * h + (i16 >> 2);
-#pragma unroll
-    for (int j = 0; j < N_; ++j) {
-      const int c = (first + 32 * j) / 8 + 2 * g + ((i16 & 3) >> 1);
-      a[j] = lds_base + row * (W * 2) + ((c ^ ((row & 3) << 2)) << 4) + ((i16 & 1) << 3);
-    }
+    const int l16 = lane & 15, g = lane >> 4;
+    const int row = 8 * g + (l16 >> 2);
+    a = lds_base + row * (W * 2) + ((((unsigned)first / 8 + ((l16 & 3) >> 1)) ^ ks_xor(row)) << 4) + ((l16 & 1) << 3);
   }
+  // (`first` is a multiple of the wave's columns, a power of two: block J is two chunks further, by an exclusive or)
   template <int KS_, int J>
   __device__ __forceinline__ void read(raw& d, unsigned stage) const {
-    lds_read_tr16_b64<(16 * KS_) * W * 2>(d.lo, a[J] + stage);
-    lds_read_tr16_b64<(16 * KS_ + 4) * W * 2>(d.hi, a[J] + stage);
+    lds_read_tr16_b64<32 * KS_ * W * 2>(d.lo, (a ^ (32 * J)) + stage);
+    lds_read_tr16_b64<(32 * KS_ + 4) * W * 2>(d.hi, (a ^ (32 * J)) + stage);
   }
   static __device__ __forceinline__ bf16x8 value(const raw& r) {
     typedef __attribute__((ext_vector_type(8))) short s16x8;
@@ -217,50 +219,67 @@ struct Frag<N_, true, W, KB> {
 __device__ __forceinline__ void tie(bf16x8& r) { asm volatile("" : "+v"(r)::"memory"); }
 __device__ __forceinline__ void tie(TrPair& r) { asm volatile("" : "+v"(r.lo), "+v"(r.hi)::"memory"); }
 
+// A wave's bf16 accumulators: blocks of 16 x 16, lane 16 g + l holds entries 4 g .. 4 g + 3 of A's block and row l of B's.
+template <class T>
+struct Acc {
+  f32x4 v[2 * T::MT][2 * T::NT];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 2 * T::MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2 * T::NT; ++j) v[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+};
+
 // The bf16 loop over `steps` stages.  issue(t, lds address of the stage, part) starts half of the copies of stage t (part 0
-// or 1; T::LA + T::LB per wave in all).  One barrier per stage, in front of the stage's last group of matrix instructions: by
-// then every wave has read all of the stage and its own part of the next one has landed, so behind the barrier the
-// stage's buffer takes the copies of stage t + ST, half of them at once and half behind the next group, and the first
-// fragments of the next stage are read while the last group runs.
+// or 1; T::LA + T::LB per wave in all).  A stage is two steps of k = 32 in four turns, half of the wave's blocks of A each; the
+// fragments of the next turn are read while a turn's matrix instructions run.  One barrier per stage, in front of the last
+// turn: by then every wave has read all of the stage and its own part of the next one has landed, so behind the barrier the
+// stage's buffer takes the copies of stage t + ST, half of them at once and half in the next turn.
+// The 16x16x32 instruction, not 32x32x16: the large products here run at the card's power limit, and with operands of normally
+// distributed values out of registers the one sustains 2050 TFLOP/s, the other 1340 to 1640 (zeros: 2450 and 1810 to 2210).
 template <class T, bool AKS, bool BKS, class Issue>
-__device__ __forceinline__ void mainloop_bf16(f32x16 (&acc)[T::MT][T::NT], int steps, unsigned lds_base, Issue&& issue) {
+__device__ __forceinline__ void mainloop_bf16(Acc<T>& acc, int steps, unsigned lds_base, Issue&& issue) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
-  constexpr int COPIES = T::LA + T::LB, GROUPS = T::KB / 32;
-  typedef Frag<T::MT, AKS, T::TM, T::KB> FA;
-  typedef Frag<T::NT, BKS, T::TN, T::KB> FB;
+  constexpr int COPIES = T::LA + T::LB, MT = T::MT, NT = T::NT;
+  typedef Frag<AKS, T::TM> FA;
+  typedef Frag<BKS, T::TN> FB;
   FA fa;
   FB fb;
-  fa.init(lds_base, wm * T::MT * 32, lane);
-  fb.init(lds_base + T::A_BYTES, wn * T::NT * 32, lane);
-  typename FA::raw A[2][T::MT];
-  typename FB::raw B[2][T::NT];
-  constexpr int READS = T::MT * FA::READS + T::NT * FB::READS;
-  static_assert(READS <= 15, "the wait counts 15 LDS operations at most");
-  static_assert(GROUPS == 2 || GROUPS == 4, "fragments alternate between two sets");
+  fa.init(lds_base, wm * MT * 32, lane);
+  fb.init(lds_base + T::A_BYTES, wn * NT * 32, lane);
+  typename FA::raw A[2][MT];      // of this turn and the next
+  typename FB::raw B[2][2 * NT];  // of both steps
+  constexpr int RA = MT * FA::READS, RB = NT * FB::READS;
+  static_assert(RA + RB <= 15, "the wait counts 15 LDS operations at most");
   if (steps <= 0) return;
   unsigned cur = 0, old = 0;
-  auto read = [&](auto ks_tag, int set) __attribute__((always_inline)) {
-    constexpr int KS = decltype(ks_tag)::value;
-    fb.template read<KS, 0>(B[set][0], cur);
-    if constexpr (T::NT > 1) fb.template read<KS, 1>(B[set][1], cur);
-    fa.template read<KS, 0>(A[set][0], cur);
-    if constexpr (T::MT > 1) fa.template read<KS, 1>(A[set][1], cur);
-    if constexpr (T::MT > 2) fa.template read<KS, 2>(A[set][2], cur);
-    if constexpr (T::MT > 3) fa.template read<KS, 3>(A[set][3], cur);
+  auto read_a = [&](auto turn) __attribute__((always_inline)) {
+    constexpr int U = decltype(turn)::value;
+    unrolled<MT>([&](auto i) __attribute__((always_inline)) { fa.template read<U / 2, (U & 1) * MT + decltype(i)::value>(A[U & 1][decltype(i)::value], cur); });
   };
-  auto mul = [&](int set) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < T::MT; ++i) tie(A[set][i]);
-#pragma unroll
-    for (int j = 0; j < T::NT; ++j) tie(B[set][j]);
-#pragma unroll
-    for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-      for (int j = 0; j < T::NT; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FA::value(A[set][i]), FB::value(B[set][j]), acc[i][j], 0, 0, 0);
+  auto read_b = [&](auto ks, auto half) __attribute__((always_inline)) {
+    constexpr int S = decltype(ks)::value, H = decltype(half)::value;
+    unrolled<NT>([&](auto j) __attribute__((always_inline)) { fb.template read<S, H * NT + decltype(j)::value>(B[S][H * NT + decltype(j)::value], cur); });
   };
+  auto mul = [&](auto turn) __attribute__((always_inline)) {
+    constexpr int U = decltype(turn)::value, S = U / 2, H = U & 1;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) tie(A[H][i]);
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j) tie(B[S][j]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2 * NT; ++j)
+        acc.v[H * MT + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(FA::value(A[H][i]), FB::value(B[S][j]), acc.v[H * MT + i][j], 0, 0, 0);
+  };
+  constexpr std::integral_constant<int, 0> c0{};
+  constexpr std::integral_constant<int, 1> c1{};
+  constexpr std::integral_constant<int, 2> c2{};
+  constexpr std::integral_constant<int, 3> c3{};
 #pragma unroll
   for (int s = 0; s < T::ST; ++s)
     if (s < steps) {
@@ -270,61 +289,52 @@ __device__ __forceinline__ void mainloop_bf16(f32x16 (&acc)[T::MT][T::NT], int s
   if (steps >= T::ST) vm_wait<(T::ST - 1) * COPIES>();
   else vm_wait<0>();
   wg_barrier();
-  read(std::integral_constant<int, 0>{}, 0);
-  // all groups of a stage but the last; behind the first one the second half of the copies that the barrier before allowed
-  auto groups = [&](int t) __attribute__((always_inline)) {
-    read(std::integral_constant<int, 1>{}, 1);
-    lgkm_wait<READS>();
+  read_b(c0, c0);
+  read_b(c0, c1);
+  read_a(c0);
+  // all turns of a stage but the last; in the first one the second half of the copies that the barrier before allowed
+  auto turns = [&](int t) __attribute__((always_inline)) {
+    read_a(c1);
+    read_b(c1, c0);
+    lgkm_wait<RA + RB>();
     if (t > 0 && t + T::ST - 1 < steps) issue(t + T::ST - 1, lds_base + old, 1);
-    mul(0);
-    if constexpr (GROUPS == 4) {
-      read(std::integral_constant<int, 2>{}, 0);
-      lgkm_wait<READS>();
-      mul(1);
-      read(std::integral_constant<int, 3>{}, 1);
-      lgkm_wait<READS>();
-      mul(0);
-    }
+    mul(c0);
+    read_a(c2);
+    read_b(c1, c1);
+    lgkm_wait<RA + RB>();
+    mul(c1);
+    read_a(c3);
+    lgkm_wait<RA>();
+    mul(c2);
     lgkm_wait<0>();
   };
   for (int t = 0; t < steps - 1; ++t) {
-    groups(t);
+    turns(t);
     if (T::ST > 2 && t + T::ST - 1 < steps) vm_wait<(T::ST - 2) * COPIES>();
     else vm_wait<0>();
     wg_barrier();
     old = cur;
     cur = cur == (T::ST - 1) * T::STAGE ? 0u : cur + T::STAGE;
-    read(std::integral_constant<int, 0>{}, 0);
+    read_b(c0, c0);
+    read_b(c0, c1);
+    read_a(c0);
     if (t + T::ST < steps) issue(t + T::ST, lds_base + old, 0);
-    mul(1);
+    mul(c3);
   }
-  groups(steps - 1);
-  mul(1);
+  turns(steps - 1);
+  mul(c3);
 }
 
-// A tile of bf16 results to memory through LDS, so that a row's columns leave in one piece (a lane's four columns at a time,
-// straight from the registers, every store touches 32 rows).  get(i, j, q): columns 32 i + 8 q + 4 h .. + 3 of the wave's
-// block, row block j, packed.  out: row 0, column 0 of the tile; rows, cols: how much of it exists.  Chunk c of row r lies at
-// c ^ (r & 15).
-template <class T, class Get>
-__device__ __forceinline__ void store_tile(char* lds, Get&& get, __bf16* out, long stride, long rows, long cols) {
+// A bf16 tile to memory through LDS, so that rows leave in whole lines: 16 bytes a lane where the rows begin at multiples of
+// that, else words.  fill(put) hands over the wave's results: put(row, column, four values) with columns in multiples of four.
+template <class T, class Fill>
+__device__ __forceinline__ void store_tile(char* lds, Fill&& fill, __bf16* out, long stride, long rows, long cols) {
   constexpr int CH = T::TM / 8;  // chunks of a row
   static_assert(T::TM * T::TN * 2 <= T::LDS && CH >= 16, "the results take the place of the operands");
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / T::WN, wn = wave % T::WN;
   __syncthreads();  // the tile's operands are done with
-#pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
-    const int r = (wn * T::NT + j) * 32 + l32;
-#pragma unroll
-    for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = (wm * T::MT + i) * 4 + q;
-        *reinterpret_cast<uint2*>(lds + (r * CH + (c ^ (r & 15))) * 16 + 8 * h) = get(i, j, q);
-      }
-  }
+  fill([&](int r, int c, uint2 v) __attribute__((always_inline)) {
+    *reinterpret_cast<uint2*>(lds + (r * CH + ((c >> 3) ^ (r & 15))) * 16 + 2 * (c & 4)) = v;
+  });
   __syncthreads();
   const int nr = rows < T::TN ? (int)rows : T::TN, nc = cols < T::TM ? (int)cols : T::TM;
   const unsigned odd = (unsigned)(uintptr_t)out | (unsigned)(2 * stride);
@@ -367,6 +377,24 @@ __device__ __forceinline__ void store_tile(char* lds, Get&& get, __bf16* out, lo
       else if (c < 0) o[0] = (unsigned short)hi;
     }
   }
+}
+
+// The wave's accumulators, packed in pairs, by store_tile.
+template <class T, class Pack>
+__device__ __forceinline__ void store_acc(char* lds, const Acc<T>& acc, Pack&& pack, __bf16* out, long stride, long rows, long cols) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = wave % T::WN * (32 * T::NT) + (lane & 15), c0 = wave / T::WN * (32 * T::MT) + 4 * (lane >> 4);
+  store_tile<T>(
+      lds,
+      [&](auto&& put) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2 * T::NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 2 * T::MT; ++i)
+            put(r0 + 16 * j, c0 + 16 * i, make_uint2(pack(acc.v[i][j][0], acc.v[i][j][1]), pack(acc.v[i][j][2], acc.v[i][j][3])));
+      },
+      out, stride, rows, cols);
 }
 
 }  // namespace pdllm

@@ -55,15 +55,15 @@ __device__ __forceinline__ void head_tile(const HeadParams& p, int id, int& vt, 
 }
 
 template <class T>
-__device__ __forceinline__ void head_logits(const HeadParams& p, int vt, long row0, f32x16 (&acc)[T::MT][T::NT], char* lds) {
+__device__ __forceinline__ void head_logits(const HeadParams& p, int vt, long row0, Acc<T>& acc, char* lds) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned lds_base = (unsigned)(size_t)lds;
   const long v0 = p.v0 + (long)vt * T::TM;
   const unsigned kbytes = 2u * p.D;
-  LoadKC<T::LA, T::KB> la;
+  LoadKC<T::LA> la;
   la.init(p.w + v0 * p.w_stride, p.V - v0, (unsigned)p.w_stride, kbytes, wave, lane);
-  LoadRows<T::LB, T::KB> lb;
+  LoadRows<T::LB> lb;
   lb.init(
       [&](unsigned row) __attribute__((always_inline)) {
         long t = row0 + row;
@@ -76,21 +76,13 @@ __device__ __forceinline__ void head_logits(const HeadParams& p, int vt, long ro
         return p.h + t * p.h_stride;
       },
       kbytes, wave, lane);
-#pragma unroll
-  for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < T::NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  acc.clear();
   mainloop_bf16<T, false, false>(
-      acc, (int)(kbytes + T::KB - 1) / T::KB, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
+      acc, (int)(kbytes + KB - 1) / KB, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
         if (part == 0) la.issue(t, dst + wave * (T::LA * 1024));
         else lb.issue(t, dst + T::A_BYTES + wave * (T::LB * 1024));
       });
 }
-
-// register e of a 32x32 result of lane half h holds row 8 (e / 4) + 4 h + e % 4
-__device__ __forceinline__ constexpr int row_of(int e, int h) { return 8 * (e >> 2) + 4 * h + (e & 3); }
 
 struct Stat {
   float m, s;
@@ -107,81 +99,84 @@ __device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
 }
 
 // A tile of logits and its statistics per row: a lane's own values first (their maximum, then the sum of exp(x - max)), the other
-// half of the wave, the other waves of the row.
+// three lanes of the row, the other waves of the row.
 template <class T, bool CONF>
 __device__ __forceinline__ void head_stats_tile(const HeadParams& p, int vt, long row0, char* lds) {
-  f32x16 acc[T::MT][T::NT];
+  Acc<T> acc;
   head_logits<T>(p, vt, row0, acc, lds);
 
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   const long vw = (long)vt * T::TM + wm * (32 * T::MT);  // first entry of the wave
   if (vw + 32 * T::MT > p.V) {                           // entries behind the vocabulary do not exist
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int i = 0; i < 2 * T::MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (vw + 32 * i + row_of(e, h) >= p.V)
+      for (int e = 0; e < 4; ++e)
+        if (vw + 16 * i + 4 * g + e >= p.V)
 #pragma unroll
-          for (int j = 0; j < T::NT; ++j) acc[i][j][e] = -INFINITY;
+          for (int j = 0; j < 2 * T::NT; ++j) acc.v[i][j][e] = -INFINITY;
   }
   __syncthreads();  // the tile's operands are done with: their place takes the statistics
 #pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
+  for (int j = 0; j < 2 * T::NT; ++j) {
+    const int col = wn * (32 * T::NT) + 16 * j + l16;
     if constexpr (!CONF) {
-      const long row = row0 + (wn * T::NT + j) * 32 + l32;
+      const long row = row0 + col;
       const long lab = row < p.N ? p.labels[row] : -1;
       const long rel = lab - vw;
-      const bool mine = rel >= 0 && rel < 32 * T::MT && lab < p.V;
+      const bool mine = rel >= 0 && rel < 32 * T::MT && lab < p.V && ((rel >> 2) & 3) == g;
       if (__builtin_amdgcn_ballot_w64(mine) != 0) {
-        const int at = mine ? (int)rel : -1;
+        const int at = mine ? (int)rel - 4 * g : -1;
         float x = 0.f;
 #pragma unroll
-        for (int i = 0; i < T::MT; ++i)
+        for (int i = 0; i < 2 * T::MT; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (at == 32 * i + row_of(e, h)) {
-              x = acc[i][j][e];
-              acc[i][j][e] = -INFINITY;
+          for (int e = 0; e < 4; ++e)
+            if (at == 16 * i + e) {
+              x = acc.v[i][j][e];
+              acc.v[i][j][e] = -INFINITY;
             }
-        if (mine && ((at >> 2) & 1) == h) p.xlab[row] = x;
+        if (mine) p.xlab[row] = x;
       }
     }
     float m = -INFINITY;
     int idx = 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int i = 0; i < 2 * T::MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = acc[i][j][e];
+      for (int e = 0; e < 4; ++e) {
+        const float x = acc.v[i][j][e];
         if constexpr (CONF) {
-          if (x > m) idx = 32 * i + row_of(e, 0);
+          if (x > m) idx = 16 * i + e;
         }
         m = fmaxf(m, x);
       }
-    const float ref = m == -INFINITY ? 0.f : m;
+    // the other lane groups hold the other entries of the same row
+    const float m1 = fmaxf(m, __shfl_xor(m, 16, 64));
+    const float top = half_swap_max(m1);
+    const float ref = top == -INFINITY ? 0.f : top;
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int i = 0; i < 2 * T::MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - ref) * kLog2eH);
-    // the other lane half holds the other rows of the same token
-    const float m2 = half_swap_max(m);
-    const float ref2 = m2 == -INFINITY ? 0.f : m2;
-    if (m != -INFINITY) s *= __builtin_amdgcn_exp2f((m - ref2) * kLog2eH);  // (else s is 0, or NaN from NaN alone)
+      for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc.v[i][j][e] - ref) * kLog2eH);
+    s += __shfl_xor(s, 16, 64);
     s = half_swap_sum(s);
     if constexpr (CONF) {
-      // the lowest position among the halves that hold the maximum
-      if (idx != 0x7fffffff) idx += 4 * h;
-      int cand = m == m2 ? idx : 0x7fffffff;
-      const int other = __shfl_xor(cand, 32, 64);
-      cand = other < cand ? other : cand;
+      // the lowest position among the lanes that hold the maximum
+      int cand = m == top && idx != 0x7fffffff ? idx + 4 * g : 0x7fffffff;
+#pragma unroll
+      for (int o = 16; o < 64; o <<= 1) {
+        const int other = __shfl_xor(cand, o, 64);
+        cand = other < cand ? other : cand;
+      }
       idx = cand == 0x7fffffff ? cand : cand + (int)vw;
     }
-    if (h == 0) {
-      Stat* sh = reinterpret_cast<Stat*>(lds) + wm * T::TN + (wn * T::NT + j) * 32 + l32;
-      *sh = {m2, s, idx};
+    if (g == 0) {
+      Stat* sh = reinterpret_cast<Stat*>(lds) + wm * T::TN + col;
+      *sh = {top, s, idx};
     }
   }
   __syncthreads();
@@ -323,62 +318,57 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2* __restrict
 // second plane carries the remainder of the rounding.
 template <class T>
 __device__ __forceinline__ void head_dlogits_tile(const HeadParams& p, int vt, long row0, char* lds) {
-  f32x16 acc[T::MT][T::NT];
+  Acc<T> acc;
   head_logits<T>(p, vt, row0, acc, lds);
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = 4 * (lane >> 4);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const long vl = (long)vt * T::TM + wm * (32 * T::MT);                             // first entry of the wave, in the piece
+  const int v_wave = wm * (32 * T::MT), r_wave = wn * (32 * T::NT);
+  const long vl = (long)vt * T::TM + v_wave;                                        // first entry of the wave, in the piece
   const long left = p.V - p.v0 - vl;                                               // entries of the vocabulary from there on
   const int end = left < 0 ? 0 : left < 32 * T::MT ? (int)left : 32 * T::MT;
 #pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
-    const long row = row0 + (wn * T::NT + j) * 32 + l32;
+  for (int j = 0; j < 2 * T::NT; ++j) {
+    const long row = row0 + r_wave + 16 * j + l16;
     const long lab = row < p.N ? p.labels[row] : -1;
     const bool in = lab >= 0 && lab < p.V;
     const float lse = in ? p.lse[row] : 0.f, g = in ? p.g[row] : 0.f;
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int i = 0; i < 2 * T::MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float y = -g * __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * kLog2eH);
-        acc[i][j][e] = in ? y : 0.f;  // (a row without a label may hold anything)
+      for (int e = 0; e < 4; ++e) {
+        const float y = -g * __builtin_amdgcn_exp2f((acc.v[i][j][e] - lse) * kLog2eH);
+        acc.v[i][j][e] = in ? y : 0.f;  // (a row without a label may hold anything)
       }
     const long rel = lab - p.v0 - vl;
-    const bool mine = in && rel >= 0 && rel < 32 * T::MT;
+    const bool mine = in && rel >= 0 && rel < 32 * T::MT && ((int)rel & 12) == g4;
     if (__builtin_amdgcn_ballot_w64(mine) != 0) {
-      const int at = mine ? (int)rel : -1;
+      const int at = mine ? (int)rel - g4 : -1;
       const float y = mine ? -g * expm1f(p.logp[row]) : 0.f;
 #pragma unroll
-      for (int i = 0; i < T::MT; ++i)
+      for (int i = 0; i < 2 * T::MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (at == 32 * i + row_of(e, h)) acc[i][j][e] = y;
+        for (int e = 0; e < 4; ++e)
+          if (at == 16 * i + e) acc.v[i][j][e] = y;
     }
   }
   if (end < 32 * T::MT) {  // entries behind the vocabulary: zeros, which the products read
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int i = 0; i < 2 * T::MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (32 * i + row_of(e, h) >= end)
+      for (int e = 0; e < 4; ++e)
+        if (16 * i + g4 + e >= end)
 #pragma unroll
-          for (int j = 0; j < T::NT; ++j) acc[i][j][e] = 0.f;
+          for (int j = 0; j < 2 * T::NT; ++j) acc.v[i][j][e] = 0.f;
   }
-  auto hi = [&](int i, int j, int q) __attribute__((always_inline)) {
-    return make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+  // the remainder of a rounded pair: what the second plane holds
+  auto low = [](float a, float b) __attribute__((always_inline)) {
+    const unsigned w = pack_bf16x2(a, b);
+    return pack_bf16x2(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
   };
   const long o = row0 * p.ldd + (long)vt * T::TM;
-  store_tile<T>(lds, hi, p.d + o, p.ldd, p.N - row0, T::TM);
-  if (p.dlo)
-    store_tile<T>(
-        lds,
-        [&](int i, int j, int q) __attribute__((always_inline)) {
-          const uint2 w = hi(i, j, q);
-          return make_uint2(pack_bf16x2(acc[i][j][4 * q] - __uint_as_float(w.x << 16), acc[i][j][4 * q + 1] - __uint_as_float(w.x & 0xffff0000u)),
-                            pack_bf16x2(acc[i][j][4 * q + 2] - __uint_as_float(w.y << 16), acc[i][j][4 * q + 3] - __uint_as_float(w.y & 0xffff0000u)));
-        },
-        p.dlo + o, p.ldd, p.N - row0, T::TM);
+  store_acc<T>(lds, acc, [](float a, float b) __attribute__((always_inline)) { return pack_bf16x2(a, b); }, p.d + o, p.ldd, p.N - row0, T::TM);
+  if (p.dlo) store_acc<T>(lds, acc, low, p.dlo + o, p.ldd, p.N - row0, T::TM);
 }
 
 template <class T, class TS>
@@ -424,7 +414,7 @@ struct GradParams {
 // grad_h of a piece: acc[split][row][c] (+)= sum over the split's entries of d[row][v] w[v][c]
 template <class T>
 __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, char* lds) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
@@ -434,25 +424,20 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, ch
   const long k0 = split * p.k_per;
   long kn = p.vp - k0;
   kn = kn < 0 ? 0 : (kn < p.k_per ? kn : p.k_per);  // (a last, shorter piece may leave a split without entries)
-  constexpr int SK = T::KB / 2;  // entries per stage
+  constexpr int SK = KB / 2;  // entries per stage
   const int steps = (int)((kn + SK - 1) / SK);
   const int c0 = mt * T::TM;
   const long r0 = (long)nt * T::TN;
   const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
-  LoadKS<T::LA, T::TM, T::KB> la;
+  LoadKS<T::LA, T::TM> la;
   la.init(p.w + k0 * p.w_stride + 2 * c0, p.w_stride, kn, cols, wave, lane);
-  LoadKC<T::LB, T::KB> lb;
-  const unsigned kb = (unsigned)T::KB * steps;  // d is padded with zeros to whole stages
+  LoadKC<T::LB> lb;
+  const unsigned kb = (unsigned)KB * steps;  // d is padded with zeros to whole stages
   const char* d0 = p.d + r0 * p.ldd + 2 * k0;
   lb.init(d0, p.N - r0, (unsigned)p.ldd, kb, wave, lane);
   d0 = lb.base;
-  f32x16 acc[T::MT][T::NT];
-#pragma unroll
-  for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < T::NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  Acc<T> acc;
+  acc.clear();
   mainloop_bf16<T, true, false>(
       acc, steps * p.planes, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
         const int t1 = t < steps ? t : t - steps;
@@ -464,26 +449,22 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, ch
         }
       });
 #pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
-    const long row = r0 + (wn * T::NT + j) * 32 + l32;
+  for (int j = 0; j < 2 * T::NT; ++j) {
+    const long row = r0 + wn * (32 * T::NT) + 16 * j + l16;
     if (row >= p.N) continue;
     float* out = p.acc + ((long)split * p.N + row) * p.D;
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = c0 + wm * (32 * T::MT) + 32 * i + row_of(4 * q, h);
-        if (c >= p.D) continue;
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
-        if (p.gh) {
-          *reinterpret_cast<uint2*>(p.gh + row * p.gh_stride + c) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-          continue;
-        }
-        if (p.add) v += *reinterpret_cast<const f32x4*>(out + c);
-        *reinterpret_cast<f32x4*>(out + c) = v;
+    for (int i = 0; i < 2 * T::MT; ++i) {
+      const int c = c0 + wm * (32 * T::MT) + 16 * i + 4 * g;
+      if (c >= p.D) continue;
+      f32x4 v = acc.v[i][j];
+      if (p.gh) {
+        *reinterpret_cast<uint2*>(p.gh + row * p.gh_stride + c) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        continue;
       }
+      if (p.add) v += *reinterpret_cast<const f32x4*>(out + c);
+      *reinterpret_cast<f32x4*>(out + c) = v;
+    }
   }
 }
 
@@ -514,22 +495,17 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
   const int mt = __builtin_amdgcn_readfirstlane(id % p.w_tiles);
   const int nt = __builtin_amdgcn_readfirstlane(id / p.w_tiles);
   const unsigned lds_base = (unsigned)(size_t)lds;
-  constexpr int SK = T::KB / 2;  // rows per stage
+  constexpr int SK = KB / 2;  // rows per stage
   const int steps = (int)((p.N + SK - 1) / SK);
   const int c0 = mt * T::TM;
   const long v0 = (long)nt * T::TN;
   const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
-  LoadKS<T::LA, T::TM, T::KB> la;
+  LoadKS<T::LA, T::TM> la;
   la.init(p.hz + 2 * c0, 2L * p.D, p.N, cols, wave, lane);
-  LoadKS<T::LB, T::TN, T::KB> lb;
+  LoadKS<T::LB, T::TN> lb;
   lb.init(p.d + 2 * v0, p.ldd, p.N, 2u * T::TN, wave, lane);  // the rows of d are whole tiles long
-  f32x16 acc[T::MT][T::NT];
-#pragma unroll
-  for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < T::NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  Acc<T> acc;
+  acc.clear();
   const char* d0 = lb.base;
   mainloop_bf16<T, true, true>(
       acc, steps * p.planes, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
@@ -541,12 +517,8 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
           lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
         }
       });
-  store_tile<T>(
-      lds,
-      [&](int i, int j, int q) __attribute__((always_inline)) {
-        return make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
-      },
-      p.gw + v0 * p.gw_stride + c0, p.gw_stride, p.vp - v0, p.D - c0);
+  store_acc<T>(lds, acc, [](float a, float b) __attribute__((always_inline)) { return pack_bf16x2(a, b); }, p.gw + v0 * p.gw_stride + c0,
+               p.gw_stride, p.vp - v0, p.D - c0);
 }
 
 // Both products of a piece in one launch: the tiles of grad_h first (few, with the whole piece to sum over), those of grad_w
@@ -637,7 +609,7 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
   int st;
   if (p.N <= 32) st = launch_stats<TileS, TileS, CONF>(p, s);
   else if (p.N <= 64) st = launch_stats<TileS2, TileS2, CONF>(p, s);
-  else if (p.N <= 128 && p.V >= 32768) st = launch_stats<TileM, TileM, CONF>(p, s);
+  else if (p.N <= 128 && p.V >= 32768) st = launch_stats<TileM, TileR, CONF>(p, s);
   else st = launch_stats<TileL, TileR, CONF>(p, s);
   if (st != PDLLM_OK) return st;
   hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)(parts > 256 ? p.N : (p.N + 3) / 4)), dim3(256), 0, s, p.part, p.part_idx, p.xlab,
