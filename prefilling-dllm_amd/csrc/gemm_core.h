@@ -73,6 +73,14 @@ struct LoadKC {
       off[q] = (lane / LANES) * row_bytes + 16 * c;
     }
   }
+  template <int I>
+  __device__ __forceinline__ void one(int t, unsigned dst) const {
+    const unsigned k = (unsigned)KB * t;
+    const unsigned o = k + kc[I & 1] < kbytes ? off[I & 1] + k : kOutOfRange;
+    const int left = bytes - (int)(R * I * stride);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (long)(R * I) * stride, left > 0 ? left : 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * I), 16, o, 0, 0, 0);
+  }
   __device__ __forceinline__ void issue(int t, unsigned dst) const {
     const unsigned k = (unsigned)KB * t;
     unsigned o[2];
@@ -102,6 +110,12 @@ struct LoadRows {
     for (int i = 0; i < L; ++i) p[i] = row_ptr((unsigned)(R * (wave * L + i) + lane / LANES));
 #pragma unroll
     for (int q = 0; q < 2; ++q) kc[q] = 16 * ((lane % LANES) ^ kc_xor(R * (wave * L + q) + lane / LANES));
+  }
+  template <int I>
+  __device__ __forceinline__ void one(int t, unsigned dst) const {
+    const unsigned k = (unsigned)KB * t;
+    const unsigned o = k + kc[I & 1] < kbytes ? k + kc[I & 1] : 0u;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[I] + o), lds_at(dst + 1024 * I), 16, 0, 0);
   }
   __device__ __forceinline__ void issue(int t, unsigned dst) const {
     const unsigned k = (unsigned)KB * t;
@@ -135,6 +149,14 @@ struct LoadKS {
       const unsigned row = q / CH, c = (q % CH) ^ ks_xor(row);
       off[i] = 16 * c < col_bytes ? row * (unsigned)stride_bytes + 16 * c : kOutOfRange;
     }
+  }
+  template <int I>
+  __device__ __forceinline__ void one(int t, unsigned dst) const {
+    const long r0 = (long)ROWS * t;
+    const long left = k_rows - r0;
+    const unsigned rows = left <= 0 ? 0u : (left < ROWS ? (unsigned)left : (unsigned)ROWS);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + r0 * stride, rows ? (rows - 1) * (unsigned)stride + colb : 0u);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * I), 16, off[I], 0, 0, 0);
   }
   __device__ __forceinline__ void issue(int t, unsigned dst) const {
     const long r0 = (long)ROWS * t;
@@ -255,74 +277,107 @@ __device__ __forceinline__ void mainloop_bf16(Acc<T>& acc, int steps, unsigned l
   constexpr int RA = MT * FA::READS, RB = NT * FB::READS;
   static_assert(RA + RB <= 15, "the wait counts 15 LDS operations at most");
   if (steps <= 0) return;
-  unsigned cur = 0, old = 0;
-  auto read_a = [&](auto turn) __attribute__((always_inline)) {
-    constexpr int U = decltype(turn)::value;
-    unrolled<MT>([&](auto i) __attribute__((always_inline)) { fa.template read<U / 2, (U & 1) * MT + decltype(i)::value>(A[U & 1][decltype(i)::value], cur); });
+  // fragment n of those that a turn reads for the next: blocks of A, then of B
+  auto read_a = [&](auto turn, auto n, unsigned cur) __attribute__((always_inline)) {
+    constexpr int U = decltype(turn)::value, i = decltype(n)::value;
+    fa.template read<U / 2, (U & 1) * MT + i>(A[U & 1][i], cur);
   };
-  auto read_b = [&](auto ks, auto half) __attribute__((always_inline)) {
-    constexpr int S = decltype(ks)::value, H = decltype(half)::value;
-    unrolled<NT>([&](auto j) __attribute__((always_inline)) { fb.template read<S, H * NT + decltype(j)::value>(B[S][H * NT + decltype(j)::value], cur); });
+  auto read_b = [&](auto ks, auto n, unsigned cur) __attribute__((always_inline)) {
+    constexpr int S = decltype(ks)::value, j = decltype(n)::value;
+    fb.template read<S, j>(B[S][j], cur);
   };
-  auto mul = [&](auto turn) __attribute__((always_inline)) {
+  // the matrix instructions of a turn in a fixed order, neighbours sharing an operand; behind instruction n: between(n)
+  constexpr int PRODUCTS = MT * 2 * NT;
+  auto mul = [&](auto turn, auto&& between) __attribute__((always_inline)) {
     constexpr int U = decltype(turn)::value, S = U / 2, H = U & 1;
 #pragma unroll
     for (int i = 0; i < MT; ++i) tie(A[H][i]);
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j) tie(B[S][j]);
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < 2 * NT; ++j)
-        acc.v[H * MT + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(FA::value(A[H][i]), FB::value(B[S][j]), acc.v[H * MT + i][j], 0, 0, 0);
+    unrolled<PRODUCTS>([&](auto n) __attribute__((always_inline)) {
+      constexpr int i = decltype(n)::value / (2 * NT), q = decltype(n)::value % (2 * NT), j = i % 2 ? 2 * NT - 1 - q : q;
+      acc.v[H * MT + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(FA::value(A[H][i]), FB::value(B[S][j]), acc.v[H * MT + i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      between(n);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
   constexpr std::integral_constant<int, 0> c0{};
   constexpr std::integral_constant<int, 1> c1{};
   constexpr std::integral_constant<int, 2> c2{};
   constexpr std::integral_constant<int, 3> c3{};
-#pragma unroll
-  for (int s = 0; s < T::ST; ++s)
-    if (s < steps) {
-      issue(s, lds_base + s * T::STAGE, 0);
-      issue(s, lds_base + s * T::STAGE, 1);
+  constexpr int HALF = COPIES / 2;
+  // A turn of 16 instructions or more (128 and 256 entries a wave... see below) has its reads and copies between them, and the loop no
+  // branches: copies of stages behind the last one read nothing, or the first bytes of a row.
+  constexpr bool SPREAD = PRODUCTS >= 16;
+  auto copy = [&](int s, unsigned at, auto k) __attribute__((always_inline)) {
+    if (SPREAD || s < steps) issue(s, lds_base + at, k);
+  };
+  // a turn: its matrix instructions, the reads of the next one and copies
+  auto turn = [&](auto u, auto reads, auto&& read, auto copies, auto&& next) __attribute__((always_inline)) {
+    constexpr int R = decltype(reads)::value, C = decltype(copies)::value;
+    if constexpr (SPREAD) {
+      lgkm_wait<0>();
+      mul(u, [&](auto n) __attribute__((always_inline)) {
+        constexpr int at = decltype(n)::value;
+        unrolled<R>([&](auto k) __attribute__((always_inline)) { if constexpr (decltype(k)::value * PRODUCTS / (R + 6) == at) read(k); });
+        unrolled<C>([&](auto k) __attribute__((always_inline)) { if constexpr (((2 * decltype(k)::value + 1) * PRODUCTS) / (2 * C) == at) next(k); });
+      });
+    } else {
+      constexpr int OPS = decltype(u)::value == 3 ? 0 : decltype(u)::value == 2 ? RA : RA + RB;
+      unrolled<R>(read);
+      if constexpr (decltype(u)::value != 3) lgkm_wait<OPS>();
+      unrolled<C>(next);
+      mul(u, [](auto) {});
     }
-  if (steps >= T::ST) vm_wait<(T::ST - 1) * COPIES>();
+  };
+  // (the second half of stage ST - 1 is copied in the first turn)
+  unrolled<T::ST * COPIES - (COPIES - HALF)>([&](auto n) __attribute__((always_inline)) {
+    constexpr int s = decltype(n)::value / COPIES;
+    copy(s, s * T::STAGE, std::integral_constant<int, decltype(n)::value % COPIES>{});
+  });
+  unsigned cur = 0, old = (T::ST - 1) * T::STAGE;
+  if (SPREAD || steps >= T::ST) vm_wait<(T::ST - 2) * COPIES + HALF>();
   else vm_wait<0>();
   wg_barrier();
-  read_b(c0, c0);
-  read_b(c0, c1);
-  read_a(c0);
-  // all turns of a stage but the last; in the first one the second half of the copies that the barrier before allowed
-  auto turns = [&](int t) __attribute__((always_inline)) {
-    read_a(c1);
-    read_b(c1, c0);
-    lgkm_wait<RA + RB>();
-    if (t > 0 && t + T::ST - 1 < steps) issue(t + T::ST - 1, lds_base + old, 1);
-    mul(c0);
-    read_a(c2);
-    read_b(c1, c1);
-    lgkm_wait<RA + RB>();
-    mul(c1);
-    read_a(c3);
-    lgkm_wait<RA>();
-    mul(c2);
+  unrolled<2 * NT>([&](auto j) __attribute__((always_inline)) { read_b(c0, j, cur); });
+  unrolled<MT>([&](auto i) __attribute__((always_inline)) { read_a(c0, i, cur); });
+  typedef std::integral_constant<int, MT + NT> ReadsAB;
+  auto none = [](auto) {};
+  int t = 0;
+  do {
+    turn(c0, ReadsAB{}, [&](auto k) __attribute__((always_inline)) {
+          constexpr int n = decltype(k)::value;
+          if constexpr (n < MT) read_a(c1, k, cur);
+          else read_b(c1, std::integral_constant<int, n - MT>{}, cur);
+        }, std::integral_constant<int, COPIES - HALF>{}, [&](auto k) __attribute__((always_inline)) {
+          copy(t + T::ST - 1, old, std::integral_constant<int, HALF + decltype(k)::value>{});
+        });
+    turn(c1, ReadsAB{}, [&](auto k) __attribute__((always_inline)) {
+          constexpr int n = decltype(k)::value;
+          if constexpr (n < MT) read_a(c2, k, cur);
+          else read_b(c1, std::integral_constant<int, NT + n - MT>{}, cur);
+        }, c0, none);
+    turn(c2, std::integral_constant<int, MT>{}, [&](auto k) __attribute__((always_inline)) { read_a(c3, k, cur); }, c0, none);
     lgkm_wait<0>();
-  };
-  for (int t = 0; t < steps - 1; ++t) {
-    turns(t);
-    if (T::ST > 2 && t + T::ST - 1 < steps) vm_wait<(T::ST - 2) * COPIES>();
+    if (SPREAD || t + T::ST - 1 < steps) vm_wait<(T::ST - 2) * COPIES>();
     else vm_wait<0>();
     wg_barrier();
     old = cur;
     cur = cur == (T::ST - 1) * T::STAGE ? 0u : cur + T::STAGE;
-    read_b(c0, c0);
-    read_b(c0, c1);
-    read_a(c0);
-    if (t + T::ST < steps) issue(t + T::ST, lds_base + old, 0);
-    mul(c3);
-  }
-  turns(steps - 1);
-  mul(c3);
+    // (behind the last stage: reads of whatever the buffer holds, which nothing uses)
+    turn(c3, std::integral_constant<int, MT + 2 * NT>{}, [&](auto k) __attribute__((always_inline)) {
+          constexpr int n = decltype(k)::value;
+          if constexpr (n < 2 * NT) read_b(c0, k, cur);
+          else read_a(c0, std::integral_constant<int, n - 2 * NT>{}, cur);
+        }, std::integral_constant<int, HALF>{}, [&](auto k) __attribute__((always_inline)) { copy(t + T::ST, old, k); });
+  } while (++t < steps);
+  lgkm_wait<0>();
+#pragma unroll
+  for (int i = 0; i < MT; ++i) tie(A[0][i]);
+#pragma unroll
+  for (int j = 0; j < 2 * NT; ++j) tie(B[0][j]);
+  vm_wait<0>();  // (the caller's barrier follows before the buffers are used for something else)
 }
 
 // A bf16 tile to memory through LDS, so that rows leave in whole lines: 16 bytes a lane where the rows begin at multiples of

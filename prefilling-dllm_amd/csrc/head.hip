@@ -78,9 +78,10 @@ __device__ __forceinline__ void head_logits(const HeadParams& p, int vt, long ro
       kbytes, wave, lane);
   acc.clear();
   mainloop_bf16<T, false, false>(
-      acc, (int)(kbytes + KB - 1) / KB, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
-        if (part == 0) la.issue(t, dst + wave * (T::LA * 1024));
-        else lb.issue(t, dst + T::A_BYTES + wave * (T::LB * 1024));
+      acc, (int)(kbytes + KB - 1) / KB, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
+        constexpr int I = decltype(copy)::value;
+        if constexpr (I < T::LA) la.template one<I>(t, dst + wave * (T::LA * 1024));
+        else lb.template one<I - T::LA>(t, dst + T::A_BYTES + wave * (T::LB * 1024));
       });
 }
 
@@ -439,13 +440,14 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, ch
   Acc<T> acc;
   acc.clear();
   mainloop_bf16<T, true, false>(
-      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
+      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
+        constexpr int I = decltype(copy)::value;
         const int t1 = t < steps ? t : t - steps;
-        if (part == 0) {
-          la.issue(t1, dst + wave * (T::LA * 1024));
+        if constexpr (I < T::LA) {
+          la.template one<I>(t1, dst + wave * (T::LA * 1024));
         } else {
           lb.base = t < steps ? d0 : d0 + p.plane;
-          lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
+          lb.template one<I - T::LA>(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
         }
       });
 #pragma unroll
@@ -508,13 +510,14 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
   acc.clear();
   const char* d0 = lb.base;
   mainloop_bf16<T, true, true>(
-      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, int part) __attribute__((always_inline)) {
+      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
+        constexpr int I = decltype(copy)::value;
         const int t1 = t < steps ? t : t - steps;
-        if (part == 0) {
-          la.issue(t1, dst + wave * (T::LA * 1024));
+        if constexpr (I < T::LA) {
+          la.template one<I>(t1, dst + wave * (T::LA * 1024));
         } else {
           lb.base = t < steps ? d0 : d0 + p.plane;
-          lb.issue(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
+          lb.template one<I - T::LA>(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
         }
       });
   store_acc<T>(lds, acc, [](float a, float b) __attribute__((always_inline)) { return pack_bf16x2(a, b); }, p.gw + v0 * p.gw_stride + c0,
