@@ -37,10 +37,13 @@ struct HeadParams {
   const float* logp;
   const float* g;
   __bf16* d;      // [N, ldd]: a piece of the softmax gradient, entries from v0 on
-  __bf16* dlo;    // second plane: what the rounding of the first left (or NULL)
   long ldd;
   long v0;        // first entry of the piece; n_voc_tiles covers it
-  char* hz;       // [N, D]: h with the rows of labels outside the vocabulary cleared
+  char* hz;       // [N, D]: h with the rows of labels outside the vocabulary cleared (or NULL: an earlier piece did it)
+  // few rows (np = their number rounded up to 32 or 64): d holds np rows, then np more with what its rounding left; a second
+  // copy dt [entries][2 np] and hz [D][2 np] (every row of h twice) have the rows as the fast index
+  __bf16* dt;
+  int np;
 };
 
 // tile number -> tile: four neighbouring token tiles share a strip of the weight in the L2 of one XCD
@@ -316,8 +319,8 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2* __restrict
 
 // One piece of the softmax gradient, rounded to bf16 as the operand of the two products behind it (each entry off by at
 // most 2^-8 of itself).  For few rows, where few entries make up a result and the products wait for memory anyway, the
-// second plane carries the remainder of the rounding.
-template <class T>
+// remainder of the rounding is kept beside it.
+template <class T, bool FEW>
 __device__ __forceinline__ void head_dlogits_tile(const HeadParams& p, int vt, long row0, char* lds) {
   Acc<T> acc;
   head_logits<T>(p, vt, row0, acc, lds);
@@ -362,47 +365,84 @@ __device__ __forceinline__ void head_dlogits_tile(const HeadParams& p, int vt, l
 #pragma unroll
           for (int j = 0; j < 2 * T::NT; ++j) acc.v[i][j][e] = 0.f;
   }
-  // the remainder of a rounded pair: what the second plane holds
-  auto low = [](float a, float b) __attribute__((always_inline)) {
-    const unsigned w = pack_bf16x2(a, b);
-    return pack_bf16x2(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
-  };
   const long o = row0 * p.ldd + (long)vt * T::TM;
   store_acc<T>(lds, acc, [](float a, float b) __attribute__((always_inline)) { return pack_bf16x2(a, b); }, p.d + o, p.ldd, p.N - row0, T::TM);
-  if (p.dlo) store_acc<T>(lds, acc, low, p.dlo + o, p.ldd, p.N - row0, T::TM);
+  if constexpr (FEW) {
+    // the remainder of a rounded pair
+    auto low = [](float a, float b) __attribute__((always_inline)) {
+      const unsigned w = pack_bf16x2(a, b);
+      return pack_bf16x2(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
+    };
+    store_acc<T>(lds, acc, low, p.d + p.np * p.ldd + o, p.ldd, p.N, T::TM);
+    // the same with the rows as the fast index, through LDS: [entries of the tile][2 np], 16 bytes behind each
+    const int pitch = 4 * p.np + 16;
+    static_assert(T::TN == 64 && T::TM * (4 * 64 + 16) <= T::LDS, "");
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2 * T::NT; ++j) {
+      const int r = r_wave + 16 * j + l16;
+      if (r >= p.np) break;
+#pragma unroll
+      for (int i = 0; i < 2 * T::MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const float x = acc.v[i][j][e], y = acc.v[i][j][e + 1];
+          const unsigned h = pack_bf16x2(x, y), l = low(x, y);
+          char* at = lds + (v_wave + 16 * i + g4 + e) * pitch + 2 * r;
+          *reinterpret_cast<unsigned short*>(at) = (unsigned short)h;
+          *reinterpret_cast<unsigned short*>(at + pitch) = (unsigned short)(h >> 16);
+          *reinterpret_cast<unsigned short*>(at + 2 * p.np) = (unsigned short)l;
+          *reinterpret_cast<unsigned short*>(at + pitch + 2 * p.np) = (unsigned short)(l >> 16);
+        }
+    }
+    __syncthreads();
+    const int chunks = p.np / 4;  // of a row
+    char* dt = reinterpret_cast<char*>(p.dt + (long)vt * T::TM * (2 * p.np));
+    for (int k = threadIdx.x; k < T::TM * chunks; k += T::THREADS)
+      *reinterpret_cast<uint4*>(dt + 16L * k) = *reinterpret_cast<const uint4*>(lds + k / chunks * pitch + k % chunks * 16);
+  }
 }
 
-template <class T, class TS>
+template <class T, class TS, bool FEW>
 __global__ __launch_bounds__(T::THREADS, 2) void head_dlogits_kernel(const HeadParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS > TS::LDS ? T::LDS : TS::LDS];
   if (p.hz) {
     // grad_w must not see the rows without a label (their states may hold anything): a copy with those rows cleared
     const int chunks = p.D / 8;
-    for (long i = (long)blockIdx.x * T::THREADS + threadIdx.x; i < p.N * chunks; i += (long)gridDim.x * T::THREADS) {
-      const long r = i / chunks;
-      const int c = (int)(i - r * chunks);
-      const long lab = p.labels[r];
+    const long rows = FEW ? p.np : p.N;
+    for (long i = (long)blockIdx.x * T::THREADS + threadIdx.x; i < rows * chunks; i += (long)gridDim.x * T::THREADS) {
+      const long r = FEW ? i % p.np : i / chunks;
+      const int c = (int)(FEW ? i / p.np : i - r * chunks);
+      const long lab = !FEW || r < p.N ? p.labels[r] : -1;
       uint4 v = {0, 0, 0, 0};
       if (lab >= 0 && lab < p.V) v = *reinterpret_cast<const uint4*>(p.h + r * p.h_stride + 16 * c);
-      *reinterpret_cast<uint4*>(p.hz + i * 16) = v;
+      if constexpr (FEW) {
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+        unsigned short* o = reinterpret_cast<unsigned short*>(p.hz) + (long)c * 8 * (2 * p.np) + r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e * 2 * p.np] = o[e * 2 * p.np + p.np] = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+      } else {
+        *reinterpret_cast<uint4*>(p.hz + i * 16) = v;
+      }
     }
   }
   head_dispatch<T, TS>(p, [&](auto* t, int vt, long row0) __attribute__((always_inline)) {
-    head_dlogits_tile<std::remove_pointer_t<decltype(t)>>(p, vt, row0, lds);
+    head_dlogits_tile<std::remove_pointer_t<decltype(t)>, FEW>(p, vt, row0, lds);
   });
 }
 
 struct GradParams {
   const char* w;   // rows of the weight from the piece's first on
-  const char* hz;  // [N, D]
-  const char* d;   // [planes][N, ldd]
-  long plane;      // bytes between the planes of d
+  const char* hz;  // [N, D], few rows: [D][2 np]
+  const char* d;   // [N, ldd], few rows: [2 np, ldd]
+  const char* dt;  // few rows: [entries][2 np]
   long w_stride, ldd;  // bytes
   long N;
   long vp;         // entries of the piece
-  int D, planes;
+  int D;
   int m_tiles, n_tiles, splits;  // of grad_h: column tiles, row tiles, splits of the entries
   int w_tiles;                   // of grad_w: column tiles
+  int v_per;                     // of grad_w of few rows: entries of a wave
   long k_per;      // entries per split, a multiple of 64
   float* acc;      // [splits][N][D]
   __bf16* gh;      // written directly when the one split of the one piece is all of the sum
@@ -412,8 +452,9 @@ struct GradParams {
   long gw_stride;  // elements
 };
 
-// grad_h of a piece: acc[split][row][c] (+)= sum over the split's entries of d[row][v] w[v][c]
-template <class T>
+// grad_h of a piece: acc[split][row][c] (+)= sum over the split's entries of d[row][v] w[v][c].  Few rows: the tile holds all of them
+// and behind them the remainders' rows, whose results a lane has beside the others.
+template <class T, bool FEW>
 __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, char* lds) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -435,23 +476,17 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, ch
   LoadKC<T::LB> lb;
   const unsigned kb = (unsigned)KB * steps;  // d is padded with zeros to whole stages
   const char* d0 = p.d + r0 * p.ldd + 2 * k0;
-  lb.init(d0, p.N - r0, (unsigned)p.ldd, kb, wave, lane);
-  d0 = lb.base;
+  lb.init(d0, FEW ? T::TN : p.N - r0, (unsigned)p.ldd, kb, wave, lane);
   Acc<T> acc;
   acc.clear();
   mainloop_bf16<T, true, false>(
-      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
+      acc, steps, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
         constexpr int I = decltype(copy)::value;
-        const int t1 = t < steps ? t : t - steps;
-        if constexpr (I < T::LA) {
-          la.template one<I>(t1, dst + wave * (T::LA * 1024));
-        } else {
-          lb.base = t < steps ? d0 : d0 + p.plane;
-          lb.template one<I - T::LA>(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
-        }
+        if constexpr (I < T::LA) la.template one<I>(t, dst + wave * (T::LA * 1024));
+        else lb.template one<I - T::LA>(t, dst + T::A_BYTES + wave * (T::LB * 1024));
       });
 #pragma unroll
-  for (int j = 0; j < 2 * T::NT; ++j) {
+  for (int j = 0; j < (FEW ? T::NT : 2 * T::NT); ++j) {
     const long row = r0 + wn * (32 * T::NT) + 16 * j + l16;
     if (row >= p.N) continue;
     float* out = p.acc + ((long)split * p.N + row) * p.D;
@@ -460,6 +495,7 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, ch
       const int c = c0 + wm * (32 * T::MT) + 16 * i + 4 * g;
       if (c >= p.D) continue;
       f32x4 v = acc.v[i][j];
+      if constexpr (FEW) v += acc.v[i][j + T::NT];
       if (p.gh) {
         *reinterpret_cast<uint2*>(p.gh + row * p.gh_stride + c) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
         continue;
@@ -508,17 +544,11 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
   lb.init(p.d + 2 * v0, p.ldd, p.N, 2u * T::TN, wave, lane);  // the rows of d are whole tiles long
   Acc<T> acc;
   acc.clear();
-  const char* d0 = lb.base;
   mainloop_bf16<T, true, true>(
-      acc, steps * p.planes, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
+      acc, steps, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
         constexpr int I = decltype(copy)::value;
-        const int t1 = t < steps ? t : t - steps;
-        if constexpr (I < T::LA) {
-          la.template one<I>(t1, dst + wave * (T::LA * 1024));
-        } else {
-          lb.base = t < steps ? d0 : d0 + p.plane;
-          lb.template one<I - T::LA>(t1, dst + T::A_BYTES + wave * (T::LB * 1024));
-        }
+        if constexpr (I < T::LA) la.template one<I>(t, dst + wave * (T::LA * 1024));
+        else lb.template one<I - T::LA>(t, dst + T::A_BYTES + wave * (T::LB * 1024));
       });
   store_acc<T>(lds, acc, [](float a, float b) __attribute__((always_inline)) { return pack_bf16x2(a, b); }, p.gw + v0 * p.gw_stride + c0,
                p.gw_stride, p.vp - v0, p.D - c0);
@@ -527,15 +557,85 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
 // Both products of a piece in one launch: the tiles of grad_h first (few, with the whole piece to sum over), those of grad_w
 // (many, with the rows to sum over) fill the compute units they leave.
 // The small tiles (80 KB of LDS, at most 128 registers) leave room for two workgroups on a compute unit, which hide each other's
-// start and end: with few rows a tile of grad_w is two or three stages and then 64 KB of results.
+// start and end: with few rows a tile of grad_w is a few stages and then 32 KB of results.
 template <class TH, class TW>
 __global__ __launch_bounds__(TW::THREADS, TW::MT * TW::NT <= 2 ? 4 : 2) void head_grad_kernel(const GradParams p) {
   static_assert(TH::THREADS == TW::THREADS, "");
   __shared__ __attribute__((aligned(1024))) char lds[TH::LDS > TW::LDS ? TH::LDS : TW::LDS];
 #ifdef __HIP_DEVICE_COMPILE__  // (the host compiler cannot resolve the calls: their lambdas hold buffer descriptors)
   const int n_h = p.m_tiles * p.n_tiles * p.splits;
-  if ((int)blockIdx.x < n_h) head_grad_h_tile<TH>(p, xcd_remap(blockIdx.x, n_h), lds);
+  if ((int)blockIdx.x < n_h) head_grad_h_tile<TH, false>(p, xcd_remap(blockIdx.x, n_h), lds);
   else head_grad_w_tile<TW>(p, xcd_remap(blockIdx.x - n_h, gridDim.x - n_h), lds);
+#endif
+}
+
+// grad_w of few rows: 2 np products for each result, so the call waits for its results to be written.  Each wave keeps its
+// columns of h in registers and goes through its entries by itself, 16 at a time: one fragment of d, the products, a
+// store of 8 columns a lane (block 2 q holds columns 32 q + 8 g + e, e < 4, in lane group g, block 2 q + 1 those four further on).
+template <int NT>
+constexpr int few_columns = NT == 2 ? 128 : 64;  // of a wave: as many as the registers hold
+template <int NT>
+__device__ __forceinline__ void head_grad_w_few(const GradParams& p, long id) {
+  constexpr int C = few_columns<NT>, BLOCKS = C / 16, ROW = 64 * NT;  // bytes of a row of hz and dt
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int ct = __builtin_amdgcn_readfirstlane((int)(id % p.w_tiles));
+  const long v0 = (long)__builtin_amdgcn_readfirstlane((int)(id / p.w_tiles)) * p.v_per;
+  const long v1 = v0 + p.v_per < p.vp ? v0 + p.v_per : p.vp;
+  if (v0 >= p.vp) return;
+  const int c0 = ct * C;
+  bf16x8 a[BLOCKS][NT];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    const int c = c0 + 32 * (b / 2) + 8 * (l16 >> 2) + 4 * (b & 1) + (l16 & 3);
+    const char* at = p.hz + (long)(c < p.D ? c : p.D - 1) * ROW + 16 * g;
+#pragma unroll
+    for (int k = 0; k < NT; ++k) a[b][k] = *reinterpret_cast<const bf16x8*>(at + 64 * k);
+  }
+  const char* src = p.dt + (v0 + l16) * ROW + 16 * g;
+  bf16x8 d[NT], next[NT];
+#pragma unroll
+  for (int k = 0; k < NT; ++k) next[k] = *reinterpret_cast<const bf16x8*>(src + 64 * k);
+  const bool wide = (((uintptr_t)p.gw | (uintptr_t)(2 * p.gw_stride)) & 15) == 0;
+  for (long v = v0; v < v1; v += 16) {
+#pragma unroll
+    for (int k = 0; k < NT; ++k) d[k] = next[k];
+    if (v + 16 < v1) {
+      src += 16 * ROW;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) next[k] = *reinterpret_cast<const bf16x8*>(src + 64 * k);
+    }
+    f32x4 acc[BLOCKS];
+#pragma unroll
+    for (int k = 0; k < NT; ++k)
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+        acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[b][k], d[k], k == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[b], 0, 0, 0);
+    if (v + l16 >= v1) continue;
+    __bf16* out = p.gw + (v + l16) * p.gw_stride + c0 + 8 * g;
+#pragma unroll
+    for (int q = 0; q < BLOCKS / 2; ++q) {
+      if (c0 + 32 * q + 8 * g >= p.D) continue;
+      const uint4 w = {pack_bf16x2(acc[2 * q][0], acc[2 * q][1]), pack_bf16x2(acc[2 * q][2], acc[2 * q][3]),
+                       pack_bf16x2(acc[2 * q + 1][0], acc[2 * q + 1][1]), pack_bf16x2(acc[2 * q + 1][2], acc[2 * q + 1][3])};
+      if (wide) {
+        *reinterpret_cast<uint4*>(out + 32 * q) = w;
+      } else {
+        *reinterpret_cast<uint2*>(out + 32 * q) = {w.x, w.y};
+        *reinterpret_cast<uint2*>(out + 32 * q + 4) = {w.z, w.w};
+      }
+    }
+  }
+}
+
+// Both products of up to 16 NT rows: tiles of grad_h, 256 columns x all rows and a share of the piece, then the waves of grad_w.
+template <int NT>
+__global__ __launch_bounds__(512, 4) void head_grad_few_kernel(const GradParams p) {
+  typedef Tile<1, NT, 8, 1, 2> T;
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
+#ifdef __HIP_DEVICE_COMPILE__
+  const int n_h = p.m_tiles * p.splits;
+  if ((int)blockIdx.x < n_h) head_grad_h_tile<T, true>(p, xcd_remap(blockIdx.x, n_h), lds);
+  else head_grad_w_few<NT>(p, 8L * xcd_remap(blockIdx.x - n_h, gridDim.x - n_h) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 #endif
 }
 
@@ -623,13 +723,13 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
 // ---- gradient: sizes of the workspace's regions ----
 constexpr long kPieceBytes = 256L << 20;  // the piece of d the products read back stays within the last-level cache
 constexpr long kMaxPiece = 1L << 21;        // 256 rows of a piece lie within 31-bit offsets
-constexpr int kPlaneRows = 64;            // up to here the second plane is carried
+constexpr int kFewRows = 64;                // up to here the remainders are carried
 
 struct GradPlan {
-  long planes, ldd, vp;  // ldd = entries of a piece (a multiple of 256)
-  int splits, small;     // small: the small tiles
-  int direct;            // grad_h needs no accumulators
-  int64_t hz, d, acc;    // bytes
+  int np, splits, small;  // np: rows of few, rounded up (or 0); small: the small tiles
+  long vp;                // entries of a piece (a multiple of 256)
+  int direct;             // grad_h needs no accumulators
+  int64_t hz, d, dt, acc;  // bytes
 };
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
@@ -637,37 +737,39 @@ int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 // Pieces as long as the workspace allows, up to kPieceBytes of d: of 4096 rows 32768 entries, 128 x 16 tiles of logits and 128 x 14 of
 // grad_w (3584 columns), whole rounds of the 256 compute units.  have < 0: the size that is asked for.
 bool plan_grad(long n, long v, int d, int64_t have, GradPlan& g) {
-  g.planes = n <= kPlaneRows ? 2 : 1;
+  g.np = n <= 32 ? 32 : n <= kFewRows ? 64 : 0;
   const long vall = (v + 255) / 256 * 256;
   // the small tiles where the sums over rows are short or the large ones would leave compute units idle
   g.small = n <= 256 || ((d + 255) / 256) * (vall / 256) < 192;
-  const long tiles = ((d + 255) / 256) * (g.small ? (n + 63) / 64 : (n + 255) / 256);
-  const long slots = g.small ? 512 : 256;  // workgroups at a time
+  const long tiles = ((d + 255) / 256) * (g.np ? 1 : g.small ? (n + 63) / 64 : (n + 255) / 256);
+  const long slots = g.np == 64 || !g.small ? 256 : 512;  // workgroups at a time
   const long most = tiles < slots ? slots / tiles : 1;
-  g.hz = align256(2L * n * d);
-  for (long piece = kPieceBytes / (2 * n * g.planes);; piece = g.vp / 2) {
+  const long rows = g.np ? 2 * g.np : n;  // of d
+  g.hz = align256(2L * rows * d);
+  for (long piece = kPieceBytes / (2 * rows);; piece = g.vp / 2) {
     piece = piece < kMaxPiece ? piece : kMaxPiece;
     piece = piece >= 8192 ? piece / 4096 * 4096 : piece / 256 * 256;
     piece = piece < 256 ? 256 : (piece < vall ? piece : vall);
     // grad_h: enough splits of the piece for every compute unit, at least four stages each
     const long s = piece / 256;
     g.splits = (int)(s < 1 ? 1 : (s < most ? s : most));
-    g.ldd = g.vp = piece;
-    g.d = align256(2L * n * piece * g.planes);
+    g.vp = piece;
+    g.d = align256(2L * rows * piece);
+    g.dt = g.np ? g.d : 0;
     // a short sum is not split: the launch that would join the splits costs more than 16 stages
     g.direct = piece >= vall && (g.splits == 1 || vall <= 1024);
     if (g.direct) g.splits = 1;
     g.acc = g.direct ? 0 : align256(4L * g.splits * n * d);
-    if (have < 0 || g.hz + g.d + g.acc <= have) return true;
+    if (have < 0 || g.hz + g.d + g.dt + g.acc <= have) return true;
     if (piece <= 256) return false;
   }
 }
 
-template <class T, class TS>
+template <class T, class TS, bool FEW>
 int launch_dlogits(HeadParams& p, hipStream_t s) {
   const long grid = head_grid<T, TS>(p);
   if (grid < 0) return PDLLM_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((head_dlogits_kernel<T, TS>), dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
+  hipLaunchKernelGGL((head_dlogits_kernel<T, TS, FEW>), dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
   return launch_status();
 }
 
@@ -772,7 +874,7 @@ extern "C" int64_t pdllm_head_selfinfo_grad_workspace_bytes(int64_t n_rows, int6
   if (n_rows == 0) return 0;
   GradPlan g;
   plan_grad(n_rows, vocab, dim, -1, g);
-  return g.hz + g.d + g.acc;
+  return g.hz + g.d + g.dt + g.acc;
 }
 
 extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
@@ -790,7 +892,6 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
   if (n_rows == 0) {  // a sum over no rows
     GradParams q = {};
     q.D = dim;
-    q.planes = 1;
     q.w_tiles = (dim + 255) / 256;  // (no tiles of grad_h)
     const long tiles = q.w_tiles * ((vocab + 255) / 256);
     q.vp = vocab;
@@ -817,33 +918,33 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
   p.logp = logp;
   p.g = grad_logp;
   p.d = reinterpret_cast<__bf16*>(ws + g.hz);
-  p.dlo = g.planes > 1 ? p.d + n_rows * g.ldd : nullptr;
-  p.ldd = g.ldd;
+  p.dt = reinterpret_cast<__bf16*>(ws + g.hz + g.d);
+  p.np = g.np;
+  p.ldd = g.vp;
   GradParams q = {};
   q.hz = ws;
   q.d = ws + g.hz;
-  q.plane = 2 * n_rows * g.ldd;
+  q.dt = ws + g.hz + g.d;
   q.w_stride = p.w_stride;
-  q.ldd = 2 * g.ldd;
+  q.ldd = 2 * g.vp;
   q.N = n_rows;
   q.D = dim;
-  q.planes = (int)g.planes;
   q.m_tiles = (dim + 255) / 256;
-  const int tw = g.small ? TileW2::TM : TileH::TM;
+  const bool few = g.np != 0;
   static_assert(TileW2::TM == TileW2::TN && TileH::TM == TileH::TN, "square tiles");
+  const int tw = few ? (g.np <= 32 ? few_columns<2> : few_columns<4>) : g.small ? TileW2::TM : TileH::TM;
   q.w_tiles = (dim + tw - 1) / tw;
-  q.n_tiles = (int)(g.small ? (n_rows + TileH2::TN - 1) / TileH2::TN : (n_rows + TileH::TN - 1) / TileH::TN);
-  q.acc = reinterpret_cast<float*>(ws + g.hz + g.d);
+  q.n_tiles = (int)(few ? 1 : g.small ? (n_rows + TileH2::TN - 1) / TileH2::TN : (n_rows + TileH::TN - 1) / TileH::TN);
+  q.acc = reinterpret_cast<float*>(ws + g.hz + g.d + g.dt);
   q.gw_stride = grad_weight_stride;
   q.gh = g.direct ? static_cast<__bf16*>(grad_hidden) : nullptr;
   q.gh_stride = grad_hidden_stride;
-  const bool few = n_rows <= 64;
   for (long v0 = 0; v0 < vocab; v0 += g.vp) {
     const long vp = vocab - v0 < g.vp ? vocab - v0 : g.vp;
     p.v0 = v0;
     p.hz = v0 == 0 ? ws : nullptr;
     p.n_voc_tiles = (int)((vp + (few ? TileS2::TM : TileL::TM) - 1) / (few ? TileS2::TM : TileL::TM));
-    st = few ? launch_dlogits<TileS2, TileS2>(p, s) : launch_dlogits<TileL, TileR>(p, s);
+    st = few ? launch_dlogits<TileS2, TileS2, true>(p, s) : launch_dlogits<TileL, TileR, false>(p, s);
     if (st != PDLLM_OK) return st;
     q.w = p.w + v0 * p.w_stride;
     q.vp = vp;
@@ -851,10 +952,16 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     q.splits = g.splits;
     q.k_per = ((vp + g.splits - 1) / g.splits + 63) / 64 * 64;
     q.gw = static_cast<__bf16*>(grad_weight) + v0 * grad_weight_stride;
-    const long grid = (long)q.m_tiles * q.n_tiles * q.splits + (long)q.w_tiles * ((vp + tw - 1) / tw);
+    // few rows: 256 entries to a wave (16 KB of h read for 64 KB of results), fewer where the card would not be full
+    q.v_per = q.w_tiles * ((vp + 255) / 256) >= 4096 ? 256 : 64;
+    const long n_w = few ? (q.w_tiles * ((vp + q.v_per - 1) / q.v_per) + 7) / 8 : q.w_tiles * ((vp + tw - 1) / tw);
+    const long grid = (long)q.m_tiles * q.n_tiles * q.splits + n_w;
     if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
-    if (g.small) hipLaunchKernelGGL((head_grad_kernel<TileH2, TileW2>), dim3((unsigned)grid), dim3(TileW2::THREADS), 0, s, q);
-    else hipLaunchKernelGGL((head_grad_kernel<TileH, TileH>), dim3((unsigned)grid), dim3(TileH::THREADS), 0, s, q);
+    const dim3 blocks((unsigned)grid), threads(512);
+    if (g.np == 32) hipLaunchKernelGGL(head_grad_few_kernel<2>, blocks, threads, 0, s, q);
+    else if (g.np == 64) hipLaunchKernelGGL(head_grad_few_kernel<4>, blocks, threads, 0, s, q);
+    else if (g.small) hipLaunchKernelGGL((head_grad_kernel<TileH2, TileW2>), blocks, threads, 0, s, q);
+    else hipLaunchKernelGGL((head_grad_kernel<TileH, TileH>), blocks, threads, 0, s, q);
     if ((st = launch_status()) != PDLLM_OK) return st;
   }
   if (g.direct) return PDLLM_OK;

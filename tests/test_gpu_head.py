@@ -102,9 +102,10 @@ def test_gradient_in_pieces(dev):
         logp, lse = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
         full = ops.head_selfinfo_grad(h, w, labels, logp, lse, g)
         need = int(_lib.lib.pdllm_head_selfinfo_grad_workspace_bytes(n, 5000, 264))
-        planes = 2 if n <= 64 else 1
-        least = 2 * n * 264 + 2 * n * 256 * planes + 4 * n * 264 + 3 * 256
-        for have in (need // 2, least + 2 * n * 256 * planes, least):
+        # a copy of the states, a piece of 256 entries, fp32 sums; up to 64 rows: rounded up to 32 or 64, twice, and the piece twice
+        rows, copies = (128, 2) if n <= 64 else (n, 1)
+        least = 2 * rows * 264 + 2 * rows * 256 * copies + 4 * n * 264 + 3 * 256
+        for have in (need // 2, least + 2 * rows * 256 * copies, least):
             got = ops.head_selfinfo_grad(h, w, labels, logp, lse, g, max_workspace_bytes=have)
             check_grad(*got, h, w, d)
             assert torch.equal(got[1], full[1])             # grad_w does not depend on the pieces
