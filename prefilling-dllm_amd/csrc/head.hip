@@ -572,11 +572,10 @@ __global__ __launch_bounds__(TW::THREADS, TW::MT * TW::NT <= 2 ? 4 : 2) void hea
 // grad_w of few rows: 2 np products for each result, so the call waits for its results to be written.  Each wave keeps its
 // columns of h in registers and goes through its entries by itself, 16 at a time: one fragment of d, the products, a
 // store of 8 columns a lane (block 2 q holds columns 32 q + 8 g + e, e < 4, in lane group g, block 2 q + 1 those four further on).
-template <int NT>
-constexpr int few_columns = NT == 2 ? 128 : 64;  // of a wave: as many as the registers hold
+constexpr int kFewColumns = 64;  // of a wave (128, with half the waves' registers for them, were no faster)
 template <int NT>
 __device__ __forceinline__ void head_grad_w_few(const GradParams& p, long id) {
-  constexpr int C = few_columns<NT>, BLOCKS = C / 16, ROW = 64 * NT;  // bytes of a row of hz and dt
+  constexpr int C = kFewColumns, BLOCKS = C / 16, ROW = 64 * NT;  // bytes of a row of hz and dt
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int ct = __builtin_amdgcn_readfirstlane((int)(id % p.w_tiles));
   const long v0 = (long)__builtin_amdgcn_readfirstlane((int)(id / p.w_tiles)) * p.v_per;
@@ -932,7 +931,7 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
   q.m_tiles = (dim + 255) / 256;
   const bool few = g.np != 0;
   static_assert(TileW2::TM == TileW2::TN && TileH::TM == TileH::TN, "square tiles");
-  const int tw = few ? (g.np <= 32 ? few_columns<2> : few_columns<4>) : g.small ? TileW2::TM : TileH::TM;
+  const int tw = few ? kFewColumns : g.small ? TileW2::TM : TileH::TM;
   q.w_tiles = (dim + tw - 1) / tw;
   q.n_tiles = (int)(few ? 1 : g.small ? (n_rows + TileH2::TN - 1) / TileH2::TN : (n_rows + TileH::TN - 1) / TileH::TN);
   q.acc = reinterpret_cast<float*>(ws + g.hz + g.d + g.dt);
@@ -952,8 +951,8 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     q.splits = g.splits;
     q.k_per = ((vp + g.splits - 1) / g.splits + 63) / 64 * 64;
     q.gw = static_cast<__bf16*>(grad_weight) + v0 * grad_weight_stride;
-    // few rows: 256 entries to a wave (16 KB of h read for 64 KB of results), fewer where the card would not be full
-    q.v_per = q.w_tiles * ((vp + 255) / 256) >= 4096 ? 256 : 64;
+    // few rows: 512 entries to a wave (8 or 16 KB of h read for 64 KB of results), fewer where the card would not be full
+    q.v_per = q.w_tiles * ((vp + 511) / 512) >= 4096 ? 512 : 64;
     const long n_w = few ? (q.w_tiles * ((vp + q.v_per - 1) / q.v_per) + 7) / 8 : q.w_tiles * ((vp + tw - 1) / tw);
     const long grid = (long)q.m_tiles * q.n_tiles * q.splits + n_w;
     if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
