@@ -79,7 +79,6 @@ __device__ __forceinline__ void head_logits(const HeadParams& p, int vt, long ro
         return p.h + t * p.h_stride;
       },
       kbytes, wave, lane);
-  acc.clear();
   mainloop_bf16<T, false, false>(
       acc, (int)(kbytes + KB - 1) / KB, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
         constexpr int I = decltype(copy)::value;
@@ -478,7 +477,6 @@ __device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, ch
   const char* d0 = p.d + r0 * p.ldd + 2 * k0;
   lb.init(d0, FEW ? T::TN : p.N - r0, (unsigned)p.ldd, kb, wave, lane);
   Acc<T> acc;
-  acc.clear();
   mainloop_bf16<T, true, false>(
       acc, steps, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
         constexpr int I = decltype(copy)::value;
@@ -543,7 +541,6 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
   LoadKS<T::LB, T::TN> lb;
   lb.init(p.d + 2 * v0, p.ldd, p.N, 2u * T::TN, wave, lane);  // the rows of d are whole tiles long
   Acc<T> acc;
-  acc.clear();
   mainloop_bf16<T, true, true>(
       acc, steps, lds_base, [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
         constexpr int I = decltype(copy)::value;
