@@ -131,24 +131,25 @@ struct Fp8Params {
   int m_tiles, n_tiles;  // tiles of output features, of rows
 };
 
-// A wave's operand fragments, blocks of 32 rows: step ks holds, in lane half h, the 16 bytes of k at 32 ks + 16 h of its row; two
-// steps make one operand of the 32x32x64 instruction (k is permuted alike in both operands, which a sum over k does not see).
+// A wave's operand fragments, blocks of 16 rows: lane 16 g + l holds, of row l, the 16 bytes of k at 16 g and at 64 + 16 g (any order
+// that both operands share does).
 struct Frag8 {
-  unsigned a[4];
+  unsigned a[2];
   __device__ __forceinline__ void init(unsigned lds_base, int first, int lane) {
-    const int l32 = lane & 31, h = lane >> 5;
+    const int l16 = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) a[ks] = lds_base + (first + l32) * KB + (((2 * ks + h) ^ kc_xor(l32)) << 4);
+    for (int q = 0; q < 2; ++q) a[q] = lds_base + (first + l16) * KB + (((4 * q + g) ^ kc_xor(l16)) << 4);
   }
-  template <int KS, int J>
-  __device__ __forceinline__ void read(bf16x8& d, unsigned stage) const {
-    lds_read_b128<J * 32 * KB>(d, a[KS] + stage);
+  template <int J>
+  __device__ __forceinline__ void read(bf16x8 (&d)[2], unsigned stage) const {
+    lds_read_b128<J * 16 * KB>(d[0], a[0] + stage);
+    lds_read_b128<J * 16 * KB>(d[1], a[1] + stage);
   }
 };
 
 template <class T>
 __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31;
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   const unsigned lds_base = (unsigned)(size_t)lds;
@@ -166,171 +167,131 @@ __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
   la.init(p.w + f0 * p.w_stride, p.N - f0, (unsigned)p.w_stride, (unsigned)p.K, wave, lane);
   LoadKC<T::LB> lb;
   lb.init(p.x + r0 * p.x_stride, p.M - r0, (unsigned)p.x_stride, (unsigned)p.K, wave, lane);
-  auto issue = [&](int t, unsigned dst) __attribute__((always_inline)) {
-    la.issue(t, dst + wave * (T::LA * 1024));
-    lb.issue(t, dst + T::A_BYTES + wave * (T::LB * 1024));
+  auto issue = [&](int t, unsigned dst, auto copy) __attribute__((always_inline)) {
+    constexpr int I = decltype(copy)::value;
+    if constexpr (I < T::LA) la.template one<I>(t, dst + wave * (T::LA * 1024));
+    else lb.template one<I - T::LA>(t, dst + T::A_BYTES + wave * (T::LB * 1024));
   };
   // scales: the wave's features lie in one block of 128
   const long fw = f0 + wm * (32 * T::MT);
   const long fb = fw < p.N ? fw / 128 : (p.N - 1) / 128;
   const float* sw = p.sw + fb * p.sw_row;
   const float* sx = p.sx + r0 * p.sx_row;
-  unsigned sx_off[T::NT];
+  constexpr int NI = 2 * T::MT, NJ = 2 * T::NT;  // blocks of 16 features, of 16 rows
+  unsigned sx_off[NJ];
 #pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
-    const int row = (wn * T::NT + j) * 32 + l32;
+  for (int j = 0; j < NJ; ++j) {
+    const int row = wn * (32 * T::NT) + 16 * j + l16;
     sx_off[j] = (unsigned)(r0 + row < p.M ? row : (int)(p.M - 1 - r0)) * (unsigned)p.sx_row;
   }
 
   Frag8 fa, fb_;
   fa.init(lds_base, wm * T::MT * 32, lane);
   fb_.init(lds_base + T::A_BYTES, wn * T::NT * 32, lane);
-  f32x16 acc[T::MT][T::NT];
-#pragma unroll
-  for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < T::NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  Acc<T> acc;
+  acc.clear();
   const int steps = (p.K + 127) / 128;
-  constexpr int COPIES = T::LA + T::LB;
+  constexpr int COPIES = T::LA + T::LB, HALF = COPIES / 2;
   // The scales of a stage are fetched ST - 1 stages ahead, right in front of the copies of the stage behind it: loads return in
   // order, so waiting for them never waits for copies that are not needed yet.
   constexpr int AHEAD = T::ST - 1;
-  float sc[T::NT], qx[AHEAD][T::NT], qw[AHEAD];
-  auto fetch = [&](int t, float (&x)[T::NT], float& w) __attribute__((always_inline)) {
+  float sc[NJ], qx[AHEAD][NJ], qw[AHEAD];
+  auto fetch = [&](int t, float (&x)[NJ], float& w) __attribute__((always_inline)) {
     t = t < steps ? t : steps - 1;
     w = sw[t * p.sw_blk];
 #pragma unroll
-    for (int j = 0; j < T::NT; ++j) x[j] = (sx + t * p.sx_blk)[sx_off[j]];
+    for (int j = 0; j < NJ; ++j) x[j] = (sx + t * p.sx_blk)[sx_off[j]];
   };
 #pragma unroll
   for (int a = 0; a < AHEAD; ++a) fetch(a, qx[a], qw[a]);
-#pragma unroll
-  for (int s = 0; s < T::ST; ++s)
-    if (s < steps) issue(s, lds_base + s * T::STAGE);
-  if (steps >= T::ST) vm_wait<(T::ST - 1) * COPIES>();
-  else vm_wait<0>();
+  // Copies of stages behind the last one read nothing: no branches in the loop.  The second half of stage ST - 1 follows in the
+  // first stage.
+  unrolled<T::ST * COPIES - (COPIES - HALF)>([&](auto n) __attribute__((always_inline)) {
+    constexpr int s = decltype(n)::value / COPIES;
+    issue(s, lds_base + s * T::STAGE, std::integral_constant<int, decltype(n)::value % COPIES>{});
+  });
+  vm_wait<(T::ST - 2) * COPIES + HALF>();
   wg_barrier();
-  unsigned cur = 0;
-  bf16x8 A[2][4], B[T::NT][4];
-  auto read_a = [&](auto jt, bf16x8 (&d)[4]) __attribute__((always_inline)) {
-    constexpr int J = decltype(jt)::value;
-    fa.template read<0, J>(d[0], cur);
-    fa.template read<1, J>(d[1], cur);
-    fa.template read<2, J>(d[2], cur);
-    fa.template read<3, J>(d[3], cur);
-  };
-  auto read_b = [&](auto jt, bf16x8 (&d)[4]) __attribute__((always_inline)) {
-    constexpr int J = decltype(jt)::value;
-    fb_.template read<0, J>(d[0], cur);
-    fb_.template read<1, J>(d[1], cur);
-    fb_.template read<2, J>(d[2], cur);
-    fb_.template read<3, J>(d[3], cur);
-  };
-  auto pair = [](const bf16x8& a, const bf16x8& b) __attribute__((always_inline)) {
+  unsigned cur = 0, old = (T::ST - 1) * T::STAGE;
+  bf16x8 A[2][2], B[NJ][2];  // A: this block and the next
+  unrolled<NJ>([&](auto j) __attribute__((always_inline)) { fb_.template read<decltype(j)::value>(B[decltype(j)::value], cur); });
+  fa.template read<0>(A[0], cur);
+  auto whole = [](const bf16x8 (&a)[2]) __attribute__((always_inline)) {
     typedef __attribute__((ext_vector_type(4))) int i32x4;
-    return __builtin_shufflevector(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_shufflevector(__builtin_bit_cast(i32x4, a[0]), __builtin_bit_cast(i32x4, a[1]), 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  constexpr std::integral_constant<int, 0> c0{};
-  constexpr std::integral_constant<int, (T::NT > 1 ? 1 : 0)> n1{};
-  constexpr std::integral_constant<int, (T::MT > 1 ? 1 : 0)> m1{};
-  constexpr std::integral_constant<int, (T::MT > 2 ? 2 : 0)> m2{};
-  constexpr std::integral_constant<int, (T::MT > 3 ? 3 : 0)> m3{};
-  read_a(c0, A[0]);
-  read_b(c0, B[0]);
-  if constexpr (T::NT > 1) read_b(n1, B[1]);
-  f32x16 zero;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  int t = 0;
+  do {
+    // Blocks of 16 features in turn.  The products of a block of 16 x 16 are added to the accumulators behind the matrix
+    // instruction after the next one, so that the additions never wait for their result.
+    f32x4 d[3];
+    auto add = [&](auto n_tag) __attribute__((always_inline)) {
+      constexpr int n = decltype(n_tag)::value;
+      if constexpr (n >= 0) {
+        f32x4& to = acc.v[n / NJ][n % NJ];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) zero[e] = 0.f;
-
-  auto stage = [&](int t, auto more_tag) __attribute__((always_inline)) {
-    constexpr bool more = decltype(more_tag)::value;  // another stage follows
-    lgkm_wait<0>();
+        for (int e = 0; e < 4; ++e) to[e] = __builtin_fmaf(d[n % 3][e], sc[n % NJ], to[e]);
+        // (pinned here: moved behind the loop's end, the additions would keep the products of a whole stage alive)
+        asm volatile("" : "+v"(to));
+      }
+    };
+    unrolled<NI>([&](auto block) __attribute__((always_inline)) {
+      constexpr int i = decltype(block)::value;
+      lgkm_wait<0>();
+      tie(A[i & 1][0]);
+      tie(A[i & 1][1]);
+      if constexpr (i == 0) {
 #pragma unroll
-    for (int j = 0; j < T::NT; ++j) {
+        for (int j = 0; j < NJ; ++j) {
+          tie(B[j][0]);
+          tie(B[j][1]);
+          sc[j] = qx[0][j] * qw[0];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) tie(B[j][k]);
-      sc[j] = qx[0][j] * qw[0];
+          for (int a = 0; a + 1 < AHEAD; ++a) qx[a][j] = qx[a + 1][j];
+        }
 #pragma unroll
-      for (int a = 0; a + 1 < AHEAD; ++a) qx[a][j] = qx[a + 1][j];
-    }
-#pragma unroll
-    for (int a = 0; a + 1 < AHEAD; ++a) qw[a] = qw[a + 1];
-    // Blocks of 32 features in turn.  The products of one block of 32 x 32 are added to the accumulators behind the matrix
-    // instructions of the next one, so that the additions never wait for their result.
-    f32x16 d[2];
-#pragma unroll
-    for (int i = 0; i < T::MT; ++i) {
-      if (i > 0) lgkm_wait<0>();
-#pragma unroll
-      for (int k = 0; k < 4; ++k) tie(A[i & 1][k]);
-      const bool last = i + 1 == T::MT;
-      if (!last) {
-        if (i == 0) read_a(m1, A[1]);
-        else if (i == 1) read_a(m2, A[0]);
-        else read_a(m3, A[1]);
-      } else if (more) {
+        for (int a = 0; a + 1 < AHEAD; ++a) qw[a] = qw[a + 1];
+      }
+      if constexpr (i + 1 == NI) {
         // the stage has been read by this wave; behind the barrier by all, and the next one has landed
-        if (T::ST > 2 && t + T::ST - 1 < steps) vm_wait<(T::ST - 2) * COPIES>();
-        else vm_wait<0>();
+        vm_wait<(T::ST - 2) * COPIES>();
         wg_barrier();
         fetch(t + AHEAD, qx[AHEAD - 1], qw[AHEAD - 1]);
-        if (t + T::ST < steps) issue(t + T::ST, lds_base + cur);
+        old = cur;
         cur = cur == (T::ST - 1) * T::STAGE ? 0u : cur + T::STAGE;
-        if constexpr (T::MT % 2 == 0) read_a(c0, A[0]);
       }
+      unrolled<NJ>([&](auto row) __attribute__((always_inline)) {
+        constexpr int j = decltype(row)::value, n = i * NJ + j;
+        __builtin_amdgcn_sched_barrier(0);
+        d[n % 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(whole(A[i & 1]), whole(B[j]), zero, 0, 0, 0, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        // (behind the last stage: reads of whatever the buffer holds, which nothing uses)
+        if constexpr (j == 0) fa.template read<(i + 1) % NI>(A[(i + 1) & 1], cur);
+        if constexpr (i + 1 == NI) fb_.template read<j>(B[j], cur);
+        unrolled<COPIES>([&](auto copy) __attribute__((always_inline)) {
+          constexpr int c = decltype(copy)::value;
+          if constexpr (c < HALF && i + 1 == NI && c * NJ / HALF == j) issue(t + T::ST, lds_base + old, copy);
+          if constexpr (c >= HALF && i == 0 && (c - HALF) * NJ / (COPIES - HALF) == j) issue(t + T::ST - 1, lds_base + old, copy);
+        });
+        add(std::integral_constant<int, n - 2>{});
+      });
+    });
+    add(std::integral_constant<int, NI * NJ - 2>{});
+    add(std::integral_constant<int, NI * NJ - 1>{});
+  } while (++t < steps);
+  lgkm_wait<0>();
+  tie(A[0][0]);
+  tie(A[0][1]);
 #pragma unroll
-      for (int j = 0; j < T::NT; ++j) {
-        const int n = i * T::NT + j, q = n - 1;
-        auto add = [&](int e0) __attribute__((always_inline)) {
-          if (n > 0)
-#pragma unroll
-            for (int e = e0; e < e0 + 8; ++e)
-              acc[q / T::NT][q % T::NT][e] = __builtin_fmaf(d[q & 1][e], sc[q % T::NT], acc[q / T::NT][q % T::NT][e]);
-          // (pinned here: moved behind the next branch, the additions would keep the products of a whole stage alive)
-          if (n > 0 && e0 == 8) asm volatile("" : "+v"(acc[q / T::NT][q % T::NT]));
-        };
-        __builtin_amdgcn_sched_barrier(0);
-        d[n & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(A[i & 1][0], A[i & 1][1]), pair(B[j][0], B[j][1]), zero,
-                                                                   0, 0, 0, 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        add(0);
-        __builtin_amdgcn_sched_barrier(0);
-        d[n & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pair(A[i & 1][2], A[i & 1][3]), pair(B[j][2], B[j][3]),
-                                                                   d[n & 1], 0, 0, 0, 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (last && more) {
-          if (j == 0) read_b(c0, B[0]);
-          else read_b(n1, B[1]);
-        }
-        add(8);
-      }
-      if (last && more) {
-        if constexpr (T::MT % 2 != 0) read_a(c0, A[0]);
-      }
-    }
-    constexpr int q = T::MT * T::NT - 1;
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      acc[q / T::NT][q % T::NT][e] = __builtin_fmaf(d[q & 1][e], sc[q % T::NT], acc[q / T::NT][q % T::NT][e]);
-  };
-  for (int t = 0; t < steps - 1; ++t) stage(t, std::true_type{});
-  stage(steps - 1, std::false_type{});
+  for (int j = 0; j < NJ; ++j) {
+    tie(B[j][0]);
+    tie(B[j][1]);
+  }
+  vm_wait<0>();
 
-  store_tile<T>(
-      lds,
-      [&](auto&& put) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < T::NT; ++j)
-#pragma unroll
-          for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              put((wn * T::NT + j) * 32 + l32, (wm * T::MT + i) * 32 + 8 * q + 4 * (lane >> 5),
-                  make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])));
-      },
-      p.out + r0 * p.o_stride + f0, p.o_stride, p.M - r0, p.N - f0);
+  store_acc<T>(lds, acc, [](float a, float b) __attribute__((always_inline)) { return pack_bf16x2(a, b); }, p.out + r0 * p.o_stride + f0,
+               p.o_stride, p.M - r0, p.N - f0);
 }
 
 // (a function of its own: the host compiler cannot emit a kernel whose lambda holds a buffer descriptor)

@@ -81,18 +81,6 @@ struct LoadKC {
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (long)(R * I) * stride, left > 0 ? left : 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * I), 16, o, 0, 0, 0);
   }
-  __device__ __forceinline__ void issue(int t, unsigned dst) const {
-    const unsigned k = (unsigned)KB * t;
-    unsigned o[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) o[q] = k + kc[q] < kbytes ? off[q] + k : kOutOfRange;
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int left = bytes - (int)(R * i * stride);
-      const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (long)(R * i) * stride, left > 0 ? left : 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, o[i & 1], 0, 0, 0);
-    }
-  }
 };
 
 // Rows of k-contiguous data at a 64-bit address per row (rows gathered from two tensors).  Rows past the end repeat a
@@ -116,16 +104,6 @@ struct LoadRows {
     const unsigned k = (unsigned)KB * t;
     const unsigned o = k + kc[I & 1] < kbytes ? k + kc[I & 1] : 0u;
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[I] + o), lds_at(dst + 1024 * I), 16, 0, 0);
-  }
-  __device__ __forceinline__ void issue(int t, unsigned dst) const {
-    const unsigned k = (unsigned)KB * t;
-    unsigned o[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) o[q] = k + kc[q] < kbytes ? k + kc[q] : 0u;
-#pragma unroll
-    for (int i = 0; i < L; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p[i] + o[i & 1]),
-                                       lds_at(dst + 1024 * i), 16, 0, 0);
   }
 };
 
@@ -157,15 +135,6 @@ struct LoadKS {
     const unsigned rows = left <= 0 ? 0u : (left < ROWS ? (unsigned)left : (unsigned)ROWS);
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + r0 * stride, rows ? (rows - 1) * (unsigned)stride + colb : 0u);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * I), 16, off[I], 0, 0, 0);
-  }
-  __device__ __forceinline__ void issue(int t, unsigned dst) const {
-    const long r0 = (long)ROWS * t;
-    const long left = k_rows - r0;
-    const unsigned rows = left <= 0 ? 0u : (left < ROWS ? (unsigned)left : (unsigned)ROWS);
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(base + r0 * stride, rows ? (rows - 1) * (unsigned)stride + colb : 0u);
-#pragma unroll
-    for (int i = 0; i < L; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(dst + 1024 * i), 16, off[i], 0, 0, 0);
   }
 };
 
