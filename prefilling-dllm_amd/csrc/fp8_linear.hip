@@ -302,7 +302,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void fp8_linear_kernel(const Fp8Para
 }
 
 // Up to 32 rows: the weight is read once, straight into registers, and the call waits for memory.  A workgroup takes FT = 16 or
-// 32 features and all rows; its eight waves take every eighth block of k, so that all of the workgroup's weight (FT x K
+// 32 features and all rows (more rows: 32 of them); its eight waves take every eighth block of k, so that all of the workgroup's weight (FT x K
 // bytes) is on its way at once, and their fp32 sums meet in LDS, added in wave order.  16x16x128 instruction: lane l holds row
 // l & 15 of an operand, bytes 16 (l >> 4) .. + 15 of each half of the block (any order of k that both operands share).
 template <int FT, int TT, bool BF>
@@ -313,9 +313,10 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long f0 = (long)blockIdx.x * FT;
   const long nf = p.N - f0 < FT ? p.N - f0 : FT;
-  const int m = (int)p.M;
+  const long r0 = 16L * TT * blockIdx.y;  // first row of the workgroup's
+  const int m = p.M - r0 < 16 * TT ? (int)(p.M - r0) : 16 * TT;
   const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.w + f0 * p.w_stride, (unsigned)((nf - 1) * p.w_stride) + (unsigned)p.K);
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, (unsigned)((m - 1) * p.x_stride) + (unsigned)(BF ? 2 * p.K : p.K));
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x + r0 * p.x_stride, (unsigned)((m - 1) * p.x_stride) + (unsigned)(BF ? 2 * p.K : p.K));
   unsigned wo[NF], xo[TT], so[TT];
 #pragma unroll
   for (int f = 0; f < NF; ++f) wo[f] = f * 16 + l16 < nf ? (unsigned)(f * 16 + l16) * (unsigned)p.w_stride : kOutOfRange;
@@ -326,6 +327,7 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
     so[t] = (unsigned)(row < m ? row : m - 1) * (unsigned)p.sx_row;
   }
   const float* sw = p.sw + f0 / 128 * p.sw_row;
+  const float* sx = BF ? nullptr : p.sx + r0 * p.sx_row;
   f32x4 acc[NF][TT];
 #pragma unroll
   for (int f = 0; f < NF; ++f)
@@ -388,7 +390,7 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
           s[u][t] = kb < blocks ? s[u][t] * ws : 0.f;
         } else {
           x[u][t] = load(xr, xo[t], kb);
-          s[u][t] = kb < blocks ? (p.sx + ks * p.sx_blk)[so[t]] * ws : 0.f;
+          s[u][t] = kb < blocks ? (sx + ks * p.sx_blk)[so[t]] * ws : 0.f;
         }
       }
     }
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
     float v = part[0][row][f];
 #pragma unroll
     for (int q = 1; q < 8; ++q) v += part[q][row][f];
-    p.out[row * p.o_stride + f0 + f] = (__bf16)v;
+    p.out[(r0 + row) * p.o_stride + f0 + f] = (__bf16)v;
   }
 }
 
@@ -601,6 +603,23 @@ int launch_resident(Fp8Params& p, hipStream_t s) {
   return launch_status();
 }
 
+// 32 features to a workgroup of the streaming kernel read the rows half as often; 16 where 32 would leave compute units idle
+bool stream_wide(const Fp8Params& p) { return (p.N + 31) / 32 * ((p.M + 31) / 32) >= 512; }
+
+template <bool BF>
+int launch_stream(Fp8Params& p, hipStream_t s) {
+  const bool wide = stream_wide(p);
+  const dim3 grid((unsigned)((p.N + (wide ? 31 : 15)) / (wide ? 32 : 16)), (unsigned)((p.M + 31) / 32));
+  if (p.M <= 16) {
+    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 1, BF>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fp8_stream_kernel<16, 1, BF>), grid, dim3(512), 0, s, p);
+  } else {
+    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 2, BF>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fp8_stream_kernel<16, 2, BF>), grid, dim3(512), 0, s, p);
+  }
+  return launch_status();
+}
+
 // up to 32 rows
 template <bool BF>
 int launch_few(Fp8Params& p, hipStream_t s) {
@@ -610,17 +629,7 @@ int launch_few(Fp8Params& p, hipStream_t s) {
     if (p.M <= 16 && resident_lds<16>(blocks, groups) <= 160 * 1024) return launch_resident<1, BF>(p, s);
     if (p.M > 16 && resident_lds<32>(blocks, groups) <= 160 * 1024) return launch_resident<2, BF>(p, s);
   }
-  // 32 features to a workgroup read the rows half as often; 16 where 32 would leave compute units idle
-  const bool wide = (p.N + 31) / 32 >= 512;
-  const unsigned grid = (unsigned)((p.N + (wide ? 31 : 15)) / (wide ? 32 : 16));
-  if (p.M <= 16) {
-    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 1, BF>), dim3(grid), dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fp8_stream_kernel<16, 1, BF>), dim3(grid), dim3(512), 0, s, p);
-  } else {
-    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 2, BF>), dim3(grid), dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fp8_stream_kernel<16, 2, BF>), dim3(grid), dim3(512), 0, s, p);
-  }
-  return launch_status();
+  return launch_stream<BF>(p, s);
 }
 
 int launch_many(Fp8Params& p, hipStream_t s) {
@@ -628,6 +637,13 @@ int launch_many(Fp8Params& p, hipStream_t s) {
   const auto tiles = [&](long tm, long tn) { return ((p.N + tm - 1) / tm) * ((p.M + tn - 1) / tn); };
   if (p.M > 128 && tiles(256, 256) >= 160) return launch_fp8<TileL>(p, s);
   if (p.M > 64 && tiles(256, 128) >= 160) return launch_fp8<TileM>(p, s);
+  // Few tiles of a long k wait for one stage after the other, 0.4 us each behind a start and end of 3 us; the streaming kernel, 32
+  // rows at a time, has all of k on its way at once, but reads rows and features once per workgroup, at 9 TB/s out of L2.
+  // (us by tiles and streamed: 59 rows x 280 x 8304 28.8 and 10.2, 64 x 4096 x 4096 16.2 and 13.6, 333 x 2201 x 1168 10.7 and 7.7;
+  // 1398 x 304 x 4688 18.8 and 21.6, 155 x 7585 x 8176 38 and 61)
+  const long f = stream_wide(p) ? 32 : 16;
+  const double read = (double)((p.M + 31) / 32 * ((p.N + f - 1) / f)) * (32 + f) * p.K;
+  if (read < 9e6 * (3 + 0.4 * ((p.K + 127) / 128))) return launch_stream<false>(p, s);
   return launch_fp8<TileS2>(p, s);
 }
 

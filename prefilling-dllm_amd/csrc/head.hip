@@ -650,9 +650,13 @@ using TileS = Tile<1, 1, 4, 1, 4>;   // 128 x 32
 constexpr long kMaxRows = 1L << 24;
 constexpr long kMaxVocab = 1L << 30;
 
+// Up to 32 tiles of 256 x 256: eight times as many of 128 x 64, for which the idle compute units have room (1024 rows x 2048
+// entries x 3584: 37 us in 32 tiles, 31 in 256; x 4096 entries: 41 in 64, 42.5 in 512)
+bool small_tiles(long n, long v) { return n <= 64 || ((v + 255) / 256) * ((n + 255) / 256) <= 32; }
+
 // parts of a row in the workspace: the vocabulary tiles
 int stat_parts(long n, long v) {
-  const int tm = n <= 64 ? TileS::TM : TileL::TM;
+  const int tm = small_tiles(n, v) ? TileS::TM : TileL::TM;
   static_assert(TileS::TM == TileS2::TM && TileM::TM == TileL::TM, "two heights of tiles");
   return (int)((v + tm - 1) / tm);
 }
@@ -707,7 +711,7 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
   if (un.block_ids) p.joined = un.joined = p.part_idx + (long)parts * p.N;
   int st;
   if (p.N <= 32) st = launch_stats<TileS, TileS, CONF>(p, s);
-  else if (p.N <= 64) st = launch_stats<TileS2, TileS2, CONF>(p, s);
+  else if (small_tiles(p.N, p.V)) st = launch_stats<TileS2, TileS2, CONF>(p, s);
   else if (p.N <= 128 && p.V >= 32768) st = launch_stats<TileM, TileR, CONF>(p, s);
   else st = launch_stats<TileL, TileR, CONF>(p, s);
   if (st != PDLLM_OK) return st;
@@ -939,8 +943,10 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     const long vp = vocab - v0 < g.vp ? vocab - v0 : g.vp;
     p.v0 = v0;
     p.hz = v0 == 0 ? ws : nullptr;
-    p.n_voc_tiles = (int)((vp + (few ? TileS2::TM : TileL::TM) - 1) / (few ? TileS2::TM : TileL::TM));
-    st = few ? launch_dlogits<TileS2, TileS2, true>(p, s) : launch_dlogits<TileL, TileR, false>(p, s);
+    const int tm = small_tiles(n_rows, vp) ? TileS2::TM : TileL::TM;
+    p.n_voc_tiles = (int)((vp + tm - 1) / tm);
+    st = few ? launch_dlogits<TileS2, TileS2, true>(p, s)
+         : tm == TileS2::TM ? launch_dlogits<TileS2, TileS2, false>(p, s) : launch_dlogits<TileL, TileR, false>(p, s);
     if (st != PDLLM_OK) return st;
     q.w = p.w + v0 * p.w_stride;
     q.vp = vp;

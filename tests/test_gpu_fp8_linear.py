@@ -54,7 +54,9 @@ def operands(dev, m, n, k, seed=0):
                                    (17, 40, 18944), (2, 20001, 64),
                                    # up to 32 rows: kept in shared memory beside many features, or streamed with them
                                    (5, 16400, 1040), (17, 20001, 1168), (32, 16385, 2064), (4, 16384, 1024), (9, 16384, 896),
-                                   (20, 8200, 272)])
+                                   (20, 8200, 272),
+                                   # few tiles of a long k, streamed 32 rows at a time: ragged rows and features, either width
+                                   (59, 280, 8304), (97, 1003, 2048), (65, 8400, 144), (130, 17, 4112)])
 def test_linear(dev, m, n, k):
     from prefilling_dllm_amd import ops
     x, wq, ws = operands(dev, m, n, k, seed=m + n + k)

@@ -74,7 +74,9 @@ def check_grad(gh, gw, h, w, d):
 SHAPES = [(1, 1, 8), (1, 300, 64), (5, 1000, 520), (31, 127, 72), (32, 129, 64), (33, 2570, 136), (64, 3000, 256),
           (65, 257, 8), (128, 1025, 1032), (129, 3001, 512), (300, 2571, 136), (1030, 700, 200), (2, 40000, 64),
           # one piece of few entries (no sum of partial results), just more than that, the last row of the small tiles
-          (20, 1024, 520), (20, 1030, 520), (256, 2000, 264), (257, 2001, 264), (200, 20000, 72)]
+          (20, 1024, 520), (20, 1030, 520), (256, 2000, 264), (257, 2001, 264), (200, 20000, 72),
+          # just more than 32 tiles of 256 x 256
+          (1025, 1700, 72)]
 
 
 @pytest.mark.parametrize("n,v,d", SHAPES)
