@@ -986,8 +986,8 @@ def _head_args(hidden: torch.Tensor, weight: torch.Tensor) -> Tuple[int, int, in
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    """The row stride of a 2-D tensor (a single row may carry any stride)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    """The row stride of a 2-D tensor (that of a single row, which may be anything, is not used)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _head_rows(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, device) -> torch.Tensor:

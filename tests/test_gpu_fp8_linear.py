@@ -126,12 +126,17 @@ def test_strides_and_out(dev):
     rows = torch.full((m + 10, n), 7.0, dtype=torch.bfloat16, device=dev)
     ops.fp8_block_linear(x, wq, ws, out=rows[:m])
     assert bool((rows[m:] == 7).all())
+    # a single row of a tensor whose rows begin anywhere
+    odd = torch.zeros(2 * 403, dtype=torch.bfloat16, device=dev)[:403 * 2].view(2, 403)[:1, :400]
+    odd.copy_(x[:1])
+    assert torch.equal(ops.fp8_block_linear(odd, wq, ws, out=buf[:1, 3:3 + n]), ops.fp8_block_linear(x[:1], wq, ws))
 
 
-def test_empty_rows_and_graph(dev):
+@pytest.mark.parametrize("m,n,k", [(40, 300, 256), (9, 17000, 1040), (300, 5000, 400)])
+def test_empty_rows_and_graph(dev, m, n, k):
     from prefilling_dllm_amd import ops
-    x, wq, ws = operands(dev, 40, 300, 256, seed=1)
-    assert ops.fp8_block_linear(x[:0], wq, ws).shape == (0, 300)
+    x, wq, ws = operands(dev, m, n, k, seed=1)
+    assert ops.fp8_block_linear(x[:0], wq, ws).shape == (0, n)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
@@ -141,7 +146,7 @@ def test_empty_rows_and_graph(dev):
     with torch.cuda.graph(graph):
         out = ops.fp8_block_linear(x, wq, ws)
     for seed in (2, 3, 4):
-        x.copy_(operands(dev, 40, 300, 256, seed=seed)[0])
+        x.copy_(operands(dev, m, n, k, seed=seed)[0])
         want = ops.fp8_block_linear(x, wq, ws)
         graph.replay()
         torch.cuda.synchronize()

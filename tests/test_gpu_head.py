@@ -75,8 +75,8 @@ SHAPES = [(1, 1, 8), (1, 300, 64), (5, 1000, 520), (31, 127, 72), (32, 129, 64),
           (65, 257, 8), (128, 1025, 1032), (129, 3001, 512), (300, 2571, 136), (1030, 700, 200), (2, 40000, 64),
           # one piece of few entries (no sum of partial results), just more than that, the last row of the small tiles
           (20, 1024, 520), (20, 1030, 520), (256, 2000, 264), (257, 2001, 264), (200, 20000, 72),
-          # just more than 32 tiles of 256 x 256
-          (1025, 1700, 72)]
+          # just more than 32 tiles of 256 x 256; the large tiles of the gradient, ragged in every direction
+          (1025, 1700, 72), (300, 25001, 264), (257, 50100, 72)]
 
 
 @pytest.mark.parametrize("n,v,d", SHAPES)
@@ -271,12 +271,12 @@ def test_empty_calls(dev):
     assert tr.shape == (0, 8) and left.shape == (0,)
 
 
-def test_graph_replays_against_new_states(dev):
+@pytest.mark.parametrize("n,v,d", [(96, 3000, 256), (32, 3000, 72), (320, 25000, 264)])
+def test_graph_replays_against_new_states(dev, n, v, d):
     """Logp, gradient and denoise step of one capture, replayed with new states and eager work in between."""
     from prefilling_dllm_amd import ops
-    n, v, d = 96, 3000, 256
     h, w, labels, g = make(dev, n, v, d, seed=1)
-    ids0 = torch.full((3, 32), 7, dtype=torch.int64, device=dev)
+    ids0 = torch.full((n // 32, 32), 7, dtype=torch.int64, device=dev)
 
     def step(ids):
         logp, lse = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
@@ -319,6 +319,27 @@ def test_another_stream_gives_the_same(dev):
     for o in outs:
         for x, y in zip(a + ga, o):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n,v,d", [(20, 1100, 264), (100, 1100, 264), (300, 25000, 264), (20, 300, 72)])
+def test_gradients_with_strides_of_their_own(dev, n, v, d):
+    """The C entry with gradients whose rows begin at multiples of 8 bytes only: the same values, nothing written beside them."""
+    from prefilling_dllm_amd import _lib, ops
+    h, w, labels, g = make(dev, n, v, d, seed=n)
+    logp, lse = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
+    want = ops.head_selfinfo_grad(h, w, labels, logp, lse, g)
+    gh = torch.full((n + 2, d + 4), 7.0, dtype=torch.bfloat16, device=dev)
+    gw = torch.full((v + 2, d + 12), 7.0, dtype=torch.bfloat16, device=dev)
+    need = int(_lib.lib.pdllm_head_selfinfo_grad_workspace_bytes(n, v, d))
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device=dev)     # (what it held before, NaN here, does not matter)
+    st = _lib.lib.pdllm_head_selfinfo_grad(
+        h.data_ptr(), d, w.data_ptr(), d, labels.data_ptr(), logp.data_ptr(), lse.data_ptr(), g.data_ptr(), n, v, d,
+        ws.data_ptr(), need, gh[1:, 4:].data_ptr(), d + 4, gw[1:, 4:].data_ptr(), d + 12, torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    assert torch.equal(gh[1:n + 1, 4:4 + d], want[0]) and torch.equal(gw[1:v + 1, 4:4 + d], want[1])
+    gh[1:n + 1, 4:4 + d] = 7
+    gw[1:v + 1, 4:4 + d] = 7
+    assert bool((gh == 7).all()) and bool((gw == 7).all()) and bool((ws[need:] == 255).all())
 
 
 def test_head_scores_rank_chunks_like_the_logits(dev):
