@@ -489,9 +489,9 @@ int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_scale, int6
                      int64_t weight_scale_row_stride, int64_t weight_scale_block_stride, int64_t m, int64_t n, int32_t k,
                      void* out, int64_t out_stride, pdllm_stream_t stream);
 
-/* The same product from bf16 x [m, k] (x_stride a multiple of 8, below 2^22), quantised as pdllm_fp8_quantize_rows does: up to 32
- * rows where they are read, in one launch and without a workspace, more of them into the workspace first.  Same bits as the
- * two calls.  workspace: 16-byte aligned. */
+/* The same product from bf16 x [m, k] (x_stride a multiple of 8, below 2^22), quantised as pdllm_fp8_quantize_rows does: up to 16
+ * rows where they are read, in one launch and without a workspace, more of them (beside many features: more than 32) into the
+ * workspace first.  Same bits as the two calls.  workspace: 16-byte aligned. */
 int64_t pdllm_fp8_linear_bf16_workspace_bytes(int64_t m, int32_t k);
 int pdllm_fp8_linear_bf16(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                           const float* weight_scale, int64_t weight_scale_row_stride, int64_t weight_scale_block_stride,

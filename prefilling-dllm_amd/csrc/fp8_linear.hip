@@ -307,7 +307,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void fp8_linear_kernel(const Fp8Para
 // l & 15 of an operand, bytes 16 (l >> 4) .. + 15 of each half of the block (any order of k that both operands share).
 template <int FT, int TT, bool BF>
 __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
-  constexpr int NF = FT / 16, U = BF && TT == 2 ? 1 : 2;  // U blocks of a wave in flight (as many as the registers hold)
+  constexpr int NF = FT / 16, U = 2;  // U blocks of a wave in flight
   __shared__ float part[8][TT * 16][FT + 1];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -606,30 +606,33 @@ int launch_resident(Fp8Params& p, hipStream_t s) {
 // 32 features to a workgroup of the streaming kernel read the rows half as often; 16 where 32 would leave compute units idle
 bool stream_wide(const Fp8Params& p) { return (p.N + 31) / 32 * ((p.M + 31) / 32) >= 512; }
 
-template <bool BF>
+template <int TT, bool BF>
 int launch_stream(Fp8Params& p, hipStream_t s) {
   const bool wide = stream_wide(p);
-  const dim3 grid((unsigned)((p.N + (wide ? 31 : 15)) / (wide ? 32 : 16)), (unsigned)((p.M + 31) / 32));
-  if (p.M <= 16) {
-    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 1, BF>), grid, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fp8_stream_kernel<16, 1, BF>), grid, dim3(512), 0, s, p);
-  } else {
-    if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, 2, BF>), grid, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fp8_stream_kernel<16, 2, BF>), grid, dim3(512), 0, s, p);
-  }
+  const dim3 grid((unsigned)((p.N + (wide ? 31 : 15)) / (wide ? 32 : 16)), (unsigned)((p.M + 16 * TT - 1) / (16 * TT)));
+  if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, TT, BF>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((fp8_stream_kernel<16, TT, BF>), grid, dim3(512), 0, s, p);
   return launch_status();
+}
+
+// Up to 32 rows beside many features: the rows stay in LDS where they fit (K = 3584, 152064 features, us streamed and resident: e4m3
+// rows 88 and 90 for 1, 97 and 96 for 8, 110 and 99 for 16, 141 and 107 for 32; bf16 rows, which every streaming workgroup
+// quantises again, 122 and 92 for 1, 161 and 102 for 16, 229 and 112 for 32.  16384 features x 4096: 14.8 and 15.8 for 1 row, 16.3
+// and 16.1 for 16; 12288 x 2048: 10.8 and 9.7 for 32 rows, 8.2 and 9.2 for 16).
+bool resident_fits(const Fp8Params& p, bool bf) {
+  const long blocks = (p.K + 127) / 128, groups = ((p.N + 31) / 32 + 255) / 256;
+  if (blocks < kResidentQ || p.M > 32) return false;
+  if (p.M > 16) return p.N >= 12288 && resident_lds<32>(blocks, groups) <= 160 * 1024;
+  return p.N >= 16384 && (bf || p.M > 4) && resident_lds<16>(blocks, groups) <= 160 * 1024;
 }
 
 // up to 32 rows
 template <bool BF>
 int launch_few(Fp8Params& p, hipStream_t s) {
-  const long blocks = (p.K + 127) / 128, groups = ((p.N + 31) / 32 + 255) / 256;
-  // (measured, K = 3584, 152064 features: 1 row 91 us resident, 88 us streamed; 16 rows 100 and 110; 32 rows 107 and 140)
-  if (p.M > 4 && p.N >= 16384 && blocks >= kResidentQ) {
-    if (p.M <= 16 && resident_lds<16>(blocks, groups) <= 160 * 1024) return launch_resident<1, BF>(p, s);
-    if (p.M > 16 && resident_lds<32>(blocks, groups) <= 160 * 1024) return launch_resident<2, BF>(p, s);
-  }
-  return launch_stream<BF>(p, s);
+  if (resident_fits(p, BF)) return p.M <= 16 ? launch_resident<1, BF>(p, s) : launch_resident<2, BF>(p, s);
+  if constexpr (!BF)
+    if (p.M > 16) return launch_stream<2, false>(p, s);
+  return launch_stream<1, BF>(p, s);
 }
 
 int launch_many(Fp8Params& p, hipStream_t s) {
@@ -643,11 +646,12 @@ int launch_many(Fp8Params& p, hipStream_t s) {
   // 1398 x 304 x 4688 18.8 and 21.6, 155 x 7585 x 8176 38 and 61)
   const long f = stream_wide(p) ? 32 : 16;
   const double read = (double)((p.M + 31) / 32 * ((p.N + f - 1) / f)) * (32 + f) * p.K;
-  if (read < 9e6 * (3 + 0.4 * ((p.K + 127) / 128))) return launch_stream<false>(p, s);
+  if (read < 9e6 * (3 + 0.4 * ((p.K + 127) / 128))) return launch_stream<2, false>(p, s);
   return launch_fp8<TileS2>(p, s);
 }
 
 constexpr int kFewRows = 32;
+constexpr int kFewBf16Rows = 16;  // streamed as they are (20.6 us for 32 rows x 2048 x 8192, where a launch that quantises them and the product take 17)
 
 int check_quantize(const void* x, int64_t x_stride, int64_t rows, int32_t K, const void* q, int64_t q_stride, const void* scale,
                    int64_t s_row, int64_t s_blk) {
@@ -751,7 +755,7 @@ extern "C" int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_
 
 extern "C" int64_t pdllm_fp8_linear_bf16_workspace_bytes(int64_t m, int32_t k) {
   if (check_linear(m, 1, k) != PDLLM_OK) return PDLLM_ERR_SHAPE;
-  return m <= kFewRows ? 0 : m * k + 4 * m * ((k + 127) / 128);
+  return m <= kFewBf16Rows ? 0 : m * k + 4 * m * ((k + 127) / 128);
 }
 
 extern "C" int pdllm_fp8_linear_bf16(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
@@ -767,8 +771,9 @@ extern "C" int pdllm_fp8_linear_bf16(const void* x, int64_t x_stride, const void
   Fp8Params p = linear_params(x, 2 * x_stride, weight, weight_stride, weight_scale, weight_scale_row_stride,
                               weight_scale_block_stride, m, n, k, out, out_stride);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (m <= kFewRows) return launch_few<true>(p, s);  // quantised where they are read: one launch
-  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < pdllm_fp8_linear_bf16_workspace_bytes(m, k)) return PDLLM_ERR_WORKSPACE;
+  if (m > kFewBf16Rows && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < pdllm_fp8_linear_bf16_workspace_bytes(m, k)))
+    return PDLLM_ERR_WORKSPACE;
+  if (m <= kFewBf16Rows || resident_fits(p, true)) return launch_few<true>(p, s);  // quantised where they are read: one launch
   char* q = static_cast<char*>(workspace);
   float* scale = reinterpret_cast<float*>(q + m * k);
   st = pdllm_fp8_quantize_rows(x, x_stride, m, k, q, k, scale, 1, m, stream);
@@ -778,5 +783,5 @@ extern "C" int pdllm_fp8_linear_bf16(const void* x, int64_t x_stride, const void
   p.sx = scale;
   p.sx_row = 1;
   p.sx_blk = m;
-  return launch_many(p, s);
+  return m <= kFewRows ? launch_few<false>(p, s) : launch_many(p, s);
 }

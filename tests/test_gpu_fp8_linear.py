@@ -53,7 +53,7 @@ def operands(dev, m, n, k, seed=0):
                                    (65, 2201, 400), (128, 256, 2048), (129, 513, 1024), (333, 2201, 1168), (600, 130, 5120),
                                    (17, 40, 18944), (2, 20001, 64),
                                    # up to 32 rows: kept in shared memory beside many features, or streamed with them
-                                   (5, 16400, 1040), (17, 20001, 1168), (32, 16385, 2064), (4, 16384, 1024), (9, 16384, 896),
+                                   (5, 16400, 1040), (17, 20001, 1168), (32, 16385, 2064), (4, 16384, 1024), (9, 16384, 896), (1, 16390, 1040), (18, 12300, 1040), (16, 4100, 2064), (17, 4100, 2064),
                                    (20, 8200, 272),
                                    # few tiles of a long k, streamed 32 rows at a time: ragged rows and features, either width
                                    (59, 280, 8304), (97, 1003, 2048), (65, 8400, 144), (130, 17, 4112)])

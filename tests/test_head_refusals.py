@@ -95,7 +95,7 @@ def test_fp8_sizes_and_pointers(lib, p):
         assert call(**kw) == st, kw
     g = lib.pdllm_fp8_linear_bf16
     need = lib.pdllm_fp8_linear_bf16_workspace_bytes(40, 64)
-    assert need == 40 * 64 + 4 * 40 and lib.pdllm_fp8_linear_bf16_workspace_bytes(32, 64) == 0
+    assert need == 40 * 64 + 4 * 40 and lib.pdllm_fp8_linear_bf16_workspace_bytes(16, 64) == 0
     for bad in ((-1, 64), (4, 0), (4, 40), (4, (1 << 20) + 16), ((1 << 24) + 1, 64)):
         assert lib.pdllm_fp8_linear_bf16_workspace_bytes(*bad) == -2
     ok.update(m=40, ws_p=p, ws_n=need)
