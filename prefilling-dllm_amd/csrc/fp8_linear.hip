@@ -2,9 +2,10 @@
 //
 //   y[m, n] = sum over blocks kb of  sx[m, kb] * sw[n / 128, kb] * sum over k in kb of xq[m, k] * wq[n, k]
 //
-// One pass of 128 bytes of k is one block: its product is formed by the 32x32x64 matrix instruction from zero and added to
+// One pass of 128 bytes of k is one block: its product is formed by one 16x16x128 matrix instruction from zero and added to
 // the fp32 accumulators with its scale.  A lane owns one row m of the result, so the scale is one number per lane, column
-// of tiles and block.
+// of tiles and block.  (From registers, with normally distributed values, 16x16x128 sustains 4430 TFLOP/s at the card's power limit,
+// 32x32x64 4020.)
 //
 // Precision.  The instruction multiplies exactly and adds eight products at a time on a grid of 2^-13 of the largest of
 // them (measured: beside a product of 2^16 one of 2^3 counts in full, one of 2^2 not at all), then adds the groups in
@@ -56,7 +57,7 @@ __device__ __forceinline__ uint2 to_e4m3(const uint4& v, float inv) {
 }
 
 // One scale for each row and 128 columns; 16 lanes to a block, 16 blocks of a row to a workgroup.  HBM-bound: 2 bytes read and 1
-// written per value.
+// written per value (8200 x 3584: 18 us, 4.9 TB/s).
 __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const char* __restrict__ x, long x_stride, int groups, int K,
                                                                 char* __restrict__ q, long q_stride, float* __restrict__ scale,
                                                                 long s_row, long s_blk) {
@@ -147,6 +148,10 @@ struct Frag8 {
   }
 };
 
+// A tile of T::TM features x T::TN rows; bound by the matrix instructions and, for the largest products, the card's power.  The
+// tile's whole stage of B stays in registers, blocks of A pass by; each product waits two instructions before it is added, and reads
+// of the next block, and copies of the stages behind, go between the instructions (8200 rows x 18944 x 3584: 541 us with
+// 32x32x64 instructions, reads and copies in front of them; 489 us so, 2.27 PFLOP/s.  2048 x 8192 x 8192: 109 us, 2.52 PFLOP/s).
 template <class T>
 __device__ __forceinline__ void fp8_tile(const Fp8Params& p, char* lds) {
   const int lane = threadIdx.x & 63, l16 = lane & 15;
@@ -302,9 +307,10 @@ __global__ __launch_bounds__(T::THREADS, 2) void fp8_linear_kernel(const Fp8Para
 }
 
 // Up to 32 rows: the weight is read once, straight into registers, and the call waits for memory.  A workgroup takes FT = 16 or
-// 32 features and all rows (more rows: 32 of them); its eight waves take every eighth block of k, so that all of the workgroup's weight (FT x K
-// bytes) is on its way at once, and their fp32 sums meet in LDS, added in wave order.  16x16x128 instruction: lane l holds row
-// l & 15 of an operand, bytes 16 (l >> 4) .. + 15 of each half of the block (any order of k that both operands share).
+// 32 features and all rows (more rows: 32 of them); its eight waves take every eighth block of k, so that all of the
+// workgroup's weight (FT x K bytes) is on its way at once, and their fp32 sums meet in LDS, added in wave order.  16x16x128
+// instruction: lane l holds row l & 15 of an operand, bytes 16 (l >> 4) .. + 15 of each half of the block (any order of k that
+// both operands share).  1 row x 152064 x 3584: 88 us, 6.2 TB/s; 1 x 4096 x 4096: 4.7 us, of which the weight's 16.8 MB are 3.4.
 template <int FT, int TT, bool BF>
 __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
   constexpr int NF = FT / 16, U = 2;  // U blocks of a wave in flight
@@ -427,7 +433,8 @@ __global__ __launch_bounds__(512, 4) void fp8_stream_kernel(const Fp8Params p) {
 // otherwise be read again for every group of features: twice the weight's bytes, through the same L2), and walks over groups
 // of 32 features.  Wave (q, c) takes blocks q, q + 8, ... of k of the 16 features c of the group, so that the group's rows of the
 // weight, which lie side by side in memory, are asked for together; a ring of U blocks in registers runs on from group to
-// group.  The eight partial sums of a result meet in LDS, added in wave order.
+// group.  The eight partial sums of a result meet in LDS, added in wave order.  32 rows x 152064 x 3584: 107 us, 5.2 TB/s of weight
+// and results.
 // Rows in LDS: block kb of row r, chunk c at ((kb * R + r) * 8 + (c ^ (r >> 1 & 7))) * 16: 16 rows of one chunk cover all banks.
 constexpr int kResidentPad = 33;
 constexpr int kResidentQ = 8;  // waves that share the features' k
@@ -636,10 +643,13 @@ int launch_few(Fp8Params& p, hipStream_t s) {
 }
 
 int launch_many(Fp8Params& p, hipStream_t s) {
-  // The largest tile that still gives most of the 256 compute units one: tiles re-read their operands less the larger they are
+  // Large tiles read their operands less often, small ones leave fewer compute units idle: the fewest rounds, a round of 256 x 256
+  // (256 at a time) counted as 20, of 256 x 128 as 13, of 128 x 64 (512 at a time) as 10.  (us in the three, K = 3584: 600 rows
+  // x 18944 49, 59, 64; 300 rows 44, 31, 42; 129 rows 39, 27, 22; 100 rows x 37888 42, 29, 37; 300 rows x 37888 84, 58, 74)
   const auto tiles = [&](long tm, long tn) { return ((p.N + tm - 1) / tm) * ((p.M + tn - 1) / tn); };
-  if (p.M > 128 && tiles(256, 256) >= 160) return launch_fp8<TileL>(p, s);
-  if (p.M > 64 && tiles(256, 128) >= 160) return launch_fp8<TileM>(p, s);
+  const long l = 20 * ((tiles(256, 256) + 255) / 256), m = 13 * ((tiles(256, 128) + 255) / 256), t = 10 * ((tiles(128, 64) + 511) / 512);
+  if (l <= m && l <= t) return launch_fp8<TileL>(p, s);
+  if (m <= t) return launch_fp8<TileM>(p, s);
   // Few tiles of a long k wait for one stage after the other, 0.4 us each behind a start and end of 3 us; the streaming kernel, 32
   // rows at a time, has all of k on its way at once, but reads rows and features once per workgroup, at 9 TB/s out of L2.
   // (us by tiles and streamed: 59 rows x 280 x 8304 28.8 and 10.2, 64 x 4096 x 4096 16.2 and 13.6, 333 x 2201 x 1168 10.7 and 7.7;
@@ -651,7 +661,8 @@ int launch_many(Fp8Params& p, hipStream_t s) {
 }
 
 constexpr int kFewRows = 32;
-constexpr int kFewBf16Rows = 16;  // streamed as they are (20.6 us for 32 rows x 2048 x 8192, where a launch that quantises them and the product take 17)
+// bf16 rows streamed as they are (32 rows x 2048 x 8192: 20.6 us so, 16.0 with a launch that quantises them first)
+constexpr int kFewBf16Rows = 16;
 
 int check_quantize(const void* x, int64_t x_stride, int64_t rows, int32_t K, const void* q, int64_t q_stride, const void* scale,
                    int64_t s_row, int64_t s_blk) {

@@ -218,6 +218,10 @@ __device__ __forceinline__ void head_dispatch(const HeadParams& p, F&& tile) {
   }
 }
 
+// Bound by the weight's bytes up to 128 rows (152064 x 3584: 182 us for 32 rows, 6.0 TB/s; 214 us for 128, 5.1 TB/s), above by the
+// matrix instructions and the card's power (4096 rows: 3.16 ms, 1.41 PFLOP/s with the statistics; a library product of the same
+// size, which writes its logits, 3.07 ms).  Forming one tile after the other in 256 workgroups, the next tile's copies in flight during
+// the statistics, was no faster (4096 rows 3.31 ms, 1000 rows x 50021 x 1032 116.7 us for 117.4).
 template <class T, class TS, bool CONF>
 __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS > TS::LDS ? T::LDS : TS::LDS];
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2* __restrict
 
 // One piece of the softmax gradient, rounded to bf16 as the operand of the two products behind it (each entry off by at
 // most 2^-8 of itself).  For few rows, where few entries make up a result and the products wait for memory anyway, the
-// remainder of the rounding is kept beside it.
+// remainder of the rounding is kept beside it.  4096 rows x 32768 entries x 3584: 740 us, 1.30 PFLOP/s.
 template <class T, bool FEW>
 __device__ __forceinline__ void head_dlogits_tile(const HeadParams& p, int vt, long row0, char* lds) {
   Acc<T> acc;
@@ -555,6 +559,7 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
 // (many, with the rows to sum over) fill the compute units they leave.
 // The small tiles (80 KB of LDS, at most 128 registers) leave room for two workgroups on a compute unit, which hide each other's
 // start and end: with few rows a tile of grad_w is a few stages and then 32 KB of results.
+// 4096 rows x 32768 entries x 3584: 1454 us, 1.32 PFLOP/s, bound as the statistics are.
 template <class TH, class TW>
 __global__ __launch_bounds__(TW::THREADS, TW::MT * TW::NT <= 2 ? 4 : 2) void head_grad_kernel(const GradParams p) {
   static_assert(TH::THREADS == TW::THREADS, "");
@@ -624,6 +629,8 @@ __device__ __forceinline__ void head_grad_w_few(const GradParams& p, long id) {
 }
 
 // Both products of up to 16 NT rows: tiles of grad_h, 256 columns x all rows and a share of the piece, then the waves of grad_w.
+// Bound by the weight read and its gradient written: 32 rows x 126464 x 4096 485 us, 4.3 TB/s (a copy of 2 GiB reaches 4.9); with
+// tiles of 128 x 128 through LDS for grad_w, two stages and 32 KB of results each, 600 to 710 us.
 template <int NT>
 __global__ __launch_bounds__(512, 4) void head_grad_few_kernel(const GradParams p) {
   typedef Tile<1, NT, 8, 1, 2> T;
@@ -650,9 +657,9 @@ using TileS = Tile<1, 1, 4, 1, 4>;   // 128 x 32
 constexpr long kMaxRows = 1L << 24;
 constexpr long kMaxVocab = 1L << 30;
 
-// Up to 32 tiles of 256 x 256: eight times as many of 128 x 64, for which the idle compute units have room (1024 rows x 2048
-// entries x 3584: 37 us in 32 tiles, 31 in 256; x 4096 entries: 41 in 64, 42.5 in 512)
-bool small_tiles(long n, long v) { return n <= 64 || ((v + 255) / 256) * ((n + 255) / 256) <= 32; }
+// Tiles of 128 x 64 where they are at most one round, two to a compute unit (us in tiles of 256 x 256 and so: 150 rows x 20000 x 3584
+// 72 and 41, 100 x 16000 x 4096 42 and 36, 407 x 448 x 3096 33 and 27, 1024 x 4096 x 3584 44 and 43, 300 x 9000 x 2048 27 and 29)
+bool small_tiles(long n, long v) { return n <= 64 || ((v + 127) / 128) * ((n + 63) / 64) <= 512; }
 
 // parts of a row in the workspace: the vocabulary tiles
 int stat_parts(long n, long v) {
@@ -663,9 +670,9 @@ int stat_parts(long n, long v) {
 
 int64_t stats_ws(long n, long v, bool conf) { return (int64_t)stat_parts(n, v) * n * (conf ? 12 : 8) + (conf ? 4 : 4 * n); }
 
-// The grid over n_voc_tiles x N rows: whole tiles of T, pieces of TS where fewer than 96 tiles would be the last round of the
-// 256 compute units (their four pieces take about half a tile's time each: 784 tiles of 1000 rows x 50021 entries were four rounds,
-// 148 us, and are three and a half), and for up to 128 rows behind the last whole column.
+// The grid over n_voc_tiles x N rows: whole tiles of T; pieces of TS where an almost empty last round of the 256 compute units becomes
+// one round of them (784 tiles of 1000 rows x 50021 entries x 3584: 335 us in four rounds, 297 in three and one of pieces; x 1032 127
+// and 114; 594 tiles of 128 rows x 152064 x 3584: 222 and 215), and for up to 128 rows behind the last whole column.
 template <class T, class TS>
 long head_grid(HeadParams& p) {
   constexpr int Q = T::TN / TS::TN;
@@ -674,7 +681,7 @@ long head_grid(HeadParams& p) {
   p.n_tok_tiles = (int)(p.N / T::TN + (rest > 0 && !cut_rest));
   p.rest_cols = cut_rest ? (int)((rest + TS::TN - 1) / TS::TN) : 0;
   const long whole = (long)p.n_voc_tiles * p.n_tok_tiles, last = whole % 256;
-  const long full = Q > 1 && last <= 96 ? whole - last : whole;
+  const long full = Q > 1 && Q * last <= 256 ? whole - last : whole;
   const long grid = full + Q * (whole - full) + (long)p.n_voc_tiles * p.rest_cols;
   p.n_full = (int)full;
   p.n_cut = (int)(Q * (whole - full));
@@ -712,7 +719,7 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
   int st;
   if (p.N <= 32) st = launch_stats<TileS, TileS, CONF>(p, s);
   else if (small_tiles(p.N, p.V)) st = launch_stats<TileS2, TileS2, CONF>(p, s);
-  else if (p.N <= 128 && p.V >= 32768) st = launch_stats<TileM, TileR, CONF>(p, s);
+  else if (p.N <= 128) st = launch_stats<TileM, TileR, CONF>(p, s);
   else st = launch_stats<TileL, TileR, CONF>(p, s);
   if (st != PDLLM_OK) return st;
   hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)(parts > 256 ? p.N : (p.N + 3) / 4)), dim3(256), 0, s, p.part, p.part_idx, p.xlab,
