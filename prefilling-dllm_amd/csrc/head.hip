@@ -458,21 +458,16 @@ struct GradParams {
 // grad_h of a piece: acc[split][row][c] (+)= sum over the split's entries of d[row][v] w[v][c].  Few rows: the tile holds all of them
 // and behind them the remainders' rows, whose results a lane has beside the others.
 template <class T, bool FEW>
-__device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int id, char* lds) {
+__device__ __forceinline__ void head_grad_h_tile(const GradParams& p, int c0, long r0, int split, char* lds) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
-  const int mt = __builtin_amdgcn_readfirstlane(id % p.m_tiles);
-  const int nt = __builtin_amdgcn_readfirstlane((id / p.m_tiles) % p.n_tiles);
-  const int split = __builtin_amdgcn_readfirstlane(id / (p.m_tiles * p.n_tiles));
   const unsigned lds_base = (unsigned)(size_t)lds;
   const long k0 = split * p.k_per;
   long kn = p.vp - k0;
   kn = kn < 0 ? 0 : (kn < p.k_per ? kn : p.k_per);  // (a last, shorter piece may leave a split without entries)
   constexpr int SK = KB / 2;  // entries per stage
   const int steps = (int)((kn + SK - 1) / SK);
-  const int c0 = mt * T::TM;
-  const long r0 = (long)nt * T::TN;
   const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
   LoadKS<T::LA, T::TM> la;
   la.init(p.w + k0 * p.w_stride + 2 * c0, p.w_stride, kn, cols, wave, lane);
@@ -529,16 +524,12 @@ __global__ __launch_bounds__(256) void head_grad_h_join_kernel(const float* __re
 
 // grad_w, the rows of a piece: gw[v][c] = sum over rows r of d[r][v] hz[r][c]
 template <class T>
-__device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, char* lds) {
+__device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int c0, long v0, char* lds) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int mt = __builtin_amdgcn_readfirstlane(id % p.w_tiles);
-  const int nt = __builtin_amdgcn_readfirstlane(id / p.w_tiles);
   const unsigned lds_base = (unsigned)(size_t)lds;
   constexpr int SK = KB / 2;  // rows per stage
   const int steps = (int)((p.N + SK - 1) / SK);
-  const int c0 = mt * T::TM;
-  const long v0 = (long)nt * T::TN;
   const unsigned cols = 2u * (unsigned)(p.D - c0 < T::TM ? p.D - c0 : T::TM);
   LoadKS<T::LA, T::TM> la;
   la.init(p.hz + 2 * c0, 2L * p.D, p.N, cols, wave, lane);
@@ -560,14 +551,30 @@ __device__ __forceinline__ void head_grad_w_tile(const GradParams& p, int id, ch
 // The small tiles (80 KB of LDS, at most 128 registers) leave room for two workgroups on a compute unit, which hide each other's
 // start and end: with few rows a tile of grad_w is a few stages and then 32 KB of results.
 // 4096 rows x 32768 entries x 3584: 1454 us, 1.32 PFLOP/s, bound as the statistics are.
-template <class TH, class TW>
+// The last strip of up to half a tile's columns takes tiles of half the width (TN): the gradient of 1000 rows x 50021 entries x 1032 364
+// instead of 370 us, of 600 x 60000 x 520 190 instead of 196.
+template <class TH, class TW, class TN>
 __global__ __launch_bounds__(TW::THREADS, TW::MT * TW::NT <= 2 ? 4 : 2) void head_grad_kernel(const GradParams p) {
-  static_assert(TH::THREADS == TW::THREADS, "");
+  static_assert(TH::THREADS == TW::THREADS && TN::THREADS == TW::THREADS && TN::LDS <= TW::LDS, "");
+  constexpr bool NARROW = TN::TM < TW::TM;
+  static_assert(!NARROW || (TN::TN == TH::TN && TN::TN == TW::TN && 2 * TN::TM == TH::TM && TH::TM == TW::TM), "");
   __shared__ __attribute__((aligned(1024))) char lds[TH::LDS > TW::LDS ? TH::LDS : TW::LDS];
 #ifdef __HIP_DEVICE_COMPILE__  // (the host compiler cannot resolve the calls: their lambdas hold buffer descriptors)
   const int n_h = p.m_tiles * p.n_tiles * p.splits;
-  if ((int)blockIdx.x < n_h) head_grad_h_tile<TH, false>(p, xcd_remap(blockIdx.x, n_h), lds);
-  else head_grad_w_tile<TW>(p, xcd_remap(blockIdx.x - n_h, gridDim.x - n_h), lds);
+  if ((int)blockIdx.x < n_h) {
+    const int id = xcd_remap(blockIdx.x, n_h);
+    const int c0 = __builtin_amdgcn_readfirstlane(id % p.m_tiles) * TH::TM;
+    const long r0 = (long)__builtin_amdgcn_readfirstlane((id / p.m_tiles) % p.n_tiles) * TH::TN;
+    const int split = __builtin_amdgcn_readfirstlane(id / (p.m_tiles * p.n_tiles));
+    if (NARROW && p.D - c0 <= TN::TM) head_grad_h_tile<TN, false>(p, c0, r0, split, lds);
+    else head_grad_h_tile<TH, false>(p, c0, r0, split, lds);
+  } else {
+    const int id = xcd_remap(blockIdx.x - n_h, gridDim.x - n_h);
+    const int c0 = __builtin_amdgcn_readfirstlane(id % p.w_tiles) * TW::TM;
+    const long v0 = (long)__builtin_amdgcn_readfirstlane(id / p.w_tiles) * TW::TN;
+    if (NARROW && p.D - c0 <= TN::TM) head_grad_w_tile<TN>(p, c0, v0, lds);
+    else head_grad_w_tile<TW>(p, c0, v0, lds);
+  }
 #endif
 }
 
@@ -632,13 +639,17 @@ __device__ __forceinline__ void head_grad_w_few(const GradParams& p, long id) {
 // Bound by the weight read and its gradient written: 32 rows x 126464 x 4096 485 us, 4.3 TB/s (a copy of 2 GiB reaches 4.9); with
 // tiles of 128 x 128 through LDS for grad_w, two stages and 32 KB of results each, 600 to 710 us.
 template <int NT>
-__global__ __launch_bounds__(512, 4) void head_grad_few_kernel(const GradParams p) {
+__global__ __launch_bounds__(512, NT == 2 ? 4 : 2) void head_grad_few_kernel(const GradParams p) {
   typedef Tile<1, NT, 8, 1, 2> T;
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS];
 #ifdef __HIP_DEVICE_COMPILE__
   const int n_h = p.m_tiles * p.splits;
-  if ((int)blockIdx.x < n_h) head_grad_h_tile<T, true>(p, xcd_remap(blockIdx.x, n_h), lds);
-  else head_grad_w_few<NT>(p, 8L * xcd_remap(blockIdx.x - n_h, gridDim.x - n_h) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  if ((int)blockIdx.x < n_h) {
+    const int id = xcd_remap(blockIdx.x, n_h);
+    head_grad_h_tile<T, true>(p, __builtin_amdgcn_readfirstlane(id % p.m_tiles) * T::TM, 0, __builtin_amdgcn_readfirstlane(id / p.m_tiles), lds);
+    return;
+  }
+  head_grad_w_few<NT>(p, 8L * xcd_remap(blockIdx.x - n_h, gridDim.x - n_h) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 #endif
 }
 
@@ -781,6 +792,7 @@ int launch_dlogits(HeadParams& p, hipStream_t s) {
 }
 
 using TileH = Tile<4, 2, 2, 4, 2>;  // grad_h, grad_w: 256 columns x 256 rows or entries
+using TileN = Tile<2, 2, 2, 4, 2>;   // 128 columns x 256: the last strip
 using TileH2 = Tile<1, 2, 8, 1, 2>;  // grad_h of small problems: 256 columns x 64 rows
 using TileW2 = Tile<1, 2, 4, 2, 2>;  // grad_w of small problems: 128 columns x 128 entries
 
@@ -905,7 +917,7 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     q.gw = static_cast<__bf16*>(grad_weight);
     q.gw_stride = grad_weight_stride;
     if (tiles > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((head_grad_kernel<TileH, TileH>), dim3((unsigned)tiles), dim3(TileH::THREADS), 0, s, q);
+    hipLaunchKernelGGL((head_grad_kernel<TileH, TileH, TileN>), dim3((unsigned)tiles), dim3(TileH::THREADS), 0, s, q);
     return launch_status();
   }
   GradPlan g;
@@ -969,8 +981,8 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     const dim3 blocks((unsigned)grid), threads(512);
     if (g.np == 32) hipLaunchKernelGGL(head_grad_few_kernel<2>, blocks, threads, 0, s, q);
     else if (g.np == 64) hipLaunchKernelGGL(head_grad_few_kernel<4>, blocks, threads, 0, s, q);
-    else if (g.small) hipLaunchKernelGGL((head_grad_kernel<TileH2, TileW2>), blocks, threads, 0, s, q);
-    else hipLaunchKernelGGL((head_grad_kernel<TileH, TileH>), blocks, threads, 0, s, q);
+    else if (g.small) hipLaunchKernelGGL((head_grad_kernel<TileH2, TileW2, TileW2>), blocks, threads, 0, s, q);
+    else hipLaunchKernelGGL((head_grad_kernel<TileH, TileH, TileN>), blocks, threads, 0, s, q);
     if ((st = launch_status()) != PDLLM_OK) return st;
   }
   if (g.direct) return PDLLM_OK;
