@@ -683,12 +683,16 @@ int64_t stats_ws(long n, long v, bool conf) { return (int64_t)stat_parts(n, v) *
 
 // The grid over n_voc_tiles x N rows: whole tiles of T; pieces of TS where an almost empty last round of the 256 compute units becomes
 // one round of them (784 tiles of 1000 rows x 50021 entries x 3584: 335 us in four rounds, 297 in three and one of pieces; x 1032 127
-// and 114; 594 tiles of 128 rows x 152064 x 3584: 222 and 215), and for up to 128 rows behind the last whole column.
+// and 114; 594 tiles of 128 rows x 152064 x 3584: 222 and 215).  Up to 128 rows behind the last whole column are pieces too (2051
+// rows x 126464 x 4096: 1793 us as a column of whole tiles, 1654 so; 640 x 50021 x 3584: 255 and 237); beside a single column, where
+// reading the weight again counts, up to 64 and only if it stays in the last-level cache (300 x 50000 x 2048: 96 and 81; but 290 x
+// 152064 x 3584 461 and 511, 384 x 152064 x 3584 467 and 575).
 template <class T, class TS>
 long head_grid(HeadParams& p) {
   constexpr int Q = T::TN / TS::TN;
   const long rest = p.N % T::TN;
-  const bool cut_rest = Q > 1 && rest > 0 && rest <= T::TN / 2;
+  const bool again = p.N >= 2 * T::TN || (long)p.n_voc_tiles * T::TM * 2 * p.D <= (256L << 20);
+  const bool cut_rest = Q > 1 && rest > 0 && again && rest <= (p.N >= 2 * T::TN ? T::TN / 2 : T::TN / 4);
   p.n_tok_tiles = (int)(p.N / T::TN + (rest > 0 && !cut_rest));
   p.rest_cols = cut_rest ? (int)((rest + TS::TN - 1) / TS::TN) : 0;
   const long whole = (long)p.n_voc_tiles * p.n_tok_tiles, last = whole % 256;

@@ -77,7 +77,9 @@ SHAPES = [(1, 1, 8), (1, 300, 64), (5, 1000, 520), (31, 127, 72), (32, 129, 64),
           (20, 1024, 520), (20, 1030, 520), (256, 2000, 264), (257, 2001, 264), (200, 20000, 72),
           # just more than 32 tiles of 256 x 256; the large tiles of the gradient, ragged in every direction
           (1025, 1700, 72), (300, 25001, 264), (257, 50100, 72), (300, 25001, 384),
-          (300, 25001, 392)]
+          (300, 25001, 392),
+          # rows behind the last whole column: in pieces or as a column of their own
+          (384, 17000, 64), (600, 17000, 64), (700, 9000, 72)]
 
 
 @pytest.mark.parametrize("n,v,d", SHAPES)
