@@ -102,7 +102,8 @@ __device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
 }
 
 // A tile of logits and its statistics per row: a lane's own values first (their maximum, then the sum of exp(x - max)), the other
-// three lanes of the row, the other waves of the row.
+// three lanes of the row, the other waves of the row.  Groups of up to 64 entries, whatever the tile: equal rows have equal
+// statistics in tiles and in pieces of them, so that a tie between rows stays one.
 template <class T, bool CONF>
 __device__ __forceinline__ void head_stats_tile(const HeadParams& p, int vt, long row0, char* lds) {
   Acc<T> acc;
@@ -121,6 +122,8 @@ __device__ __forceinline__ void head_stats_tile(const HeadParams& p, int vt, lon
 #pragma unroll
           for (int j = 0; j < 2 * T::NT; ++j) acc.v[i][j][e] = -INFINITY;
   }
+  constexpr int GROUPS = T::MT > 2 ? T::MT / 2 : 1, BLOCKS = 2 * T::MT / GROUPS;
+  static_assert(sizeof(Stat) * T::WM * GROUPS * T::TN <= T::LDS, "");
   __syncthreads();  // the tile's operands are done with: their place takes the statistics
 #pragma unroll
   for (int j = 0; j < 2 * T::NT; ++j) {
@@ -144,42 +147,42 @@ __device__ __forceinline__ void head_stats_tile(const HeadParams& p, int vt, lon
         if (mine) p.xlab[row] = x;
       }
     }
-    float m = -INFINITY;
-    int idx = 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < 2 * T::MT; ++i)
+    for (int q = 0; q < GROUPS; ++q) {
+      float m = -INFINITY;
+      int idx = 0x7fffffff;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = acc.v[i][j][e];
-        if constexpr (CONF) {
-          if (x > m) idx = 16 * i + e;
+      for (int i = q * BLOCKS; i < (q + 1) * BLOCKS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = acc.v[i][j][e];
+          if constexpr (CONF) {
+            if (x > m) idx = 16 * i + e;
+          }
+          m = fmaxf(m, x);
         }
-        m = fmaxf(m, x);
+      // the other lane groups hold the other entries of the same row
+      const float m1 = fmaxf(m, __shfl_xor(m, 16, 64));
+      const float top = half_swap_max(m1);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float s = 0.f;
+#pragma unroll
+      for (int i = q * BLOCKS; i < (q + 1) * BLOCKS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc.v[i][j][e] - ref) * kLog2eH);
+      s += __shfl_xor(s, 16, 64);
+      s = half_swap_sum(s);
+      if constexpr (CONF) {
+        // the lowest position among the lanes that hold the maximum
+        int cand = m == top && idx != 0x7fffffff ? idx + 4 * g : 0x7fffffff;
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+          const int other = __shfl_xor(cand, o, 64);
+          cand = other < cand ? other : cand;
+        }
+        idx = cand == 0x7fffffff ? cand : cand + (int)vw;
       }
-    // the other lane groups hold the other entries of the same row
-    const float m1 = fmaxf(m, __shfl_xor(m, 16, 64));
-    const float top = half_swap_max(m1);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2 * T::MT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc.v[i][j][e] - ref) * kLog2eH);
-    s += __shfl_xor(s, 16, 64);
-    s = half_swap_sum(s);
-    if constexpr (CONF) {
-      // the lowest position among the lanes that hold the maximum
-      int cand = m == top && idx != 0x7fffffff ? idx + 4 * g : 0x7fffffff;
-#pragma unroll
-      for (int o = 16; o < 64; o <<= 1) {
-        const int other = __shfl_xor(cand, o, 64);
-        cand = other < cand ? other : cand;
-      }
-      idx = cand == 0x7fffffff ? cand : cand + (int)vw;
-    }
-    if (g == 0) {
-      Stat* sh = reinterpret_cast<Stat*>(lds) + wm * T::TN + col;
-      *sh = {top, s, idx};
+      if (g == 0) reinterpret_cast<Stat*>(lds)[(wm * GROUPS + q) * T::TN + col] = {top, s, idx};
     }
   }
   __syncthreads();
@@ -189,7 +192,7 @@ __device__ __forceinline__ void head_stats_tile(const HeadParams& p, int vt, lon
     const Stat* sh = reinterpret_cast<const Stat*>(lds) + c;
     Stat a = sh[0];
 #pragma unroll
-    for (int q = 1; q < T::WM; ++q) a = stat_join(a, sh[q * T::TN]);
+    for (int q = 1; q < T::WM * GROUPS; ++q) a = stat_join(a, sh[q * T::TN]);
     const long o = row * p.parts + vt;
     p.part[o] = make_float2(a.m, a.s);
     if constexpr (CONF) p.part_idx[o] = a.idx;

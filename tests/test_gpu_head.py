@@ -201,6 +201,21 @@ def test_extreme_logits(dev):
     assert bool(torch.isnan(conf[2])) and 0 <= int(tok[2]) < 300
 
 
+@pytest.mark.parametrize("n,v", [(1030, 17200), (130, 3000), (384, 17000), (60, 700)])
+def test_equal_rows_have_equal_results(dev, n, v):
+    """The same state in every row, in whole tiles, in pieces of them and behind them: the same bits, so that the most confident
+    position of a block is its first one."""
+    from prefilling_dllm_amd import ops
+    h, w, labels, _ = make(dev, n, v, 72, seed=n)
+    h, labels = h[:1].expand(n, 72).contiguous(), labels[:1].expand(n).contiguous()
+    logp, lse = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
+    assert bool((logp == logp[0]).all()) and bool((lse == lse[0]).all())
+    ids = torch.full((2, n // 2), v - 1, dtype=torch.int64, device=dev)
+    conf, tok, tr, _ = ops.head_denoise_unmask(h, w, ids, v - 1, 2.0, shift=True)
+    assert bool((conf == conf[0]).all()) and bool((tok == tok[0]).all())
+    assert bool(tr[:, 0].all()) and int(tr.sum()) == 2
+
+
 def test_views_and_strides(dev):
     """States that are columns of a wider tensor, a weight that is a slice of rows, int32 labels, a single row of any stride."""
     from prefilling_dllm_amd import ops
