@@ -1089,10 +1089,10 @@ def head_denoise_unmask(hidden: torch.Tensor, weight: torch.Tensor, block_ids: t
     last = _head_last(last_hidden, n_seqs, dim, dev)
     conf = torch.empty(n, dtype=torch.float32, device=dev)
     tok = torch.empty(n, dtype=torch.int64, device=dev)
-    transfer = torch.empty((n_seqs, block_len), dtype=torch.uint8, device=dev)
+    transfer = torch.empty((n_seqs, block_len), dtype=torch.bool, device=dev)
     left = torch.empty(n_seqs, dtype=torch.int32, device=dev)
     if n == 0:
-        return conf, tok, transfer.view(torch.bool), left.zero_()
+        return conf, tok, transfer, left.zero_()
     with _on(dev):
         ws = _scratch(dev, int(lib.pdllm_head_workspace_bytes(n, vocab)))
         check(lib.pdllm_head_denoise_unmask(_ptr(hidden), _row_stride(hidden), _ptr(last), dim, weight.data_ptr(),
@@ -1100,7 +1100,7 @@ def head_denoise_unmask(hidden: torch.Tensor, weight: torch.Tensor, block_ids: t
                                             block_ids.data_ptr(), int(mask_token_id), float(threshold), _ptr(ws), ws.numel(),
                                             conf.data_ptr(), tok.data_ptr(), transfer.data_ptr(), left.data_ptr(),
                                             _stream(hidden)), "head_denoise_unmask")
-    return conf, tok, transfer.view(torch.bool), left
+    return conf, tok, transfer, left
 
 
 # ----------------------------------------------------------------------------------------
