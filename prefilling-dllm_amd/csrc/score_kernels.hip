@@ -23,13 +23,14 @@ struct RowStat {
   long idx;  // first index of the maximum
 };
 
+// what the exponents are taken relative to: with nothing but -inf (or NaN) so far 0, so that -inf counts 0 and a NaN stays one
+__device__ __forceinline__ float stat_ref(float m) { return m == -INFINITY ? 0.f : m; }
+
 __device__ __forceinline__ void stat_merge(RowStat& a, const RowStat& b) {
   // maximum with lowest-index tie-break, sums rescaled to the common maximum
   const bool b_wins = (b.m > a.m) || (b.m == a.m && b.idx < a.idx);
-  const float mm = fmaxf(a.m, b.m);
-  const float sa = (a.m == -INFINITY) ? 0.f : a.s * __builtin_amdgcn_exp2f((a.m - mm) * kLog2e);
-  const float sb = (b.m == -INFINITY) ? 0.f : b.s * __builtin_amdgcn_exp2f((b.m - mm) * kLog2e);
-  a.s = sa + sb;
+  const float mm = fmaxf(a.m, b.m), ref = stat_ref(mm);
+  a.s = a.s * __builtin_amdgcn_exp2f((a.m - ref) * kLog2e) + b.s * __builtin_amdgcn_exp2f((b.m - ref) * kLog2e);
   a.m = mm;
   if (b_wins) a.idx = b.idx;
 }
@@ -40,7 +41,7 @@ __device__ __forceinline__ void stat_push(RowStat& st, float x, long i) {
     st.m = x;
     st.idx = i;
   } else {
-    st.s += __builtin_amdgcn_exp2f((x - st.m) * kLog2e);
+    st.s += __builtin_amdgcn_exp2f((x - stat_ref(st.m)) * kLog2e);
   }
 }
 
@@ -90,12 +91,11 @@ __global__ __launch_bounds__(256) void vocab_partial_kernel(
           st.m = vm;
           st.idx = i + vi;
         }
-        if (st.m > -INFINITY) {
-          float acc = 0.f;
+        const float ref = stat_ref(st.m);
+        float acc = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) acc += __builtin_amdgcn_exp2f((x[k] - st.m) * kLog2e);
-          st.s += acc;
-        }
+        for (int k = 0; k < 8; ++k) acc += __builtin_amdgcn_exp2f((x[k] - ref) * kLog2e);
+        st.s += acc;
       } else {
         for (long j = i; j < end; ++j)
           stat_push(st, bf16_bits_to_f32(__builtin_bit_cast(unsigned short, src[j])), j);
@@ -143,6 +143,11 @@ __device__ __forceinline__ RowStat row_stat(const float* __restrict__ part_m, co
   return a;
 }
 
+// max softmax probability; NaN for a row whose logits are all -inf (its sum is 0), as softmax has it
+__device__ __forceinline__ float stat_conf(const RowStat& a) { return a.s == 0.f ? NAN : 1.f / a.s; }
+// position of the maximum; 0 for a row without one (nothing but -inf and NaN)
+__device__ __forceinline__ long stat_token(const RowStat& a) { return a.idx == 0x7fffffffffffffffL ? 0 : a.idx; }
+
 // log-softmax of the label: logits[row, label] - logsumexp(row); labels outside the vocabulary give -inf
 __device__ __forceinline__ float label_logprob(const RowStat& a, const __bf16* __restrict__ logits,
                                                long logits_stride, const long* __restrict__ labels, long vocab,
@@ -164,8 +169,8 @@ __global__ __launch_bounds__(64) void vocab_final_kernel(
   if (mode == 0) {
     out_f[row] = label_logprob(a, logits, logits_stride, labels, vocab, row);
   } else {
-    out_f[row] = 1.f / a.s;
-    out_i[row] = a.idx;
+    out_f[row] = stat_conf(a);
+    out_i[row] = stat_token(a);
   }
 }
 
@@ -262,9 +267,9 @@ __global__ __launch_bounds__(64) void unmask_tail_kernel(
   int n_masked = 0;
   for (long i = lane; i < block_len; i += 64) {
     const RowStat a = row_stat(part_m, part_s, part_idx, nsplit, base + i);
-    const float c = 1.f / a.s;
+    const float c = stat_conf(a);
     conf_out[base + i] = c;
-    token_out[base + i] = a.idx;
+    token_out[base + i] = stat_token(a);
     if (block_ids[base + i] == mask_token_id) {
       ++n_masked;
       if (c > best || besti == 0x7fffffffffffffffL) { best = c; besti = i; }
