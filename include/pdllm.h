@@ -383,7 +383,7 @@ int pdllm_conf_argmax(const void* logits, int64_t logits_stride, const void* las
 
 /* Replaces the transfer rule of decode_from_pd_record (ENG:2146-2157) without host
  * syncs: per block b over the positions with block_ids == mask_token_id, transfer the
- * most confident one (lowest index on ties) and every one with conf >= threshold;
+ * most confident one (lowest index on ties, a NaN above every number as in torch.topk) and every one with conf >= threshold;
  * writes the tokens into block_ids in place, transfer_out[b, i] in {0,1} and
  * n_masked_left[b] = masked positions remaining after the update. */
 int pdllm_threshold_unmask(const float* conf, const int64_t* token, int64_t* block_ids,

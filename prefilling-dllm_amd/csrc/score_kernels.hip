@@ -260,41 +260,18 @@ __global__ __launch_bounds__(64) void unmask_tail_kernel(
     float* __restrict__ conf_out, long* __restrict__ token_out, uint8_t* __restrict__ transfer,
     int* __restrict__ n_left) {
   const long b = blockIdx.x;
-  const int lane = threadIdx.x;
   const long base = b * block_len;
-  float best = -INFINITY;
-  long besti = 0x7fffffffffffffffL;
-  int n_masked = 0;
-  for (long i = lane; i < block_len; i += 64) {
+  BestMasked best;
+  for (long i = threadIdx.x; i < block_len; i += 64) {
     const RowStat a = row_stat(part_m, part_s, part_idx, nsplit, base + i);
     const float c = stat_conf(a);
     conf_out[base + i] = c;
     token_out[base + i] = stat_token(a);
-    if (block_ids[base + i] == mask_token_id) {
-      ++n_masked;
-      if (c > best || besti == 0x7fffffffffffffffL) { best = c; besti = i; }
-    }
+    if (block_ids[base + i] == mask_token_id) best_push(best, c, i);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ob = __shfl_xor(best, o, 64);
-    const long oi = __shfl_xor(besti, o, 64);
-    n_masked += __shfl_xor(n_masked, o, 64);
-    const bool o_valid = oi != 0x7fffffffffffffffL, s_valid = besti != 0x7fffffffffffffffL;
-    const bool take = o_valid && (!s_valid || ob > best || (ob == best && oi < besti));
-    if (take) { best = ob; besti = oi; }
-  }
-  int moved = 0;
-  for (long i = lane; i < block_len; i += 64) {
-    // this lane wrote conf_out / token_out of position i itself
-    const bool masked = block_ids[base + i] == mask_token_id;
-    const bool t = masked && (i == besti || conf_out[base + i] >= threshold);
-    transfer[base + i] = t ? 1 : 0;
-    if (t) { block_ids[base + i] = token_out[base + i]; ++moved; }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) moved += __shfl_xor(moved, o, 64);
-  if (lane == 0 && n_left) n_left[b] = n_masked - moved;
+  best_join_wave(best);
+  // (a lane reads back the conf_out / token_out that it wrote itself)
+  unmask_transfer(best, conf_out, token_out, block_ids, b, base, block_len, mask_token_id, threshold, transfer, n_left);
 }
 
 // one wave per block of the batch
