@@ -314,7 +314,8 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2* __restrict
       float lp = -(fmaxf(d, 0.f) + log1pf(expf(-fabsf(d))));
       if (x == INFINITY || (x == -INFINITY && L == -INFINITY)) lp = NAN;
       out[row] = lp;
-      if (lse_out) lse_out[row] = x - lp;
+      // log(exp L + exp x), not x - logp: that loses digits where the label is far below the others, and is NaN at -inf
+      if (lse_out) lse_out[row] = L == x ? L + 0.69314718f : fmaxf(L, x) + log1pf(expf(-fabsf(d)));
     }
   }
 }
