@@ -453,7 +453,8 @@ int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_stride, const vo
 /* pdllm_conf_argmax (ENG:1647-1681) from the states: row i of block b uses state row b*block_len + i, or with shift the
  * row before it: for i = 0 last_hidden[b] (the state in front of the block; the block's own row 0 when NULL).
  * Confidence = max softmax probability, token = first index of the largest logit (of the fp32 logits: where two round
- * to the same bf16 value, pdllm_conf_argmax sees a tie and this call does not).  A row whose logits are all NaN: token 0. */
+ * to the same bf16 value, pdllm_conf_argmax sees a tie and this call does not).  A row whose logits hold a NaN or +inf, or are
+ * all -inf, has confidence NaN; one of NaN and -inf alone token 0. */
 int pdllm_head_conf_argmax(const void* hidden, int64_t hidden_stride, const void* last_hidden, int64_t last_hidden_stride,
                            const void* weight, int64_t weight_stride, int64_t n_seqs, int64_t block_len, int64_t vocab,
                            int32_t dim, int32_t shift, void* workspace, int64_t workspace_bytes, float* conf_out,

@@ -287,8 +287,8 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2* __restrict
   const bool writes = at == 0 && row < N;
   if constexpr (CONF) {
     if (writes) {
-      out[row] = 1.f / a.s;
-      token_out[row] = a.idx == 0x7fffffff ? 0 : a.idx;  // a row of NaN alone has no maximum
+      out[row] = a.s == 0.f ? NAN : 1.f / a.s;           // every entry -inf: as softmax has it
+      token_out[row] = a.idx == 0x7fffffff ? 0 : a.idx;  // a row of -inf and NaN alone has no maximum
     }
     if (!un.block_ids) return;
     // the workgroup that is done last makes the step's transfers (its order decides nothing: it sees every row's result)
