@@ -109,24 +109,26 @@ def select_chunks_from_logits(logits: torch.Tensor, labels: torch.Tensor, topk_c
     return ops.chunk_select_from_logits(logits, labels, k, mean=mean, sorted_ascending=True)
 
 
-# ------------------------------------------------------------------------------------------
-# token keep set (ENG:903-927)
-# ------------------------------------------------------------------------------------------
-
-def select_chunks_from_hidden(hidden: torch.Tensor, head_weight: torch.Tensor, labels: torch.Tensor, topk_chunks: int,
+def select_chunks_from_hidden(hidden: torch.Tensor, head_weight: torch.Tensor, labels: torch.Tensor, topk_chunks: Optional[int],
                               mean: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """Chunk scoring and ranking from the hidden states in front of the head (ENG:1098-1152 and 1199-1204), without the
     logits: hidden [n_chunks, n_labels, dim] bf16, head_weight [vocab, dim] bf16, labels [n_chunks, n_labels] -> (scores fp32
-    [n_chunks], the indices of the best min(topk_chunks, n_chunks), ascending)."""
+    [n_chunks], the indices of the best min(topk_chunks, n_chunks), ascending; of all chunks where topk_chunks is None or not
+    positive, as in select_chunks_from_logits)."""
     if hidden.dim() != 3 or tuple(labels.shape) != tuple(hidden.shape[:2]):
         raise ValueError("hidden must be [n_chunks, n_labels, dim], labels [n_chunks, n_labels]")
     c, j, dim = hidden.shape
-    if c == 0 or j == 0 or topk_chunks <= 0:
-        raise ValueError("chunks, labels and topk_chunks must be positive")
+    if c == 0 or j == 0:
+        raise ValueError("there must be chunks and labels")
+    k = c if int(topk_chunks or 0) <= 0 else min(int(topk_chunks), c)
     logp = ops.head_selfinfo_logprob(hidden.reshape(c * j, dim), head_weight, labels.reshape(c * j))
     scores = ops.chunk_score_reduce(logp, c, mean)
-    return scores, ops.topk_lowest_index(scores, topk_chunks)
+    return scores, ops.topk_lowest_index(scores, k)
 
+
+# ------------------------------------------------------------------------------------------
+# token keep set (ENG:903-927)
+# ------------------------------------------------------------------------------------------
 
 def select_positions_from_token_scores(token_scores: torch.Tensor, *, capacity: int, chunk_len: int,
                                        keep_high: bool = True, force_keep_first: bool = True) -> torch.Tensor:
