@@ -425,7 +425,9 @@ int pdllm_denoise_unmask_static(const void* logits, int64_t logits_stride, const
 /* The head's logits z = hidden weight^T are formed tile by tile on the matrix cores (bf16 products, fp32 sums) and
  * reduced where they are made; they are not rounded to bf16.  hidden [n_rows, dim], weight [vocab, dim] bf16, row strides in
  * elements and multiples of 8, bases 16-byte aligned, dim a multiple of 8 (at most 2^20), weight_stride below 2^22,
- * n_rows <= 2^24, vocab <= 2^30.  workspace: 16-byte aligned. */
+ * n_rows <= 2^24, vocab <= 2^30; PDLLM_ERR_UNSUPPORTED where a launch would hold 2^32 work-items or more (some 8 million tiles of
+ * 256 x 256 logits; 2^34 elements of grad_hidden).  workspace: 16-byte aligned, asked for with the sizes of the call (fewer rows may
+ * need more). */
 int64_t pdllm_head_workspace_bytes(int64_t n_rows, int64_t vocab);
 
 /* pdllm_selfinfo_logprob (ENG:1148-1152) from the states: logp[r] = log softmax(z[r])[label[r]], computed as
@@ -484,7 +486,8 @@ int pdllm_fp8_quantize_blocks(const void* w, int64_t w_stride, int64_t n_rows, i
 /* out[i, j] = sum_b x_scale[i, b] * weight_scale[j / 128, b] * sum_{c in block b} x[i, c] * weight[j, c] for e4m3 x [m, k]
  * and weight [n, k] (rows contiguous, strides in elements, multiples of 16, below 2^23; bases 16-byte aligned), blocks of 128
  * columns, any fp32 scales; out bf16.  Sums in fp32, apart from those of eight neighbouring products, which the matrix
- * instruction adds on a grid of 2^-13 of the largest of them.  k a multiple of 16 (at most 2^20), m <= 2^24, n <= 2^30.  Same bits on every call. */
+ * instruction adds on a grid of 2^-13 of the largest of them.  k a multiple of 16 (at most 2^20), m <= 2^24, n <= 2^30 (as above:
+ * PDLLM_ERR_UNSUPPORTED beyond 2^32 work-items, here some 8 million tiles, up to 32 rows 2^28 features).  Same bits on every call. */
 int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_scale, int64_t x_scale_row_stride,
                      int64_t x_scale_block_stride, const void* weight, int64_t weight_stride, const float* weight_scale,
                      int64_t weight_scale_row_stride, int64_t weight_scale_block_stride, int64_t m, int64_t n, int32_t k,

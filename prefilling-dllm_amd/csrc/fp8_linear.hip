@@ -598,7 +598,7 @@ int launch_fp8(Fp8Params& p, hipStream_t s) {
   p.m_tiles = (int)((p.N + T::TM - 1) / T::TM);
   p.n_tiles = (int)((p.M + T::TN - 1) / T::TN);
   const long grid = (long)p.m_tiles * p.n_tiles;
-  if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+  if (!launch_fits(grid, T::THREADS)) return PDLLM_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(fp8_linear_kernel<T>, dim3((unsigned)grid), dim3(T::THREADS), 0, s, p);
   return launch_status();
 }
@@ -616,7 +616,9 @@ bool stream_wide(const Fp8Params& p) { return (p.N + 31) / 32 * ((p.M + 31) / 32
 template <int TT, bool BF>
 int launch_stream(Fp8Params& p, hipStream_t s) {
   const bool wide = stream_wide(p);
-  const dim3 grid((unsigned)((p.N + (wide ? 31 : 15)) / (wide ? 32 : 16)), (unsigned)((p.M + 16 * TT - 1) / (16 * TT)));
+  const long columns = (p.N + (wide ? 31 : 15)) / (wide ? 32 : 16), rows = (p.M + 16 * TT - 1) / (16 * TT);
+  if (!launch_fits(columns, 512) || rows > 65535) return PDLLM_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)columns, (unsigned)rows);
   if (wide) hipLaunchKernelGGL((fp8_stream_kernel<32, TT, BF>), grid, dim3(512), 0, s, p);
   else hipLaunchKernelGGL((fp8_stream_kernel<16, TT, BF>), grid, dim3(512), 0, s, p);
   return launch_status();
@@ -687,7 +689,7 @@ extern "C" int pdllm_fp8_quantize_rows(const void* x, int64_t x_stride, int64_t 
   const int st = check_quantize(x, x_stride, n_rows, k, q, q_stride, scale, scale_row_stride, scale_block_stride);
   if (st != PDLLM_OK || n_rows == 0) return st;
   const int groups = (k + 2047) / 2048;
-  if (n_rows * groups > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+  if (!launch_fits(n_rows * groups, 256)) return PDLLM_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(fp8_quantize_rows_kernel, dim3((unsigned)(n_rows * groups)), dim3(256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const char*>(x), 2L * x_stride, groups, k,
                      static_cast<char*>(q), (long)q_stride, scale, (long)scale_row_stride, (long)scale_block_stride);
@@ -700,7 +702,7 @@ extern "C" int pdllm_fp8_quantize_blocks(const void* w, int64_t w_stride, int64_
   const int st = check_quantize(w, w_stride, n_rows, k, q, q_stride, scale, scale_row_stride, scale_block_stride);
   if (st != PDLLM_OK || n_rows == 0) return st;
   const long blocks = (n_rows + 127) / 128 * ((k + 127) / 128);
-  if (blocks > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+  if (!launch_fits(blocks, 256)) return PDLLM_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(fp8_quantize_blocks_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const char*>(w), 2L * w_stride, (long)n_rows, k, static_cast<char*>(q), (long)q_stride, scale,
                      (long)scale_row_stride, (long)scale_block_stride);

@@ -704,7 +704,7 @@ long head_grid(HeadParams& p) {
   const long grid = full + Q * (whole - full) + (long)p.n_voc_tiles * p.rest_cols;
   p.n_full = (int)full;
   p.n_cut = (int)(Q * (whole - full));
-  return grid <= 0x7fffffffL ? grid : -1;
+  return launch_fits(grid, T::THREADS) ? grid : -1;
 }
 
 template <class T, class TS, bool CONF>
@@ -735,13 +735,15 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
   p.part_idx = reinterpret_cast<int*>(next);
   p.xlab = next;
   if (un.block_ids) p.joined = un.joined = p.part_idx + (long)parts * p.N;
+  const long joins = parts > 256 ? p.N : (p.N + 3) / 4;
+  if (!launch_fits(joins, 256)) return PDLLM_ERR_UNSUPPORTED;
   int st;
   if (p.N <= 32) st = launch_stats<TileS, TileS, CONF>(p, s);
   else if (small_tiles(p.N, p.V)) st = launch_stats<TileS2, TileS2, CONF>(p, s);
   else if (p.N <= 128) st = launch_stats<TileM, TileR, CONF>(p, s);
   else st = launch_stats<TileL, TileR, CONF>(p, s);
   if (st != PDLLM_OK) return st;
-  hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)(parts > 256 ? p.N : (p.N + 3) / 4)), dim3(256), 0, s, p.part, p.part_idx, p.xlab,
+  hipLaunchKernelGGL(head_join_kernel<CONF>, dim3((unsigned)joins), dim3(256), 0, s, p.part, p.part_idx, p.xlab,
                      p.labels, parts, p.N, p.V, out, lse_out, token_out, un);
   return launch_status();
 }
@@ -924,12 +926,14 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     q.vp = vocab;
     q.gw = static_cast<__bf16*>(grad_weight);
     q.gw_stride = grad_weight_stride;
-    if (tiles > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+    if (!launch_fits(tiles, TileH::THREADS)) return PDLLM_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((head_grad_kernel<TileH, TileH, TileN>), dim3((unsigned)tiles), dim3(TileH::THREADS), 0, s, q);
     return launch_status();
   }
   GradPlan g;
   if (!workspace || (uintptr_t)workspace % 256 || !plan_grad(n_rows, vocab, dim, workspace_bytes, g)) return PDLLM_ERR_WORKSPACE;
+  const long joins = (n_rows * (dim / 4) + 255) / 256;
+  if (!g.direct && !launch_fits(joins, 256)) return PDLLM_ERR_UNSUPPORTED;
   char* ws = static_cast<char*>(workspace);
   HeadParams p = {};
   p.w = static_cast<const char*>(weight);
@@ -985,7 +989,7 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     q.v_per = q.w_tiles * ((vp + 511) / 512) >= 4096 ? 512 : 64;
     const long n_w = few ? (q.w_tiles * ((vp + q.v_per - 1) / q.v_per) + 7) / 8 : q.w_tiles * ((vp + tw - 1) / tw);
     const long grid = (long)q.m_tiles * q.n_tiles * q.splits + n_w;
-    if (grid > 0x7fffffffL) return PDLLM_ERR_UNSUPPORTED;
+    if (!launch_fits(grid, 512)) return PDLLM_ERR_UNSUPPORTED;
     const dim3 blocks((unsigned)grid), threads(512);
     if (g.np == 32) hipLaunchKernelGGL(head_grad_few_kernel<2>, blocks, threads, 0, s, q);
     else if (g.np == 64) hipLaunchKernelGGL(head_grad_few_kernel<4>, blocks, threads, 0, s, q);
@@ -994,8 +998,7 @@ extern "C" int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_strid
     if ((st = launch_status()) != PDLLM_OK) return st;
   }
   if (g.direct) return PDLLM_OK;
-  const long quads = n_rows * (dim / 4);
-  hipLaunchKernelGGL(head_grad_h_join_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, q.acc, g.splits, n_rows,
-                     dim, static_cast<__bf16*>(grad_hidden), grad_hidden_stride);
+  hipLaunchKernelGGL(head_grad_h_join_kernel, dim3((unsigned)joins), dim3(256), 0, s, q.acc, g.splits, n_rows, dim,
+                     static_cast<__bf16*>(grad_hidden), grad_hidden_stride);
   return launch_status();
 }

@@ -55,6 +55,9 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// A launch holds fewer than 2^32 work-items in one direction.
+inline bool launch_fits(long workgroups, int threads) { return workgroups <= 0xffffffffL / threads; }
+
 inline int launch_status() {
   return hipGetLastError() == hipSuccess ? PDLLM_OK : PDLLM_ERR_LAUNCH;
 }
