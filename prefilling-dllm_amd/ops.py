@@ -997,19 +997,51 @@ def _head_rows(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, device) -
     return t.to(dtype).contiguous()
 
 
-def head_selfinfo_logprob(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, return_lse: bool = False):
-    """log_softmax(hidden @ weight.T)[row, label[row]] in fp32 from bf16 states [rows, dim] and the head's bf16 weight
-    [vocab, dim]: selfinfo_logprob (fastdllm_engine.py:1148-1152) without the logits in memory.  Labels outside the
-    vocabulary give -inf.  return_lse: also log sum exp of each row, which head_selfinfo_grad takes."""
+def _head_selfinfo(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, with_lse: bool):
     n, vocab, dim = _head_args(hidden, weight)
     labels = _head_rows(labels, n, torch.int64, "labels", hidden.device)
     logp = torch.empty(n, dtype=torch.float32, device=hidden.device)
-    lse = torch.empty_like(logp) if return_lse else None
+    lse = torch.empty_like(logp) if with_lse else None
     with _on(hidden.device):
         ws = _scratch(hidden.device, int(lib.pdllm_head_workspace_bytes(n, vocab)))
         check(lib.pdllm_head_selfinfo_logprob(_ptr(hidden), _row_stride(hidden), weight.data_ptr(), _row_stride(weight),
                                               labels.data_ptr(), n, vocab, dim, _ptr(ws), 0 if ws is None else ws.numel(),
                                               logp.data_ptr(), _ptr(lse), _stream(hidden)), "head_selfinfo_logprob")
+    return logp, lse
+
+
+class _HeadSelfinfo(torch.autograd.Function):
+    """head_selfinfo_logprob with head_selfinfo_grad as its backward pass."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, labels):
+        logp, lse = _head_selfinfo(hidden, weight, labels, True)
+        ctx.save_for_backward(hidden, weight, labels, logp, lse)
+        ctx.set_materialize_grads(False)
+        return logp, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logp, grad_lse):
+        if grad_lse is not None:
+            raise NotImplementedError("head_selfinfo_logprob has no gradient through its log sum exp")
+        if grad_logp is None:
+            return None, None, None
+        hidden, weight, labels, logp, lse = ctx.saved_tensors
+        grads = head_selfinfo_grad(hidden, weight, labels, logp, lse, grad_logp)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,)
+
+
+def head_selfinfo_logprob(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, return_lse: bool = False):
+    """log_softmax(hidden @ weight.T)[row, label[row]] in fp32 from bf16 states [rows, dim] and the head's bf16 weight
+    [vocab, dim]: selfinfo_logprob (fastdllm_engine.py:1148-1152) without the logits in memory.  Labels outside the
+    vocabulary give -inf.  return_lse: also log sum exp of each row, which head_selfinfo_grad takes.  Where hidden or weight
+    requires a gradient and gradients are recorded, the log-probabilities carry it (by head_selfinfo_grad, once
+    differentiable); log sum exp carries none, a backward pass through it raises."""
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        logp, lse = _HeadSelfinfo.apply(hidden, weight, labels)
+    else:
+        logp, lse = _head_selfinfo(hidden, weight, labels, return_lse)
     return (logp, lse) if return_lse else logp
 
 

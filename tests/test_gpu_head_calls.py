@@ -23,3 +23,56 @@ def test_chunk_selection_takes_what_the_selection_from_logits_takes(dev, topk):
     assert torch.equal(idx.cpu(), want)
     logits = (h.float() @ w.float().t()).to(torch.bfloat16).view(c, j, v)
     assert engine_ops.select_chunks_from_logits(logits, labels.view(c, j), topk)[1].shape == idx.shape
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 300, 64), (40, 900, 72), (130, 3000, 264)])
+def test_logprob_carries_its_gradient(dev, n, v, d):
+    """A loss on the log-probabilities, with terms beside it, gives the states and the weight the gradient of head_selfinfo_grad."""
+    from prefilling_dllm_amd import ops
+    h, w, labels = make(dev, n, v, d, seed=n)
+    if n > 4:
+        labels[2] = -100
+    rows = labels >= 0
+    g = torch.randn(n, generator=torch.Generator().manual_seed(n)).to(dev)
+    logp, lse = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
+    assert not logp.requires_grad
+    want = ops.head_selfinfo_grad(h, w, labels, logp, lse, g)
+    x, head = h.clone().requires_grad_(), torch.nn.Parameter(w.clone())
+    # (a row without a label is -inf: left out of the sum, its gradient is 0)
+    for with_lse in (False, True):
+        got = ops.head_selfinfo_logprob(x, head, labels, return_lse=with_lse)
+        got = got[0] if with_lse else got
+        assert torch.equal(got.detach(), logp)
+        a, b = torch.autograd.grad((got[rows] * g[rows]).sum() + 0 * x.float().sum(), (x, head))
+        g0 = torch.where(rows, g, torch.zeros_like(g))
+        ref = ops.head_selfinfo_grad(h, w, labels, logp, lse, g0)
+        assert torch.equal(a, ref[0]) and torch.equal(b, ref[1]) and torch.equal(a, want[0])
+    # one of the two alone, a mean, gradients that add up over two backward passes
+    ops.head_selfinfo_logprob(h, head, labels)[rows].mean().backward()
+    once = head.grad.clone()
+    ops.head_selfinfo_logprob(h, head, labels)[rows].mean().backward()
+    assert torch.equal(head.grad, once + once) and bool((once != 0).any())
+    with torch.no_grad():
+        assert not ops.head_selfinfo_logprob(x, head, labels).requires_grad
+    # states from a layer in front
+    proj = torch.eye(d, dtype=torch.bfloat16, device=dev).requires_grad_()
+    ops.head_selfinfo_logprob(h @ proj, w, labels)[rows].sum().backward()
+    assert proj.grad.shape == (d, d) and bool(torch.isfinite(proj.grad).all()) and bool((proj.grad != 0).any())
+
+
+def test_what_the_gradient_does_not_cover_raises(dev):
+    from prefilling_dllm_amd import ops
+    h, w, labels = make(dev, 12, 300, 64)
+    h.requires_grad_()
+    logp, lse = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
+    with pytest.raises(NotImplementedError, match="log sum exp"):
+        (logp.sum() + lse.square().sum()).backward()
+    logp = ops.head_selfinfo_logprob(h, w, labels)
+    (g,) = torch.autograd.grad(logp.sum(), h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    logp = ops.head_selfinfo_logprob(h, w, labels)
+    with torch.no_grad():
+        h.mul_(2)
+    with pytest.raises(RuntimeError, match="modified"):
+        logp.sum().backward()
