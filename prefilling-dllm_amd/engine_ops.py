@@ -123,7 +123,8 @@ def select_chunks_from_hidden(hidden: torch.Tensor, head_weight: torch.Tensor, l
     k = c if int(topk_chunks or 0) <= 0 else min(int(topk_chunks), c)
     logp = ops.head_selfinfo_logprob(hidden.reshape(c * j, dim), head_weight, labels.reshape(c * j))
     scores = ops.chunk_score_reduce(logp, c, mean)
-    return scores, ops.topk_lowest_index(scores, k)
+    with ops._on(scores.device):
+        return scores, ops.topk_lowest_index(scores, k)
 
 
 # ------------------------------------------------------------------------------------------

@@ -551,8 +551,9 @@ def chunk_score_reduce(logp: torch.Tensor, n_chunks: int, mean: bool = True) -> 
         raise ValueError("logp must be fp32 with the same number of labels, one at least, for every chunk")
     logp = logp.reshape(-1).contiguous()
     out = torch.empty(n_chunks, dtype=torch.float32, device=logp.device)
-    check(lib.pdllm_chunk_score_reduce(logp.data_ptr(), n_chunks, logp.numel() // n_chunks, 1 if mean else 0,
-                                       out.data_ptr(), _stream(logp)), "chunk_score_reduce")
+    with _on(logp.device):
+        check(lib.pdllm_chunk_score_reduce(logp.data_ptr(), n_chunks, logp.numel() // n_chunks, 1 if mean else 0,
+                                           out.data_ptr(), _stream(logp)), "chunk_score_reduce")
     return out
 
 

@@ -76,3 +76,46 @@ def test_what_the_gradient_does_not_cover_raises(dev):
         h.mul_(2)
     with pytest.raises(RuntimeError, match="modified"):
         logp.sum().backward()
+
+
+def test_every_launch_is_made_on_the_device_of_its_tensors(dev, monkeypatch):
+    """The device of the tensors is current around every launch of these functions (here told by the guard that makes it so)."""
+    import contextlib
+
+    from prefilling_dllm_amd import engine_ops, ops
+    inside, launches = [0], []
+
+    @contextlib.contextmanager
+    def guard(device):
+        assert device == dev
+        inside[0] += 1
+        yield
+        inside[0] -= 1
+
+    class Library:
+        def __getattr__(self, name):
+            f = getattr(real, name)
+            if name.endswith("_bytes"):
+                return f
+
+            def call(*a):
+                launches.append((name, inside[0] > 0))
+                return f(*a)
+            return call
+
+    real = ops.lib
+    monkeypatch.setattr(ops, "lib", Library())
+    monkeypatch.setattr(ops, "_on", guard)
+    h, w, labels = make(dev, 12, 300, 64)
+    ids = torch.full((3, 4), 7, dtype=torch.int64, device=dev)
+    engine_ops.select_chunks_from_hidden(h.view(3, 4, 64), w, labels.view(3, 4), 2)
+    engine_ops.denoise_unmask_step_from_hidden(h, w, ids, mask_token_id=7, threshold=0.9)
+    logp, lse = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
+    ops.head_selfinfo_grad(h, w, labels, logp, lse, logp)
+    ops.head_conf_argmax(h, w, 4)
+    ops.chunk_score_reduce(logp, 3)
+    wq, ws = ops.quantize_fp8_blocks(w)
+    xq, xs = ops.quantize_fp8_rows(h)
+    ops.fp8_block_linear(h, wq, ws)
+    ops.fp8_block_linear(xq, wq, ws, x_scale=xs)
+    assert len(launches) == 12 and [name for name, on in launches if not on] == []
