@@ -1130,9 +1130,9 @@ def head_denoise_unmask(hidden: torch.Tensor, weight: torch.Tensor, block_ids: t
         ws = _scratch(dev, int(lib.pdllm_head_workspace_bytes(n, vocab)))
         check(lib.pdllm_head_denoise_unmask(_ptr(hidden), _row_stride(hidden), _ptr(last), dim, weight.data_ptr(),
                                             _row_stride(weight), n_seqs, block_len, vocab, dim, 1 if shift else 0,
-                                            block_ids.data_ptr(), int(mask_token_id), float(threshold), _ptr(ws), ws.numel(),
-                                            conf.data_ptr(), tok.data_ptr(), transfer.data_ptr(), left.data_ptr(),
-                                            _stream(hidden)), "head_denoise_unmask")
+                                            block_ids.data_ptr(), int(mask_token_id), float(threshold), _ptr(ws),
+                                            0 if ws is None else ws.numel(), conf.data_ptr(), tok.data_ptr(),
+                                            transfer.data_ptr(), left.data_ptr(), _stream(hidden)), "head_denoise_unmask")
     return conf, tok, transfer, left
 
 

@@ -119,3 +119,17 @@ def test_every_launch_is_made_on_the_device_of_its_tensors(dev, monkeypatch):
     ops.fp8_block_linear(h, wq, ws)
     ops.fp8_block_linear(xq, wq, ws, x_scale=xs)
     assert len(launches) == 12 and [name for name, on in launches if not on] == []
+
+
+def test_a_head_without_entries_is_refused(dev):
+    """By every call with the library's own error, and block_ids stay as they were."""
+    from prefilling_dllm_amd import ops
+    h, w, labels = make(dev, 8, 300, 64)
+    none = w[:0]
+    ids = torch.full((2, 4), 7, dtype=torch.int64, device=dev)
+    for call in (lambda: ops.head_selfinfo_logprob(h, none, labels), lambda: ops.head_conf_argmax(h, none, 4),
+                 lambda: ops.head_denoise_unmask(h, none, ids, 7, 0.9),
+                 lambda: ops.head_selfinfo_grad(h, none, labels, *(labels.float() for _ in range(3)))):
+        with pytest.raises(ValueError, match="SHAPE"):
+            call()
+    assert bool((ids == 7).all())
