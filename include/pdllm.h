@@ -456,7 +456,7 @@ int pdllm_head_selfinfo_grad(const void* hidden, int64_t hidden_stride, const vo
  * row before it: for i = 0 last_hidden[b] (the state in front of the block; the block's own row 0 when NULL).
  * Confidence = max softmax probability, token = first index of the largest logit (of the fp32 logits: where two round
  * to the same bf16 value, pdllm_conf_argmax sees a tie and this call does not).  A row whose logits hold a NaN or +inf, or are
- * all -inf, has confidence NaN; one of NaN and -inf alone token 0. */
+ * all -inf, has confidence NaN; one of NaN and -inf alone token 0 (a row whose state holds an infinity may count as that). */
 int pdllm_head_conf_argmax(const void* hidden, int64_t hidden_stride, const void* last_hidden, int64_t last_hidden_stride,
                            const void* weight, int64_t weight_stride, int64_t n_seqs, int64_t block_len, int64_t vocab,
                            int32_t dim, int32_t shift, void* workspace, int64_t workspace_bytes, float* conf_out,
@@ -485,9 +485,11 @@ int pdllm_fp8_quantize_blocks(const void* w, int64_t w_stride, int64_t n_rows, i
 
 /* out[i, j] = sum_b x_scale[i, b] * weight_scale[j / 128, b] * sum_{c in block b} x[i, c] * weight[j, c] for e4m3 x [m, k]
  * and weight [n, k] (rows contiguous, strides in elements, multiples of 16, below 2^23; bases 16-byte aligned), blocks of 128
- * columns, any fp32 scales; out bf16.  Sums in fp32, apart from those of eight neighbouring products, which the matrix
- * instruction adds on a grid of 2^-13 of the largest of them.  k a multiple of 16 (at most 2^20), m <= 2^24, n <= 2^30 (as above:
- * PDLLM_ERR_UNSUPPORTED beyond 2^32 work-items, here some 8 million tiles, up to 32 rows 2^28 features).  Same bits on every call. */
+ * columns, fp32 scales whose products x_scale * weight_scale are normal numbers or zero (they are formed in fp32 first: one that
+ * overflows makes zeros NaN, one below 2^-126 loses digits), x_scale_row_stride below 2^22; out bf16, not overlapping the
+ * operands.  Sums in fp32, apart from those of eight neighbouring products, which the matrix instruction adds on a grid of
+ * 2^-13 of the largest of them.  k a multiple of 16 (at most 2^20), m <= 2^24, n <= 2^30 (as above: PDLLM_ERR_UNSUPPORTED
+ * from 2^32 work-items on, here some 8 million tiles, up to 32 rows 2^28 features).  Same bits on every call. */
 int pdllm_fp8_linear(const void* x, int64_t x_stride, const float* x_scale, int64_t x_scale_row_stride,
                      int64_t x_scale_block_stride, const void* weight, int64_t weight_stride, const float* weight_scale,
                      int64_t weight_scale_row_stride, int64_t weight_scale_block_stride, int64_t m, int64_t n, int32_t k,

@@ -230,7 +230,8 @@ struct Acc {
 // The 16x16x32 instruction, not 32x32x16: the large products here run at the card's power limit, and with operands of normally
 // distributed values out of registers the one sustains 2050 TFLOP/s, the other 1340 to 1640 (zeros: 2450 and 1810 to 2210).
 // 4096 rows x 152064 x 3584, scores only: 3.69 ms with 32x32x16, 3.47 ms so; 3.29 ms with the instructions of a turn in a fixed
-// order in which neighbours share an operand; 3.16 ms with reads and copies between them and no branch in the loop.
+// order in which neighbours share an operand; 3.16 ms with reads and copies between them and no branch in the loop (3.14 to 3.21 ms since
+// the statistics behind it are taken in groups of 64 entries).
 template <class T, bool AKS, bool BKS, class Issue>
 __device__ __forceinline__ void mainloop_bf16(Acc<T>& acc, int steps, unsigned lds_base, Issue&& issue) {
   const int lane = threadIdx.x & 63;

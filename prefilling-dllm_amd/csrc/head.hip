@@ -222,8 +222,8 @@ __device__ __forceinline__ void head_dispatch(const HeadParams& p, F&& tile) {
 }
 
 // Bound by the weight's bytes up to 128 rows (152064 x 3584: 182 us for 32 rows, 6.0 TB/s; 214 us for 128, 5.1 TB/s), above by the
-// matrix instructions and the card's power (4096 rows: 3.16 ms, 1.41 PFLOP/s with the statistics; a library product of the same
-// size, which writes its logits, 3.07 ms).  Forming one tile after the other in 256 workgroups, the next tile's copies in flight during
+// matrix instructions and the card's power (4096 rows: 3.14 to 3.21 ms, 1.39 to 1.42 PFLOP/s with the statistics; a library product
+// of the same size, which writes its logits, 3.11 ms).  Between, by what whole tiles leave empty: 290, 384 and 512 rows take 460 to 470 us.  Forming one tile after the other in 256 workgroups, the next tile's copies in flight during
 // the statistics, was no faster (4096 rows 3.31 ms, 1000 rows x 50021 x 1032 116.7 us for 117.4).
 template <class T, class TS, bool CONF>
 __global__ __launch_bounds__(T::THREADS, 2) void head_stats_kernel(const HeadParams p) {
@@ -325,8 +325,9 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float2* __restrict
 // ------------------------------------------------------------------------------------------------------------------
 
 // One piece of the softmax gradient, rounded to bf16 as the operand of the two products behind it (each entry off by at
-// most 2^-8 of itself).  For few rows, where few entries make up a result and the products wait for memory anyway, the
-// remainder of the rounding is kept beside it.  4096 rows x 32768 entries x 3584: 740 us, 1.30 PFLOP/s.
+// most 2^-8 of itself: the gradients' errors are 0.0024 of their norm, the result's own rounding to bf16 alone 0.0017).  For few rows,
+// where few entries make up a result and the products wait for memory anyway, the remainder of the rounding is kept beside it;
+// above it would be a second product of the same size.  4096 rows x 32768 entries x 3584: 740 us, 1.30 PFLOP/s.
 template <class T, bool FEW>
 __device__ __forceinline__ void head_dlogits_tile(const HeadParams& p, int vt, long row0, char* lds) {
   Acc<T> acc;
@@ -749,7 +750,9 @@ int stats(HeadParams& p, void* workspace, int64_t workspace_bytes, float* out, f
 }
 
 // ---- gradient: sizes of the workspace's regions ----
-constexpr long kPieceBytes = 256L << 20;  // the piece of d the products read back stays within the last-level cache
+// A piece of d, so that the workspace does not grow with the vocabulary; as large as the last-level cache, though not alone in it (of
+// 4096 rows the products of a piece also read 235 MB of weight and write as much).  Smaller pieces mean more launches.
+constexpr long kPieceBytes = 256L << 20;
 constexpr long kMaxPiece = 1L << 21;        // 256 rows of a piece lie within 31-bit offsets
 constexpr int kFewRows = 64;                // up to here the remainders are carried
 

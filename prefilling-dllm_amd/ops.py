@@ -1179,7 +1179,7 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
                      x_scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x @ weight.T for an e4m3 weight [n, k] with fp32 scales [ceil(n / 128), ceil(k / 128)], one for each block of
     128 x 128.  x: bf16 [m, k] (quantised on the way as quantize_fp8_rows does), or e4m3 [m, k] with its scales x_scale
-    [m, ceil(k / 128)].  The result is bf16 [m, n]; `out` receives it where given."""
+    [m, ceil(k / 128)].  The result is bf16 [m, n]; `out`, which must not overlap the operands, receives it where given."""
     _need_cuda(x, weight, weight_scale, x_scale, out)
     dev = x.device
     for t in (weight, weight_scale, x_scale, out):
