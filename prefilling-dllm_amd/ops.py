@@ -1028,6 +1028,9 @@ class _HeadSelfinfo(torch.autograd.Function):
             raise NotImplementedError("head_selfinfo_logprob has no gradient through its log sum exp")
         if grad_logp is None:
             return None, None, None
+        if torch.cuda.is_current_stream_capturing():
+            # (an eager graph of the same leaves that still lives would take the capture to its own stream and end the process)
+            raise RuntimeError("head_selfinfo_logprob: its backward pass is not captured into a graph; call head_selfinfo_grad there")
         hidden, weight, labels, logp, lse = ctx.saved_tensors
         grads = head_selfinfo_grad(hidden, weight, labels, logp, lse, grad_logp)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,)
@@ -1038,7 +1041,8 @@ def head_selfinfo_logprob(hidden: torch.Tensor, weight: torch.Tensor, labels: to
     [vocab, dim]: selfinfo_logprob (fastdllm_engine.py:1148-1152) without the logits in memory.  Labels outside the
     vocabulary give -inf.  return_lse: also log sum exp of each row, which head_selfinfo_grad takes.  Where hidden or weight
     requires a gradient and gradients are recorded, the log-probabilities carry it (by head_selfinfo_grad, once
-    differentiable); log sum exp carries none, a backward pass through it raises."""
+    differentiable); log sum exp carries none, a backward pass through it raises.  A captured backward pass raises too: what is
+    captured calls head_selfinfo_grad itself."""
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         logp, lse = _HeadSelfinfo.apply(hidden, weight, labels)
     else:

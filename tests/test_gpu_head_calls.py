@@ -133,3 +133,37 @@ def test_a_head_without_entries_is_refused(dev):
         with pytest.raises(ValueError, match="SHAPE"):
             call()
     assert bool((ids == 7).all())
+
+
+def test_a_backward_pass_under_capture_is_refused(dev, monkeypatch):
+    """(told by the question that the backward pass asks, not by a capture)"""
+    from prefilling_dllm_amd import ops
+    h, w, labels = make(dev, 12, 300, 64)
+    h.requires_grad_()
+    logp = ops.head_selfinfo_logprob(h, w, labels)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="call head_selfinfo_grad"):
+        logp.sum().backward()
+    assert h.grad is None
+
+
+def test_scores_of_a_parameter_replay_from_a_graph(dev):
+    """A weight that requires a gradient, scored under capture: the values of the eager call at every replay."""
+    from prefilling_dllm_amd import ops
+    h, w, labels = make(dev, 40, 900, 72)
+    head = torch.nn.Parameter(w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.head_selfinfo_logprob(h, head, labels)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = ops.head_selfinfo_logprob(h, head, labels, return_lse=True)
+    for seed in (1, 2, 3):
+        h.copy_(make(dev, 40, 900, 72, seed=seed)[0])
+        want = ops.head_selfinfo_logprob(h, w, labels, return_lse=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.detach(), want[0]) and torch.equal(lse.detach(), want[1])
+        torch.randn(1 << 20, device=dev).sum().item()
